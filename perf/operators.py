@@ -333,11 +333,12 @@ def _own_serve(state):
 
 def _own(state):
     from brainstorm_amd._C import router as c_router
-    from brainstorm_amd.jit import grouped_linear_fp8
 
     case = state["case"]
     kind = case["kind"]
     if kind == "fp8":
+        from brainstorm_amd.jit import grouped_linear_fp8
+
         return {"out": grouped_linear_fp8(state["x"], state["w"], state["ws"], state["loads"], bias=state["bias"],
                                           activation=case["activation"])}
     if kind == "gate":
