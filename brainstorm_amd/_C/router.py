@@ -667,13 +667,16 @@ combine_with_src_indices = combine_with_indices_and_loads
 # the dispatched buffer, 0 = dropped) and ``row_entries [P]`` (1-based entry ``t*k + j + 1`` of
 # every dispatched row, 0 = padding; for ``k == 1`` these are the row tags of dispatch).
 def gate_topk(score: torch.Tensor, top_k: int, softmax: bool = False,
-              hot_mask: bool = False) -> Tuple[torch.Tensor, ...]:
+              hot_mask: bool = False, *, differentiable: bool = False) -> Tuple[torch.Tensor, ...]:
     """``(path_ids, weights[, hot_mask])``: the ``top_k`` largest scores of every row in the order
     of ``torch.topk`` (NaN highest, lowest path among equals) and their weights -- the scores as
     fp32, or with ``softmax`` their softmax over the row (the router probabilities of
     benchmark/switch_moe/switch_transformer.py:240-253).  One kernel for what the reference does
-    with ``softmax`` + ``topk`` / ``argmax`` + ``zeros`` + ``scatter_`` (protocol/topk.py:26-31)."""
-    return _lib.native().gate_topk(score, top_k, softmax, hot_mask)
+    with ``softmax`` + ``topk`` / ``argmax`` + ``zeros`` + ``scatter_`` (protocol/topk.py:26-31).
+
+    ``differentiable=True``: the weights carry the gradient of ``score`` (one kernel as well); ids and mask have none.
+    Without it the result is cut off from autograd, as those of the other ops are."""
+    return _lib.native().gate_topk(score, top_k, softmax, hot_mask, differentiable)
 
 
 def route_by_path(
@@ -697,27 +700,40 @@ def route_by_path(
 
 def dispatch_by_rows(in_data: torch.Tensor, row_entries: torch.Tensor, k: int,
                      weights: Optional[torch.Tensor] = None,
-                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     out: Optional[torch.Tensor] = None, *, seat_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``out[r] = in_data[(row_entries[r]-1) // k]`` (times ``weights.view(-1)[row_entries[r]-1]``,
     rounded once), zero rows where ``row_entries[r] == 0``: what ``dispatch_with_indices_and_loads``
-    (router.cc:131-273) writes for the same route, every row written by the kernel."""
-    return _lib.native().dispatch_by_rows(in_data, row_entries, int(k), weights, out)
+    (router.cc:131-273) writes for the same route, every row written by the kernel.
+
+    With ``seat_rows`` (``[cells, k]``, the inverse of ``row_entries`` that ``route_by_path`` gives beside it) the result
+    carries the gradients of ``in_data`` and ``weights``: a cell's is the sum over its rows, an entry's the dot product of
+    its cell and its row's gradient, in one launch and without atomics.  At most eight entries per cell; no gradients of
+    these gradients."""
+    return _lib.native().dispatch_by_rows(in_data, row_entries, int(k), weights, out, seat_rows)
 
 
 def combine_by_rows(in_data: torch.Tensor, path_ids: torch.Tensor, seat_rows: torch.Tensor,
                     weights: Optional[torch.Tensor] = None, out_data: Optional[torch.Tensor] = None,
                     out_dtype: Optional[torch.dtype] = None, *,
-                    gates: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    gates: Optional[torch.Tensor] = None,
+                    row_entries: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``out[t] = sum_j weights[t,j] * in_data[seat_rows[t,j]-1]`` over the entries that own a row,
     in ascending path id, fp32 from zero: the result of ``combine_with_indices_and_loads``
     (router.cc:372-473) for the same route, bit for bit.  With ``out_data`` the result is
     written in place and cells without a row keep their value (the residual convention).
     ``gates`` (the ``[cells, paths]`` matrix, any data type) gives the weights instead:
-    ``gates[t, path_ids[t,j]]``; it has a column for every path id (the ids are not read back to check it)."""
+    ``gates[t, path_ids[t,j]]``; it has a column for every path id (the ids are not read back to check it).
+
+    With ``row_entries`` (``[rows]``, the inverse of ``seat_rows`` that ``route_by_path`` gives beside it) the result
+    carries the gradients of ``in_data`` and ``weights`` (or ``gates``), made in one launch: a row's is its entry's weight
+    times the gradient of its cell, zero for rows without an entry; an entry's is the dot product of the two, zero without
+    a row.  It is then a tensor of its own: ``out_data`` is not taken.  No gradients of these gradients."""
     if gates is not None and weights is not None:
         raise RuntimeError("weights or gates, not both")
+    if row_entries is not None and gates is not None:
+        weights, gates = torch.gather(gates, 1, path_ids.long()).to(torch.float32), None
     if gates is not None and not (gates.dtype in _DT and gates.dim() == 2 and gates.size(0) == path_ids.size(0)
                                   and gates.numel() < 1 << 31):
         # what the kernel does not read in place: other types (fp64 gates), more rows than cells
         weights, gates = torch.gather(gates, 1, path_ids.long()).to(torch.float32), None
-    return _lib.native().combine_by_rows(in_data, path_ids, seat_rows, weights, out_data, out_dtype, gates)
+    return _lib.native().combine_by_rows(in_data, path_ids, seat_rows, weights, out_data, out_dtype, gates, row_entries)

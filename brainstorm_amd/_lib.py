@@ -153,6 +153,19 @@ SIGNATURES = {
         [_c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int,
          _c_int, _c_int, _c_ptr],
     ),
+    "brt_hip_gate_topk_grad": (
+        _c_int,
+        [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr],
+    ),
+    "brt_hip_dispatch_by_rows_grad": (
+        _c_int,
+        [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr],
+    ),
+    "brt_hip_combine_by_rows_grad": (
+        _c_int,
+        [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+         _c_ptr],
+    ),
     "brt_hip_grouped_gemm_f32in_supported": (_c_int, [_c_int] * 6),
     "brt_hip_grouped_gemm_f32in": (
         _c_int,

@@ -24,8 +24,11 @@
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <atomic>
 #include <chrono>
 #include <stdexcept>
 #include <string>
@@ -36,8 +39,12 @@
 namespace {
 
 using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
 
-unsigned long long g_calls = 0;  // calls into the library that queued device work (under the GIL)
+// calls into the library that queued device work (gradients are queued by autograd's threads, which do not hold the GIL)
+std::atomic<unsigned long long> g_calls{0};
 
 // An error with the Python type it is raised as.
 struct Raised : std::runtime_error {
@@ -142,6 +149,35 @@ at::DimVector rows_of(const Tensor& t, int64_t rows) {  // the shape of t with a
   return s;
 }
 
+// ---- gradients ---------------------------------------------------------------------------------------
+std::optional<Tensor> optional(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+bool tracked(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
+
+// The gradients of a backward pass for its `n` arguments, filled in by `fill` (what stays undefined has none).  The kernels
+// behind them have no gradients of their own: where a graph of the backward pass is asked for, differentiating it towards
+// anything that they were made `from` raises.
+template <typename F>
+variable_list differentiable_once(size_t n, const variable_list& grads, const variable_list& saved, F&& fill) {
+  variable_list made(n);
+  const bool graph = at::GradMode::is_enabled();
+  {
+    const at::NoGradGuard no_grad;
+    fill(made);
+  }
+  if (!graph) return made;
+  variable_list from(1);
+  for (const variable_list* list : {&grads, &saved})
+    for (const Tensor& t : *list)
+      if (t.defined() && t.requires_grad()) from.push_back(t);
+  for (Tensor& t : made)
+    if (t.defined()) {
+      from[0] = t.detach().set_requires_grad(true);
+      auto error = std::make_shared<torch::autograd::DelayedError>("the gradients of the routing ops are not differentiable again", from.size());
+      t = (*error)(variable_list(from))[0];
+    }
+  return made;
+}
+
 // The menu of capacities of an index generation.
 struct Caps {
   Tensor t;
@@ -176,17 +212,45 @@ PyObject* topk_hot_mask(const Args& a) {
   return wrap(mask);
 }
 
-PyObject* gate_topk(const Args& a) {  // score, k, softmax, hot_mask
-  const long k = a.integer(1);
-  const Tensor score = scores(a.tensor(0), k);
+variable_list gate(const Tensor& given, int64_t k, bool softmax, bool hot_mask) {
+  const Tensor score = scores(given, k);
   const c10::DeviceGuard guard(score.device());
   const int64_t T = score.size(0);
   Tensor ids = empty({T, k}, at::kInt, score), weights = empty({T, k}, at::kFloat, score), mask;
-  if (a.flag(3)) mask = empty(score.sizes(), at::kInt, score);
-  if (k > 0 || mask.defined())
-    check(brt_hip_gate_topk(ptr(score), T, score.size(1), k, code_of(score.scalar_type()), a.flag(2), iptr(ids),
+  if (hot_mask) mask = empty(score.sizes(), at::kInt, score);
+  if (k > 0 || hot_mask)
+    check(brt_hip_gate_topk(ptr(score), T, score.size(1), k, code_of(score.scalar_type()), softmax, iptr(ids),
                             fptr(weights), iptr(mask), stream_of(score)));
-  return mask.defined() ? tuple(wrap(ids), wrap(weights), wrap(mask)) : tuple(wrap(ids), wrap(weights));
+  return hot_mask ? variable_list{ids, weights, mask} : variable_list{ids, weights};
+}
+
+struct GateTopk : Function<GateTopk> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& given, int64_t k, bool softmax, bool hot_mask) {
+    variable_list made = gate(given, k, softmax, hot_mask);
+    ctx->mark_non_differentiable(hot_mask ? variable_list{made[0], made[2]} : variable_list{made[0]});
+    ctx->save_for_backward({given, made[0], made[1]});
+    ctx->saved_data["softmax"] = softmax;
+    return made;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    return differentiable_once(4, grads, saved, [&](variable_list& made) {
+      if (!grads[1].defined()) return;
+      const Tensor score = dense(saved[0]), ids = saved[1], weights = saved[2], grad = dense(grads[1]);
+      const c10::DeviceGuard guard(score.device());
+      made[0] = empty(score.sizes(), score.scalar_type(), score);
+      check(brt_hip_gate_topk_grad(ptr(score), iptr(ids), fptr(weights), fptr(grad), ptr(made[0]), score.size(0), score.size(1),
+                                   ids.size(1), code_of(score.scalar_type()), ctx->saved_data["softmax"].toBool(), stream_of(score)));
+    });
+  }
+};
+
+PyObject* gate_topk(const Args& a) {  // score, k, softmax, hot_mask, differentiable
+  const Tensor score = a.tensor(0);
+  const long k = a.integer(1);
+  const bool softmax = a.flag(2), hot_mask = a.flag(3);
+  const variable_list made = a.flag(4) && tracked(score) ? GateTopk::apply(score, k, softmax, hot_mask) : gate(score, k, softmax, hot_mask);
+  return hot_mask ? tuple(wrap(made[0]), wrap(made[1]), wrap(made[2])) : tuple(wrap(made[0]), wrap(made[1]));
 }
 
 // ---- index generation --------------------------------------------------------------------------------
@@ -598,25 +662,79 @@ Tensor entry_weights(const Tensor& given, int64_t entries) {
   return dense(given);
 }
 
-PyObject* dispatch_by_rows(const Args& a) {  // in_data, row_entries, k, weights, out
-  const Tensor given = a.tensor(0), entries_given = a.tensor(1);
+Tensor rows_of_cells(const Tensor& given, const Tensor& entries_given, int64_t k, const Tensor& weights_given, Tensor out) {
   on_device(given, "in_data"), on_device(entries_given, "row_entries");
   int32(entries_given, "row_entries");
   const int type = data_type(given, "in_data data type");
   const Tensor in = dense(given), entries = dense(entries_given);
-  const int64_t T = in.size(0), cell = T > 0 ? in.numel() / T : 0, P = entries.numel(), k = a.integer(2);
-  const Tensor weights = entry_weights(a.tensor_or_none(3), T * k);
+  const int64_t T = in.size(0), cell = T > 0 ? in.numel() / T : 0, P = entries.numel();
+  const Tensor weights = entry_weights(weights_given, T * k);
   const c10::DeviceGuard guard(in.device());
-  Tensor out = a.tensor_or_none(4);
   if (!out.defined()) out = empty(rows_of(in, P), in.scalar_type(), in);
   else if (out.scalar_type() != in.scalar_type() || !out.is_contiguous() || out.numel() != P * cell || out.device() != in.device())
     runtime_error("out must be a contiguous [rows, *cell_shape] tensor of the input's type");
   check(brt_hip_dispatch_by_rows(ptr(in), ptr(out), fptr(weights), iptr(entries), P, T, k, cell, type, stream_of(in)));
-  return wrap(out);
+  return out;
 }
 
-PyObject* combine_by_rows(const Args& a) {  // in_data, path_ids, seat_rows, weights, out_data, out_dtype, gates
-  const Tensor given = a.tensor(0), ids_given = a.tensor(1), seats_given = a.tensor(2), residual = a.tensor_or_none(4);
+// seat_rows of a differentiable dispatch or combine, or its row_entries: on the device of the rows
+void same_device(const Tensor& t, const Tensor& in, const char* name) {
+  if (t.device() != in.device()) runtime_error(std::string(name) + " is on another device than in_data");
+}
+
+struct DispatchByRows : Function<DispatchByRows> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& in, const std::optional<Tensor>& given, const Tensor& entries, const Tensor& seats,
+                        int64_t k) {
+    const Tensor weights = given.value_or(Tensor());
+    const Tensor out = rows_of_cells(in, entries, k, weights, Tensor());
+    // the cells are kept for the gradient of the weights only
+    ctx->save_for_backward({tracked_weights(weights) ? in : Tensor(), weights, seats});
+    ctx->saved_data["shape"] = in.sizes().vec();
+    return out;
+  }
+  // (grad mode is off in forward: whether the weights need a gradient is all there is to ask)
+  static bool tracked_weights(const Tensor& weights) { return weights.defined() && weights.requires_grad(); }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    return differentiable_once(5, grads, saved, [&](variable_list& made) {
+      if (!grads[0].defined()) return;
+      const Tensor cells = saved[0].defined() ? dense(saved[0]) : Tensor(), weights = saved[1].defined() ? dense(saved[1]) : Tensor();
+      const Tensor seats = dense(saved[2]), grad = dense(grads[0]);
+      const c10::DeviceGuard guard(grad.device());
+      const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+      const int64_t T = seats.size(0), k = seats.size(1), P = grad.size(0);
+      int64_t cell = 1;
+      for (size_t d = 1; d < shape.size(); ++d) cell *= shape[d];
+      if (ctx->needs_input_grad(0)) made[0] = empty(shape, grad.scalar_type(), grad);
+      if (saved[1].defined() && ctx->needs_input_grad(1)) made[1] = empty(saved[1].sizes(), at::kFloat, grad);
+      check(brt_hip_dispatch_by_rows_grad(ptr(grad), ptr(cells), fptr(weights), iptr(seats), ptr(made[0]), fptr(made[1]), T, k, cell, P,
+                                          code_of(grad.scalar_type()), stream_of(grad)));
+    });
+  }
+};
+
+PyObject* dispatch_by_rows(const Args& a) {  // in_data, row_entries, k, weights, out, seat_rows
+  const Tensor in = a.tensor(0), entries = a.tensor(1), weights = a.tensor_or_none(3), out = a.tensor_or_none(4), seats = a.tensor_or_none(5);
+  const int64_t k = a.integer(2);
+  if (!seats.defined()) return wrap(rows_of_cells(in, entries, k, weights, out));
+  on_device(in, "in_data"), on_device(seats, "seat_rows");
+  int32(seats, "seat_rows");
+  same_device(seats, in, "seat_rows"), same_device(entries, in, "row_entries");
+  if (weights.defined()) same_device(weights, in, "weights");
+  if (out.defined()) runtime_error("a differentiable dispatch makes its own result: seat_rows or out, not both");
+  if (seats.dim() != 2 || seats.size(0) != in.size(0) || seats.size(1) != k) runtime_error("seat_rows must be [cells, k]");
+  if (k > 8) not_implemented("more than 8 paths per cell");
+  return wrap(tracked(in) || tracked(weights) ? DispatchByRows::apply(in, optional(weights), entries, seats, k) : rows_of_cells(in, entries, k, weights, Tensor()));
+}
+
+struct CombineOptions {
+  Tensor residual, gates;
+  bool typed = false;  // out_type was given
+  at::ScalarType out_type = at::kFloat;
+};
+Tensor cells_of_rows(const Tensor& given, const Tensor& ids_given, const Tensor& seats_given, const Tensor& weights_given,
+                     const CombineOptions& o) {
+  const Tensor& residual = o.residual;
   on_device(given, "in_data"), on_device(ids_given, "path_ids");
   int32(ids_given, "path_ids");
   on_device(seats_given, "seat_rows");
@@ -627,19 +745,17 @@ PyObject* combine_by_rows(const Args& a) {  // in_data, path_ids, seat_rows, wei
   const Tensor in = dense(given), ids = dense(ids_given), seats = dense(seats_given);
   const int64_t T = ids.size(0), k = ids.size(1), P = in.size(0);
   const int64_t cell = P > 0 ? in.numel() / P : residual.defined() && T > 0 ? residual.numel() / T : 0;
-  const Tensor weights = entry_weights(a.tensor_or_none(3), T * k);
+  const Tensor weights = entry_weights(weights_given, T * k);
   const c10::DeviceGuard guard(in.device());
   Tensor out = residual;
   if (residual.defined()) {
     if (!residual.is_contiguous() || residual.numel() != T * cell) runtime_error("out_data must be a contiguous [cells, ...] tensor");
   } else {
-    at::ScalarType type = in.scalar_type();
-    a.dtype(5, &type);
-    out = empty(rows_of(in, T), type, in);
+    out = empty(rows_of(in, T), o.typed ? o.out_type : in.scalar_type(), in);
   }
   const int out_type = code_of(out.scalar_type());
   if (out_type < 0 || (out_type != in_type && out_type != BRT_F32)) not_implemented("output data type is not supported");
-  Tensor gates = a.tensor_or_none(6);
+  Tensor gates = o.gates;
   if (gates.defined()) {
     on_device(gates, "gates");
     const int gate_type = data_type(gates, "gate data type");
@@ -647,11 +763,60 @@ PyObject* combine_by_rows(const Args& a) {  // in_data, path_ids, seat_rows, wei
     gates = dense(gates);
     check(brt_hip_combine_by_rows_gated(ptr(in), ptr(out), ptr(gates), gate_type, gates.size(1), iptr(ids), iptr(seats), T, k,
                                         cell, P, residual.defined(), in_type, out_type, stream_of(in)));
-    return wrap(out);
+    return out;
   }
   check(brt_hip_combine_by_rows(ptr(in), ptr(out), fptr(weights), iptr(ids), iptr(seats), T, k, cell, P, residual.defined(),
                                 in_type, out_type, stream_of(in)));
-  return wrap(out);
+  return out;
+}
+
+struct CombineByRows : Function<CombineByRows> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& in, const std::optional<Tensor>& given, const Tensor& ids,
+                        const Tensor& seats, const Tensor& entries, at::ScalarType out_type) {
+    const Tensor weights = given.value_or(Tensor());
+    CombineOptions o;
+    o.typed = true, o.out_type = out_type;
+    const Tensor out = cells_of_rows(in, ids, seats, weights, o);
+    // the rows are kept for the gradient of the weights only
+    ctx->save_for_backward({DispatchByRows::tracked_weights(weights) ? in : Tensor(), weights, ids, seats, entries});
+    ctx->saved_data["shape"] = in.sizes().vec();
+    ctx->saved_data["type"] = static_cast<int64_t>(in.scalar_type());
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    return differentiable_once(6, grads, saved, [&](variable_list& made) {
+      if (!grads[0].defined()) return;
+      const Tensor rows = saved[0].defined() ? dense(saved[0]) : Tensor(), weights = saved[1].defined() ? dense(saved[1]) : Tensor();
+      const Tensor ids = dense(saved[2]), seats = dense(saved[3]), entries = dense(saved[4]), grad = dense(grads[0]);
+      const c10::DeviceGuard guard(grad.device());
+      const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+      const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
+      const int64_t T = ids.size(0), k = ids.size(1), P = shape[0];
+      int64_t cell = 1;
+      for (size_t d = 1; d < shape.size(); ++d) cell *= shape[d];
+      if (ctx->needs_input_grad(0)) made[0] = empty(shape, type, grad);
+      if (saved[1].defined() && ctx->needs_input_grad(1)) made[1] = empty(saved[1].sizes(), at::kFloat, grad);
+      check(brt_hip_combine_by_rows_grad(ptr(grad), ptr(rows), fptr(weights), iptr(ids), iptr(seats), iptr(entries), ptr(made[0]),
+                                         fptr(made[1]), T, k, cell, P, code_of(type), code_of(grad.scalar_type()), stream_of(grad)));
+    });
+  }
+};
+
+PyObject* combine_by_rows(const Args& a) {  // in_data, path_ids, seat_rows, weights, out_data, out_dtype, gates, row_entries
+  const Tensor in = a.tensor(0), ids = a.tensor(1), seats = a.tensor(2), weights = a.tensor_or_none(3), entries = a.tensor_or_none(7);
+  CombineOptions o;
+  o.residual = a.tensor_or_none(4), o.gates = a.tensor_or_none(6);
+  o.typed = a.dtype(5, &o.out_type);
+  if (!entries.defined()) return wrap(cells_of_rows(in, ids, seats, weights, o));
+  on_device(in, "in_data"), on_device(entries, "row_entries");
+  int32(entries, "row_entries");
+  same_device(ids, in, "path_ids"), same_device(seats, in, "seat_rows"), same_device(entries, in, "row_entries");
+  if (weights.defined()) same_device(weights, in, "weights");
+  if (o.residual.defined() || o.gates.defined()) runtime_error("a differentiable combine takes neither out_data nor gates beside row_entries");
+  if (in.dim() < 1 || entries.numel() != in.size(0)) runtime_error("row_entries must have one entry for every row");
+  if (!tracked(in) && !tracked(weights)) return wrap(cells_of_rows(in, ids, seats, weights, o));
+  return wrap(CombineByRows::apply(in, optional(weights), ids, seats, entries, o.typed ? o.out_type : in.scalar_type()));
 }
 
 // ---- grouped GEMM ------------------------------------------------------------------------------------
@@ -1012,7 +1177,7 @@ PyObject* one_value(const Args& a) {
   return wrap(at::full({1}, static_cast<int64_t>(a.integer(0)), at::TensorOptions().dtype(at::kInt).device(like.device())));
 }
 
-PyObject* calls(const Args&) { return PyLong_FromUnsignedLongLong(g_calls); }
+PyObject* calls(const Args&) { return PyLong_FromUnsignedLongLong(g_calls.load()); }
 
 template <PyObject* (*FN)(const Args&), int N>
 PyObject* entry(PyObject*, PyObject* const* v, Py_ssize_t n) {
@@ -1033,10 +1198,10 @@ PyObject* entry(PyObject*, PyObject* const* v, Py_ssize_t n) {
 #define BRT_ENTRY(name, n) \
   { #name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&entry<name, n>)), METH_FASTCALL, nullptr }
 PyMethodDef methods[] = {
-    BRT_ENTRY(topk_hot_mask, 2),    BRT_ENTRY(gate_topk, 4),           BRT_ENTRY(throttle_hotmask, 3),
+    BRT_ENTRY(topk_hot_mask, 2),    BRT_ENTRY(gate_topk, 5),           BRT_ENTRY(throttle_hotmask, 3),
     BRT_ENTRY(generate, 5),         BRT_ENTRY(route_and_dispatch, 7),  BRT_ENTRY(route_by_path, 7),
     BRT_ENTRY(dispatch, 12),  BRT_ENTRY(dispatch_and_read, 8),        BRT_ENTRY(combine, 8),             BRT_ENTRY(combine_by_row_tags, 5),
-    BRT_ENTRY(top1_to_capacity, 2), BRT_ENTRY(top1_route_to_capacity, 4), BRT_ENTRY(dispatch_by_rows, 5), BRT_ENTRY(combine_by_rows, 7),     BRT_ENTRY(grouped_linear, 16),
+    BRT_ENTRY(top1_to_capacity, 2), BRT_ENTRY(top1_route_to_capacity, 4), BRT_ENTRY(dispatch_by_rows, 6), BRT_ENTRY(combine_by_rows, 8),     BRT_ENTRY(grouped_linear, 16),
     BRT_ENTRY(grouped_linear_f32, 16), BRT_ENTRY(cast_f32_to_bf16, 1), BRT_ENTRY(branch_key, 5),        BRT_ENTRY(int_list, 1),
     BRT_ENTRY(ordinary, 3),         BRT_ENTRY(plain, 1),            BRT_ENTRY(of_class, 2),            BRT_ENTRY(matrix, 4),
     BRT_ENTRY(grid, 5),                BRT_ENTRY(split_rows, 4),

@@ -473,6 +473,35 @@ int brt_hip_combine_by_rows_gated(const void* src, void* dst, const void* gates,
                                   int P, int is_residual, int in_dtype, int out_dtype, void* stream);
 
 /*
+ * Gradients of the compact route.  Results are rounded once from fp32 sums of fixed order; no workspace, one launch each.
+ *
+ * brt_hip_gate_topk_grad: grad_scores [T,E] (of dtype) from grad [T,k], the gradient of the weights that
+ *   brt_hip_gate_topk gave for path_ids: with softmax p * (grad at the chosen columns - sum_j grad[t,j] weights[t,j]),
+ *   p the softmax of the row; else grad at the chosen columns, zero elsewhere (weights may be NULL).  E <= 1024.
+ *
+ * brt_hip_dispatch_by_rows_grad: of grad_rows [P,cell], the gradient of dispatch_by_rows' result,
+ *   grad_cells[t] = sum_j weights[t,j] * grad_rows[seat_rows[t,j]-1] over the entries with a row, j ascending (weights
+ *   NULL = 1), and grad_weights[t,j] = <cells[t], grad_rows[seat_rows[t,j]-1]>, zero without a row.  Either result may be
+ *   NULL; cells is read for grad_weights only.
+ *
+ * brt_hip_combine_by_rows_grad: of grad [T,cell] (of dtype or fp32), the gradient of combine_by_rows' result,
+ *   grad_rows[r] = weights[e] * grad[e / k], e = row_entries[r]-1, zeros for rows without an entry, and grad_weights[t,j] =
+ *   <rows[seat_rows[t,j]-1], grad[t]>.  Entries that the combine leaves out (a path named twice by a cell) get zeros.
+ *   row_entries has to be the inverse of seat_rows, as brt_hip_route_by_path writes them.  Either result may be NULL.
+ *
+ * Rows are whole 16-byte units, k <= 8.
+ */
+int brt_hip_gate_topk_grad(const void* scores, const int32_t* path_ids, const float* weights, const float* grad,
+                           void* grad_scores, int T, int E, int k, int dtype, int softmax, void* stream);
+int brt_hip_dispatch_by_rows_grad(const void* grad_rows, const void* cells, const float* weights,
+                                  const int32_t* seat_rows, void* grad_cells, float* grad_weights, int T, int k, int cell,
+                                  int P, int dtype, void* stream);
+int brt_hip_combine_by_rows_grad(const void* grad, const void* rows, const float* weights, const int32_t* path_ids,
+                                 const int32_t* seat_rows, const int32_t* row_entries, void* grad_rows,
+                                 float* grad_weights, int T, int k, int cell, int P, int dtype, int grad_dtype,
+                                 void* stream);
+
+/*
  * brt_hip_grouped_gemm / _f32out / _routed / _routed_f32out / _by_rows on fp32 rows of x (16-byte aligned), which the
  * kernel rounds to bf16 itself: the bits of brt_hip_cast_f32_to_bf16 followed by the bf16 form, without that pass.
  * gather_in as in the routed forms, from the tag matrix (entries_per_cell = 0; row_tags_out as there) or the row

@@ -1,0 +1,400 @@
+"""Gradients of the compact route's ops against the formulas in 64 bits, against differences, and their refusals.
+
+Tolerances: a result is a sum of n fp32 products, each rounded once and added in fp32, then rounded to its type.  The sum is
+within n * 2^-23 of the sum of the terms' magnitudes (n roundings of products and n of sums, half a step of 2^-23 each), the
+last rounding within half a step of the value (``torch.finfo(t).eps / 2``, and half of the smallest subnormal).
+"""
+import pytest
+import torch
+
+import brt._C.router as c_router
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def make_route(cells, paths, k, capacity, seed, keep=1.0):
+    """Random distinct paths per cell (some entries without one where ``keep`` < 1) and the route that route_by_path lays out."""
+    gen = torch.Generator().manual_seed(seed)
+    ids = torch.rand(cells, paths, generator=gen).argsort(1)[:, :k].int()
+    if keep < 1.0:
+        ids = torch.where(torch.rand(cells, k, generator=gen) < keep, ids, -1)
+    ids = ids.contiguous().cuda()
+    caps = torch.tensor([capacity], dtype=torch.int32, device="cuda")
+    _, _, seat_rows, row_entries = c_router.route_by_path(ids, paths, caps, rows=min(cells * k, paths * capacity) + 3)
+    return ids, seat_rows, row_entries
+
+
+def normal(seed, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).cuda()
+
+
+def near(got, want, magnitude, terms):
+    info = torch.finfo(got.dtype)
+    bound = terms * 2.0 ** -23 * magnitude + info.eps / 2 * (want.abs() + terms * 2.0 ** -23 * magnitude) + info.tiny * info.eps
+    off = (got.detach().double() - want).abs()
+    assert bool((off <= bound).all()), f"off by up to {float((off / bound.clamp(min=1e-300)).max())} of the bound"
+
+
+def of_entries(rows, seat_rows):
+    padded = torch.cat([rows.new_zeros(1, rows.shape[1]), rows]).double()
+    return padded[seat_rows.long()]
+
+
+SHAPES = [  # cells, paths, k, capacity, elements
+    (1, 4, 1, 1, 8), (1, 4, 4, 1, 16), (3, 5, 2, 2, 24), (64, 8, 1, 100, 64), (65, 8, 2, 12, 136), (257, 16, 3, 40, 264),
+    (999, 12, 2, 200, 520), (130, 9, 8, 90, 1032), (515, 64, 4, 20, 72), (77, 6, 2, 20, 4104), (2048, 32, 2, 100, 1024),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("cells,paths,k,capacity,d", SHAPES)
+def test_dispatch_gradients(cells, paths, k, capacity, d, weighted, dtype):
+    dtype = TYPES[dtype]
+    ids, seat_rows, row_entries = make_route(cells, paths, k, capacity, cells, keep=0.8)
+    x = normal(1, cells, d, dtype=dtype).requires_grad_()
+    w = normal(2, cells, k).requires_grad_() if weighted else None
+    rows = c_router.dispatch_by_rows(x, row_entries, k, w, seat_rows=seat_rows)
+    plain = c_router.dispatch_by_rows(x.detach(), row_entries, k, None if w is None else w.detach())
+    assert torch.equal(rows, plain) and rows.requires_grad and not plain.requires_grad
+    grad = normal(3, *rows.shape, dtype=dtype)
+    found = torch.autograd.grad(rows, [x] + ([w] if weighted else []), grad)
+    terms = of_entries(grad, seat_rows)
+    if weighted:
+        terms_x = terms * w.detach().double()[:, :, None]
+        products = terms * x.detach().double()[:, None]
+        near(found[1], products.sum(2), products.abs().sum(2), d)
+        assert not found[1][seat_rows == 0].any()
+    else:
+        terms_x = terms
+    near(found[0], terms_x.sum(1), terms_x.abs().sum(1), k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("cells,paths,k,capacity,d", SHAPES)
+def test_combine_gradients(cells, paths, k, capacity, d, weighted, dtype, out):
+    dtype, out = TYPES[dtype], TYPES[out]
+    ids, seat_rows, row_entries = make_route(cells, paths, k, capacity, cells + 1, keep=0.8)
+    y = normal(1, row_entries.numel(), d, dtype=dtype).requires_grad_()
+    w = normal(2, cells, k).requires_grad_() if weighted else None
+    got = c_router.combine_by_rows(y, ids, seat_rows, w, out_dtype=out, row_entries=row_entries)
+    plain = c_router.combine_by_rows(y.detach(), ids, seat_rows, None if w is None else w.detach(), out_dtype=out)
+    assert torch.equal(got, plain) and got.dtype == out and got.requires_grad
+    grad = normal(3, cells, d, dtype=out)
+    found = torch.autograd.grad(got, [y] + ([w] if weighted else []), grad)
+    entry = (row_entries.long() - 1).clamp(min=0)
+    want = grad.double()[entry // k] * (1.0 if w is None else w.detach().double().reshape(-1)[entry][:, None])
+    want = torch.where((row_entries > 0)[:, None], want, 0.0)
+    assert found[0].dtype == dtype
+    near(found[0], want, want.abs(), 1)
+    assert not found[0][row_entries == 0].any()
+    if weighted:
+        products = of_entries(y.detach(), seat_rows) * grad.double()[:, None]
+        near(found[1], products.sum(2), products.abs().sum(2), d)
+
+
+GATES = [(1, 1, 1), (1, 4, 4), (5, 3, 2), (63, 8, 2), (130, 60, 3), (257, 64, 1), (33, 100, 4), (70, 128, 2), (9, 1000, 8), (17, 1024, 2), (12, 513, 13)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("softmax", [False, True])
+@pytest.mark.parametrize("cells,paths,k", GATES)
+def test_gate_gradient(cells, paths, k, softmax, dtype):
+    """p is the softmax in fp32: exp within 2 steps of 2^-23, the sum within paths steps, the quotient within one; the bracket's
+    sum over j within k + 1 steps more, and twice the weights' own error."""
+    dtype = TYPES[dtype]
+    scores = (3 * normal(cells, cells, paths)).to(dtype).requires_grad_()
+    ids, weights, mask = c_router.gate_topk(scores, k, softmax, True, differentiable=True)
+    plain = c_router.gate_topk(scores.detach(), k, softmax, True)
+    assert all(torch.equal(a, b) for a, b in zip((ids, weights, mask), plain))
+    assert weights.requires_grad and not ids.requires_grad and not mask.requires_grad
+    grad = normal(2, cells, k)
+    (got,) = torch.autograd.grad(weights, scores, grad)
+    picked = torch.zeros(cells, paths, dtype=torch.float64, device="cuda").scatter_(1, ids.long(), grad.double())
+    if not softmax:
+        return near(got, picked, picked.abs(), 0)
+    p = torch.softmax(scores.detach().double(), 1)
+    parts = p.gather(1, ids.long()) * grad.double()
+    want = p * (picked - parts.sum(1, keepdim=True))
+    near(got, want, p * (picked.abs() + parts.abs().sum(1, keepdim=True)), 2 * paths + k + 8)
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences():
+    """fp32 operands of a few bits and steps of 2^-3: every op is linear in each operand, so a difference quotient is the
+    derivative but for the fp32 roundings of the two values."""
+    cells, paths, k, d = 13, 4, 2, 8
+    ids, seat_rows, row_entries = make_route(cells, paths, k, 5, 1)
+    x, w = normal(1, cells, d).round(), normal(2, cells, k).round()
+    up = normal(3, row_entries.numel(), d).round()
+
+    def of_dispatch(x, w):
+        return (c_router.dispatch_by_rows(x, row_entries, k, w, seat_rows=seat_rows).double() * up).sum()
+
+    y, back = normal(4, row_entries.numel(), d).round(), normal(5, cells, d).round()
+
+    def of_combine(y, w):
+        return (c_router.combine_by_rows(y, ids, seat_rows, w, row_entries=row_entries).double() * back).sum()
+
+    for op, operands in ((of_dispatch, (x, w)), (of_combine, (y, w))):
+        leaves = [t.clone().requires_grad_() for t in operands]
+        grads = torch.autograd.grad(op(*leaves), leaves)
+        for n, grad in enumerate(grads):
+            flat = operands[n].reshape(-1)
+            for i in range(0, flat.numel(), 7):
+                moved = []
+                for step in (0.125, -0.125):
+                    other = [t.clone() for t in operands]
+                    other[n].view(-1)[i] += step
+                    moved.append(op(*other))
+                assert float((moved[0] - moved[1]) / 0.25) == float(grad.reshape(-1)[i])
+
+
+@pytest.mark.gpu
+def test_a_path_named_twice_by_a_cell():
+    """The dispatch copies the cell to both rows, the combine adds the first of them only: so do their gradients."""
+    ids = torch.tensor([[1, 1], [0, 1], [-1, -1]], dtype=torch.int32, device="cuda")
+    _, _, seat_rows, row_entries = c_router.route_by_path(ids, 2)
+    d = 8
+    x, w = normal(1, 3, d).requires_grad_(), normal(2, 3, 2).requires_grad_()
+    rows = c_router.dispatch_by_rows(x, row_entries, 2, w, seat_rows=seat_rows)
+    grad = normal(3, *rows.shape)
+    dx, dw = torch.autograd.grad(rows, [x, w], grad)
+    terms = of_entries(grad, seat_rows)
+    near(dx, (terms * w.detach().double()[:, :, None]).sum(1), (terms * w.detach().double()[:, :, None]).abs().sum(1), 2)
+    y = normal(4, *rows.shape).requires_grad_()
+    out = c_router.combine_by_rows(y, ids, seat_rows, w, row_entries=row_entries)
+    g = normal(5, 3, d)
+    dy, dw = torch.autograd.grad(out, [y, w], g)
+    first, second = seat_rows[0].tolist()
+    assert not dy[second - 1].any() and float(dw[0, 1]) == 0.0
+    near(dy[first - 1], w[0, 0].detach().double() * g[0].double(), (w[0, 0] * g[0]).detach().double().abs(), 1)
+    assert not dw[2].any() and not dx[2].any()
+
+
+@pytest.mark.gpu
+def test_what_belongs_to_no_entry_is_not_looked_at():
+    """NaN in rows without an entry and in weights of entries without a row do not reach the gradients."""
+    ids = torch.tensor([[0, -1], [1, 0], [0, 1]], dtype=torch.int32, device="cuda")
+    caps = torch.tensor([2], dtype=torch.int32, device="cuda")
+    _, _, seat_rows, row_entries = c_router.route_by_path(ids, 2, caps, rows=6)
+    w = normal(1, 3, 2)
+    w[seat_rows == 0] = float("nan")
+    w.requires_grad_()
+    x = normal(2, 3, 32).requires_grad_()
+    grad = normal(3, 6, 32)
+    grad[row_entries == 0] = float("nan")
+    dx, dw = torch.autograd.grad(c_router.dispatch_by_rows(x, row_entries, 2, w, seat_rows=seat_rows), [x, w], grad)
+    assert torch.isfinite(dx).all() and torch.isfinite(dw).all()
+    y = normal(4, 6, 32)
+    y[row_entries == 0] = float("nan")
+    y.requires_grad_()
+    out = c_router.combine_by_rows(y, ids, seat_rows, w, row_entries=row_entries)
+    dy, dw = torch.autograd.grad(out, [y, w], normal(5, 3, 32))
+    assert torch.isfinite(out).all() and torch.isfinite(dy).all() and torch.isfinite(dw).all()
+
+
+@pytest.mark.gpu
+def test_gate_gradient_of_masked_scores():
+    """Scores of -inf have no probability and no gradient; a row of nothing else is NaN, as its softmax is."""
+    scores = normal(1, 4, 40)
+    scores[0, 3:] = float("-inf")
+    scores[1, ::2] = torch.finfo(torch.float32).min
+    scores[2] = float("-inf")
+    scores.requires_grad_()
+    ids, weights = c_router.gate_topk(scores, 2, True, differentiable=True)
+    (got,) = torch.autograd.grad(weights, scores, torch.ones_like(weights))
+    p = torch.softmax(scores.detach().double(), 1)
+    sums = p.gather(1, ids.long()).sum(1, keepdim=True)
+    want = p * (torch.zeros_like(p).scatter_(1, ids.long(), 1.0) - sums)
+    assert not got[0, 3:].any() and not got[1, ::2].any() and got[2].isnan().all()
+    rows = [0, 1, 3]
+    near(got[rows], want[rows], p[rows] * (1 + sums[rows]), 2 * 40 + 10)
+
+
+@pytest.mark.gpu
+def test_only_what_is_asked_for():
+    cells, k, d = 50, 2, 64
+    ids, seat_rows, row_entries = make_route(cells, 4, k, 20, 1)
+    x, w = normal(1, cells, d), normal(2, cells, k)
+    assert not c_router.dispatch_by_rows(x, row_entries, k, w, seat_rows=seat_rows).requires_grad
+    with torch.no_grad():
+        assert not c_router.dispatch_by_rows(x.requires_grad_(), row_entries, k, w, seat_rows=seat_rows).requires_grad
+    x = x.detach()
+    grad = normal(3, row_entries.numel(), d)
+    both = [t.clone().requires_grad_() for t in (x, w)]
+    want = torch.autograd.grad(c_router.dispatch_by_rows(both[0], row_entries, k, both[1], seat_rows=seat_rows), both, grad)
+    for n in range(2):
+        pair = [x.clone(), w.clone()]
+        pair[n].requires_grad_()
+        (got,) = torch.autograd.grad(c_router.dispatch_by_rows(pair[0], row_entries, k, pair[1], seat_rows=seat_rows), pair[n], grad)
+        assert torch.equal(got, want[n])
+    y, back = normal(4, row_entries.numel(), d), normal(5, cells, d)
+    both = [t.clone().requires_grad_() for t in (y, w)]
+    want = torch.autograd.grad(c_router.combine_by_rows(both[0], ids, seat_rows, both[1], row_entries=row_entries), both, back)
+    for n in range(2):
+        pair = [y.clone(), w.clone()]
+        pair[n].requires_grad_()
+        (got,) = torch.autograd.grad(c_router.combine_by_rows(pair[0], ids, seat_rows, pair[1], row_entries=row_entries), pair[n], back)
+        assert torch.equal(got, want[n])
+
+
+@pytest.mark.gpu
+def test_strides_shapes_and_broadcast_gradients():
+    """Cells of several dimensions, operands that are views, a gradient without strides (that of a sum)."""
+    cells, k = 40, 2
+    ids, seat_rows, row_entries = make_route(cells, 6, k, 30, 1)
+    base = normal(1, cells, 4, 24)
+    x = base.transpose(1, 2)[:, ::2].requires_grad_()  # [cells, 12, 4], not contiguous
+    w = normal(2, k, cells).t().requires_grad_()
+    rows = c_router.dispatch_by_rows(x, row_entries, k, w, seat_rows=seat_rows)
+    assert rows.shape == (row_entries.numel(), 12, 4)
+    dx, dw = torch.autograd.grad(rows.sum(), [x, w])
+    has = (seat_rows > 0).double()
+    near(dx, (has * w.detach().double()).sum(1)[:, None, None].expand(cells, 12, 4), (has * w.detach().double().abs()).sum(1)[:, None, None], k)
+    sums = x.detach().double().sum((1, 2))[:, None] * has
+    near(dw, sums, x.detach().double().abs().sum((1, 2))[:, None] * has, 48)
+    out = c_router.combine_by_rows(rows.detach().requires_grad_(), ids, seat_rows, row_entries=row_entries)
+    assert out.shape == x.shape
+    wide = normal(3, 30, 16)[:, ::2].requires_grad_()
+    _, weights = c_router.gate_topk(wide, 2, True, differentiable=True)
+    (got,) = torch.autograd.grad(weights.sum(), wide)
+    assert got.shape == wide.shape and torch.isfinite(got).all()
+
+
+@pytest.mark.gpu
+def test_gates_of_a_differentiable_combine():
+    cells, paths, k, d = 33, 5, 2, 16
+    ids, seat_rows, row_entries = make_route(cells, paths, k, 40, 1)
+    y, gates = normal(1, row_entries.numel(), d).requires_grad_(), normal(2, cells, paths).requires_grad_()
+    out = c_router.combine_by_rows(y, ids, seat_rows, gates=gates, row_entries=row_entries)
+    assert torch.equal(out, c_router.combine_by_rows(y.detach(), ids, seat_rows, gates=gates.detach()))
+    back = normal(3, cells, d)
+    _, dgates = torch.autograd.grad(out, [y, gates], back)
+    products = of_entries(y.detach(), seat_rows) * back.double()[:, None]
+    want = torch.zeros(cells, paths, dtype=torch.float64, device="cuda").scatter_(1, ids.long(), products.sum(2))
+    near(dgates, want, torch.zeros_like(want).scatter_(1, ids.long(), products.abs().sum(2)), d)
+
+
+@pytest.mark.gpu
+def test_gradients_of_gradients_are_refused():
+    cells, k, d = 20, 1, 16
+    ids, seat_rows, row_entries = make_route(cells, 4, k, 20, 1)
+    x = normal(1, cells, d).requires_grad_()
+    rows = c_router.dispatch_by_rows(x, row_entries, k, seat_rows=seat_rows)
+    (dx,) = torch.autograd.grad((rows * rows).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable again"):
+        torch.autograd.grad(dx.sum(), x)
+
+
+@pytest.mark.gpu
+def test_refusals_of_the_differentiable_forms():
+    cells, k, d = 20, 2, 16
+    ids, seat_rows, row_entries = make_route(cells, 4, k, 20, 1)
+    x, w = normal(1, cells, d).requires_grad_(), normal(2, cells, k)
+    y = normal(3, row_entries.numel(), d).requires_grad_()
+    room = torch.empty(row_entries.numel(), d, device="cuda")
+    with pytest.raises(RuntimeError, match="not both"):
+        c_router.dispatch_by_rows(x, row_entries, k, out=room, seat_rows=seat_rows)
+    with pytest.raises(RuntimeError, match=r"\[cells, k\]"):
+        c_router.dispatch_by_rows(x, row_entries, k, seat_rows=seat_rows[:-1])
+    with pytest.raises(RuntimeError, match="int32"):
+        c_router.dispatch_by_rows(x, row_entries, k, seat_rows=seat_rows.long())
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        c_router.dispatch_by_rows(x, row_entries, k, seat_rows=seat_rows.cpu())
+    with pytest.raises(RuntimeError, match="another device"):
+        c_router.dispatch_by_rows(x, row_entries, k, w.cpu(), seat_rows=seat_rows)
+    with pytest.raises(NotImplementedError):
+        c_router.dispatch_by_rows(x, row_entries, 9, seat_rows=torch.ones(cells, 9, dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="neither out_data nor gates"):
+        c_router.combine_by_rows(y, ids, seat_rows, out_data=torch.zeros(cells, d, device="cuda"), row_entries=row_entries)
+    with pytest.raises(RuntimeError, match="one entry for every row"):
+        c_router.combine_by_rows(y, ids, seat_rows, row_entries=row_entries[:-1])
+    with pytest.raises(RuntimeError, match="fp32"):
+        c_router.combine_by_rows(y, ids, seat_rows, w.double(), row_entries=row_entries)
+    with pytest.raises(NotImplementedError):
+        c_router.combine_by_rows(y[:, :3], ids, seat_rows, row_entries=row_entries)
+    saved = x * 1
+    rows = c_router.dispatch_by_rows(saved, row_entries, k, w.requires_grad_(), seat_rows=seat_rows)
+    with torch.no_grad():
+        saved.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        rows.sum().backward()
+
+
+@pytest.mark.gpu
+def test_no_cells_and_no_rows():
+    none = torch.zeros(0, 2, dtype=torch.int32, device="cuda")
+    x = torch.zeros(0, 16, device="cuda", requires_grad=True)
+    entries = torch.zeros(3, dtype=torch.int32, device="cuda")
+    rows = c_router.dispatch_by_rows(x, entries, 2, seat_rows=none)
+    (dx,) = torch.autograd.grad(rows.sum(), x)
+    assert dx.shape == x.shape
+    y = normal(1, 3, 16).requires_grad_()
+    out = c_router.combine_by_rows(y, none, none, row_entries=entries)
+    (dy,) = torch.autograd.grad(out.sum(), y)
+    assert out.shape == (0, 16) and dy.shape == y.shape and not dy.any()
+    bare = torch.zeros(5, 1, dtype=torch.int32, device="cuda")
+    nothing = torch.zeros(0, dtype=torch.int32, device="cuda")
+    x = normal(2, 5, 16).requires_grad_()
+    w = normal(3, 5, 1).requires_grad_()
+    rows = c_router.dispatch_by_rows(x, nothing, 1, w, seat_rows=bare)
+    dx, dw = torch.autograd.grad(rows.sum(), [x, w])
+    assert rows.shape == (0, 16) and not dx.any() and not dw.any()
+
+
+@pytest.mark.gpu
+def test_a_training_step_of_all_three_on_a_stream_and_replayed():
+    """Gate, route, sort and back with identity experts: against autograd over plain torch in 64 bits, on a stream of its own,
+    and captured once and replayed for other inputs."""
+    cells, paths, k, d = 96, 8, 2, 64
+    caps = torch.tensor([20], dtype=torch.int32, device="cuda")
+
+    def step(x, scores, back):
+        ids, weights = c_router.gate_topk(scores, k, True, differentiable=True)
+        _, _, seat_rows, row_entries = c_router.route_by_path(ids, paths, caps, rows=paths * 20)
+        rows = c_router.dispatch_by_rows(x, row_entries, k, seat_rows=seat_rows)
+        out = c_router.combine_by_rows(rows, ids, seat_rows, weights, row_entries=row_entries)
+        return (seat_rows, ids, out) + torch.autograd.grad(out, [x, scores], back)
+
+    def inputs(seed):
+        return normal(seed, cells, d).requires_grad_(), normal(seed + 1, cells, paths).requires_grad_(), normal(seed + 2, cells, d)
+
+    def check(made, x, scores, back):
+        seat_rows, ids, out, dx, dscores = made
+        x64, s64 = x.detach().double().requires_grad_(), scores.detach().double().requires_grad_()
+        w64 = torch.softmax(s64, 1).gather(1, ids.long()) * (seat_rows > 0)
+        want = x64 * w64.sum(1, keepdim=True)
+        gx, gs = torch.autograd.grad(want, [x64, s64], back.double())
+        torch.testing.assert_close(out.double(), want.detach(), rtol=1e-5, atol=1e-5)
+        torch.testing.assert_close(dx.double(), gx, rtol=1e-5, atol=1e-5)
+        torch.testing.assert_close(dscores.double(), gs, rtol=1e-4, atol=2e-5)
+
+    first = inputs(1)
+    check(step(*first), *first)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        second = inputs(11)
+        made = step(*second)
+    torch.cuda.current_stream().wait_stream(stream)
+    check(made, *second)
+    del made
+    x, scores, back = inputs(21)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(x, scores, back)
+    for seed in (31, 41, 51):
+        new = inputs(seed)
+        with torch.no_grad():
+            for to, of in zip((x, scores, back), new):
+                to.copy_(of)
+        graph.replay()
+        eager = step(*new)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, eager))
+        check(held, *new)
