@@ -968,6 +968,89 @@ PyObject* cast_f32_to_bf16(const Args& a) {
   return wrap(rounded_to_bf16(given));
 }
 
+// ---- products in 8 bits ------------------------------------------------------------------------------
+constexpr int64_t kScaleBlock = 128;
+int64_t blocks_of(int64_t n) { return (n + kScaleBlock - 1) / kScaleBlock; }
+bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+struct Blocks {
+  Tensor q, scales;  // [rows, pitch] bytes, [blocks, rows]
+};
+Blocks quantized(const Tensor& given, const char* name) {
+  const int type = data_type(given, (std::string(name) + " data type").c_str());
+  if (given.dim() != 2) runtime_error(std::string(name) + " must be [rows, elements]");
+  Tensor in = dense(given);
+  if (!aligned16(in)) in = in.clone();
+  const int64_t P = in.size(0), K = in.size(1), KB = blocks_of(K);
+  Blocks b{empty({P, KB * kScaleBlock}, at::kByte, in), empty({KB, P}, at::kFloat, in)};
+  check(brt_hip_quantize_rows(ptr(in), P, K, type, ptr(b.q), KB * kScaleBlock, fptr(b.scales), stream_of(in)));
+  return b;
+}
+PyObject* as_rows(const Blocks& b, int64_t K) {  // what Python sees: e4m3 [rows, elements], [rows, blocks]
+  return tuple(wrap(b.q.view(at::kFloat8_e4m3fn).narrow(1, 0, K)), wrap(b.scales.t()));
+}
+
+PyObject* quantize_rows(const Args& a) {  // x
+  const Tensor x = a.tensor(0);
+  on_device(x, "x");
+  const c10::DeviceGuard guard(x.device());
+  return as_rows(quantized(x, "x"), x.dim() == 2 ? x.size(1) : 0);
+}
+
+// x, weight, weight_scales, loads, bias, activation, x_scales, out, out_dtype, out_blocks
+PyObject* grouped_linear_fp8(const Args& a) {
+  const Tensor x = a.tensor(0), w = a.tensor(1), w_scales = a.tensor(2), loads_given = a.tensor(3), bias_given = a.tensor_or_none(4);
+  const Tensor x_scales = a.tensor_or_none(6);
+  Tensor out = a.tensor_or_none(7);
+  const bool out_blocks = a.flag(9);
+  on_device(x, "x"), on_device(w, "weight"), on_device(w_scales, "weight_scales"), on_device(loads_given, "loads");
+  int32(loads_given, "loads");
+  if (x.dim() != 2 || w.dim() != 3 || w.size(2) != x.size(1)) runtime_error("x must be [rows, in_features], weight [experts, out_features, in_features]");
+  if (w.scalar_type() != at::kFloat8_e4m3fn) not_implemented("weight must be float8_e4m3fn");
+  const int64_t P = x.size(0), K = x.size(1), E = w.size(0), N = w.size(1), KB = blocks_of(K);
+  if (w_scales.scalar_type() != at::kFloat || w_scales.sizes() != at::IntArrayRef({E, blocks_of(N), KB}))
+    runtime_error("weight_scales must be fp32 [experts, blocks of out_features, blocks of in_features]");
+  if (loads_given.numel() != E) runtime_error("one load per expert is needed");
+  for (const Tensor* t : std::initializer_list<const Tensor*>{&w, &w_scales, &loads_given, &bias_given, &x_scales, &out})
+    if (t->defined()) same_device(*t, x, "an operand");
+  if (bias_given.defined()) {
+    data_type(bias_given, "bias data type");
+    if (bias_given.sizes() != at::IntArrayRef({E, N})) runtime_error("bias must be [experts, out_features]");
+  }
+  const c10::DeviceGuard guard(x.device());
+  const bool in_blocks = x.scalar_type() == at::kFloat8_e4m3fn;
+  if (in_blocks != x_scales.defined()) runtime_error("x_scales belong to float8_e4m3fn rows, and only to them");
+  at::ScalarType type = in_blocks ? at::kBFloat16 : x.scalar_type();
+  const bool typed = a.dtype(8, &type);
+  if (code_of(type) < 0) not_implemented(in_blocks || typed ? "output data type is not supported" : "x data type is not supported");
+  if (out.defined()) {
+    if (out_blocks || (typed && type != out.scalar_type())) runtime_error("out is given: it says its type, and holds no blocks");
+    if (data_type(out, "output data type") < 0 || out.sizes() != at::IntArrayRef({P, N}) || !out.is_contiguous())
+      runtime_error("out must be a contiguous [rows, out_features] tensor");
+  } else {
+    out = empty({P, N}, type, x);
+  }
+  const Tensor weight = dense(w), weight_scales = dense(w_scales), loads = dense(loads_given);
+  const Tensor bias = bias_given.defined() ? dense(bias_given) : bias_given;
+  Tensor rows, scales;
+  int64_t pitch;
+  if (in_blocks) {
+    if (x_scales.scalar_type() != at::kFloat || x_scales.sizes() != at::IntArrayRef({P, KB})) runtime_error("x_scales must be fp32 [rows, blocks]");
+    const bool in_place = P > 0 && (x.stride(1) == 1 || K == 1) && x.stride(0) >= K && x.stride(0) % 16 == 0 && aligned16(x);
+    rows = in_place ? x : x.contiguous();
+    if (!aligned16(rows)) rows = rows.clone();
+    pitch = in_place ? x.stride(0) : K;
+    scales = x_scales.t().contiguous();
+  } else {
+    const Blocks b = quantized(x, "x");
+    rows = b.q, scales = b.scales, pitch = b.q.size(1);
+  }
+  check(brt_hip_grouped_gemm_fp8(ptr(rows), pitch, fptr(scales), ptr(weight), fptr(weight_scales), iptr(loads), ptr(bias),
+                                 bias.defined() ? code_of(bias.scalar_type()) : BRT_F32, ptr(out), code_of(out.scalar_type()), E, P, N, K,
+                                 a.integer(5), stream_of(x)));
+  return out_blocks ? as_rows(quantized(out, "out"), N) : wrap(out);
+}
+
 // ---- values on the host ------------------------------------------------------------------------------
 // The values of an int32 vector as a list.
 PyObject* int_list(const Args& a) {
@@ -1205,6 +1288,7 @@ PyMethodDef methods[] = {
     BRT_ENTRY(grouped_linear_f32, 16), BRT_ENTRY(cast_f32_to_bf16, 1), BRT_ENTRY(branch_key, 5),        BRT_ENTRY(int_list, 1),
     BRT_ENTRY(ordinary, 3),         BRT_ENTRY(plain, 1),            BRT_ENTRY(of_class, 2),            BRT_ENTRY(matrix, 4),
     BRT_ENTRY(grid, 5),                BRT_ENTRY(split_rows, 4),
+    BRT_ENTRY(quantize_rows, 1), BRT_ENTRY(grouped_linear_fp8, 10),
     BRT_ENTRY(sum_rows_by_index, 3), BRT_ENTRY(combine_flows, 2), BRT_ENTRY(one_value, 2),         BRT_ENTRY(unique_tags, 1),      BRT_ENTRY(calls, 0),            {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "brt_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

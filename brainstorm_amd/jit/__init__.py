@@ -23,7 +23,7 @@ from brainstorm_amd import _lib
 from brainstorm_amd._C import router as c_router
 from brainstorm_amd.runtime import deferred
 
-__all__ = ["make_jit_kernel", "grouped_linear", "GroupedLinearKernel"]
+__all__ = ["make_jit_kernel", "grouped_linear", "grouped_linear_fp8", "quantize_rows", "GroupedLinearKernel"]
 
 _ACT = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "gelu": _lib.ACT_GELU, "relu": _lib.ACT_RELU}
 
@@ -65,6 +65,32 @@ def grouped_linear(x: torch.Tensor, out: torch.Tensor, weight_table: torch.Tenso
         x, out, weight_table, bias_table, loads, in_features, out_features, _ACT[activation], tags, gather,
         scatter, rows, row_entries, int(entries_per_cell), row_tags_out, gates)
     return out
+
+
+def quantize_rows(x: torch.Tensor) -> tuple:
+    """``(q, scales)`` of rows ``x`` (``[rows, elements]``, fp32 / fp16 / bf16): ``q`` float8_e4m3fn ``[rows, elements]`` and
+    one fp32 scale for every 128 elements of a row, ``scales [rows, ceil(elements / 128)]``.  With ``top = max(|x|, 2**-100)``
+    over the block, ``scale = top / 448`` and ``q = e4m3(x * (1 / top * 448))``, every operation rounded in fp32, the last one to
+    nearest even.  ``elements`` is a multiple of 16.  (``q`` is a view of rows padded to whole blocks, ``scales`` the transpose
+    of a contiguous matrix: what :func:`grouped_linear_fp8` reads in place.)"""
+    return _lib.native().quantize_rows(x)
+
+
+def grouped_linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor, loads: torch.Tensor, *,
+                       bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+                       x_scales: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                       out_dtype: Optional[torch.dtype] = None, out_blocks: bool = False):
+    """:func:`grouped_linear` on 8-bit weights: ``out[s_e : s_e + loads[e]] = act(x[s_e : s_e + loads[e]] @ W_e^T + b_e)`` with
+    ``W_e[n, k] = weight[e, n, k] * weight_scales[e, n // 128, k // 128]``, ``weight`` float8_e4m3fn ``[experts, out_features,
+    in_features]`` (in_features a multiple of 16) and fp32 scales.  ``x`` is quantized as :func:`quantize_rows` does it, or comes
+    that way (float8_e4m3fn with ``x_scales``).  The products of a block are summed by the matrix units, scaled by ``x_scale *
+    weight_scale`` in fp32 and summed in order of the blocks; bias, activation and one rounding follow.
+
+    The result has ``x``'s type (``out_dtype``, or bf16 for 8-bit rows); a given ``out`` is filled in place.  Rows behind the
+    last expert's are not written.  ``out_blocks=True`` gives ``(q, scales)``, the quantized result, rounded to that type
+    first: the rows of the next such product.  Results are cut off from autograd, as those of :func:`grouped_linear`."""
+    return _lib.native().grouped_linear_fp8(x, weight, weight_scales, loads, bias, _ACT[activation], x_scales, out, out_dtype,
+                                            bool(out_blocks))
 
 
 def _linear(x, out, weight_table, bias_table, loads, in_features, out_features, activation, *, tags=None, gather=False,
