@@ -154,10 +154,11 @@ SIGNATURES = {
          _c_int, _c_int, _c_ptr],
     ),
     "brt_hip_quantize_rows": (_c_int, [_c_ptr, _c_int, _c_int, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr]),
+    "brt_hip_grouped_gemm_fp8_quantizes": (_c_int, [_c_int, _c_int, _c_int]),
     "brt_hip_grouped_gemm_fp8": (
         _c_int,
-        [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int,
-         _c_int, _c_ptr],
+        [_c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int,
+         _c_int, _c_int, _c_ptr],
     ),
     "brt_hip_gate_topk_grad": (
         _c_int,

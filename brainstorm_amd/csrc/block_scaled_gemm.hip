@@ -12,6 +12,7 @@
 // three-hundredth of a bf16 rounding, a twentieth of an fp16 one.  An fp32 result would show it, so there the operands are
 // widened to bf16 in registers (exactly) and multiplied by v_mfma_f32_16x16x32_bf16, whose sums are off by 1.2e-8.
 #include <algorithm>
+#include <type_traits>
 
 #include "grouped_gemm.hpp"
 #include "rows.hpp"
@@ -27,6 +28,7 @@ constexpr float kMax = 448.0f;     // the largest e4m3 value
 constexpr float kLeast = 0x1p-100f;  // blocks whose largest value is below this are scaled as if it were this
 constexpr int kXcds = 8, kCusPerXcd = 32;
 constexpr int kPatchRows = 4;
+constexpr int kMostExperts = 512;  // whose row blocks a workgroup keeps in LDS
 constexpr uint32_t kNowhere = 0x7ffffff0u;  // an offset past every extent: reads as zero, costs no request
 
 // ------------------------------------------------------------------------------------- quantization
@@ -109,7 +111,16 @@ __device__ __forceinline__ void load_to_lds(const i32x4& rsrc, uint32_t voffset,
                : "{m0}"(lds_base), "v"(voffset), "s"(rsrc), "s"(soffset)
                : "memory");
 }
-__device__ __forceinline__ void wait_loads_all() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+// ... 4 bytes per lane, at lds_base + 4 * lane
+__device__ __forceinline__ void load_word_to_lds(const i32x4& rsrc, uint32_t voffset, uint32_t lds_base) {
+  asm volatile("s_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "{m0}"(lds_base), "v"(voffset), "s"(rsrc)
+               : "memory");
+}
+// all but the last N loads of this wavefront have landed
+template <int N>
+__device__ __forceinline__ void wait_loads_but() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
 __device__ __forceinline__ void block_barrier() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
@@ -178,18 +189,21 @@ __device__ __forceinline__ float activated(float v, int act) {
   return v;
 }
 
+// The biases of columns n .. n + COUNT - 1 (zeros without any).
+template <int COUNT>
+__device__ __forceinline__ void biases(const Fp8Args& a, int e, int n, float (&b)[COUNT]) {
+#pragma unroll
+  for (int q = 0; q < COUNT; ++q)
+    b[q] = a.bias != nullptr ? load_gate(a.bias, a.bias_dtype, static_cast<size_t>(e) * a.N + min(n + q, a.N - 1)) : 0.0f;
+}
+
 // COUNT results of one row, columns n .. n + COUNT - 1, biased, activated, rounded and stored; `whole`: the row's pieces are
 // aligned and N is a multiple of COUNT.
 template <int COUNT>
-__device__ __forceinline__ void finish(const Fp8Args& a, int e, size_t row, int n, bool whole, float (&v)[COUNT]) {
+__device__ __forceinline__ void finish(const Fp8Args& a, size_t row, int n, bool whole, const float (&bias)[COUNT], float (&v)[COUNT]) {
   if (n >= a.N) return;
-  if (a.bias != nullptr) {
 #pragma unroll
-    for (int q = 0; q < COUNT; ++q)
-      v[q] += load_gate(a.bias, a.bias_dtype, static_cast<size_t>(e) * a.N + min(n + q, a.N - 1));
-  }
-#pragma unroll
-  for (int q = 0; q < COUNT; ++q) v[q] = activated(v[q], a.act);
+  for (int q = 0; q < COUNT; ++q) v[q] = activated(v[q] + bias[q], a.act);
   const size_t at = row * a.N + n;
   if (whole) {
     if (a.out_dtype == BRT_F32) pack_store<BRT_F32, COUNT>(static_cast<float*>(a.out) + at, v);
@@ -205,90 +219,320 @@ __device__ __forceinline__ void finish(const Fp8Args& a, int e, size_t row, int 
   }
 }
 
-// BM x BN tiles, WM x WN wavefronts.  Both operands go straight into LDS, K-steps of 128 bytes in two stages: the next one is
-// requested when this one has landed and is read.
-template <int BM_BITS, int BN, int WM, int WN, bool EXACT>
+// The products of a K-step on their way into the accumulators: while one is on the matrix pipe, the one two before it is scaled
+// and added.  What is left of a K-step is added while the next one's fragments come, with its scales still.  (sched_barrier keeps
+// the order: left alone the compiler puts each addition behind its product and waits for it.)
+template <int MT, int NT>
+struct Pipe {
+  f32x4 held[4];
+  __device__ __forceinline__ Pipe() { clear(); }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) held[p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  __device__ __forceinline__ void add(int p, f32x4 (&acc)[MT][NT], const float (&s)[MT]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc[p % MT][p / MT][q] = __builtin_fmaf(held[p & 3][q], s[p % MT], acc[p % MT][p / MT][q]);
+  }
+  __device__ __forceinline__ void put(int p, const f32x4& product, f32x4 (&acc)[MT][NT], const float (&s)[MT]) {
+    held[p & 3] = product;
+    if (p >= 2) add(p - 2, acc, s);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __device__ __forceinline__ void drain(f32x4 (&acc)[MT][NT], const float (&s)[MT]) {
+    add(MT * NT - 2, acc, s);
+    add(MT * NT - 1, acc, s);
+  }
+};
+
+// Results of one row as they are stored: biased, activated, rounded.
+template <int ACT, int OUT>
+__device__ __forceinline__ void finish8(const Fp8Args& a, size_t row, int n, bool whole, const float (&bias)[8], float (&v)[8]) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q) v[q] = apply_act<ACT>(v[q] + bias[q]);
+  const size_t at = row * a.N + n;
+  char* const to = static_cast<char*>(a.out) + at * elem_bytes(OUT);
+  if (whole) {
+    pack_store<OUT, 8>(to, v);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (n + q < a.N) {
+        const float one[1] = {v[q]};
+        pack_store<OUT, 1>(to + q * elem_bytes(OUT), one);
+      }
+  }
+}
+
+// The results of a wavefront: MT x NT tiles from row r0 of the block and column n0, tile columns as the kernels below deal them.
+template <int MT, int NT, bool EXACT>
+__device__ __forceinline__ void store_tile(const Fp8Args& a, const Block& at, int r0, int n0, f32x4 (&acc)[MT][NT]) {
+  const int lane = lane_id(), g = lane >> 4, c16 = lane & 15;
+  const bool whole = a.N % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+  auto store = [&](auto act, auto out) {
+#pragma unroll
+    for (int j = 0; j < NT; j += 2) {
+      const int n = n0 + (j >> 2) * 64 + ((j >> 1) & 1) * 32 + g * 8;
+      float bias[8];
+      biases<8>(a, at.e, n, bias);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int r = r0 + i * 16 + c16;
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = acc[i][j][q], v[4 + q] = acc[i][j + 1][q];
+        if (r < at.rows && n < a.N)
+          finish8<decltype(act)::value, decltype(out)::value>(a, static_cast<size_t>(at.row0) + r, n, whole, bias, v);
+      }
+    }
+  };
+  auto with_act = [&](auto out) {
+    if (a.act == BRT_ACT_GELU) store(std::integral_constant<int, BRT_ACT_GELU>{}, out);
+    else if (a.act == BRT_ACT_RELU) store(std::integral_constant<int, BRT_ACT_RELU>{}, out);
+    else store(std::integral_constant<int, BRT_ACT_NONE>{}, out);
+  };
+  if constexpr (EXACT) with_act(std::integral_constant<int, BRT_F32>{});
+  else if (a.out_dtype == BRT_F16) with_act(std::integral_constant<int, BRT_F16>{});
+  else with_act(std::integral_constant<int, BRT_BF16>{});
+}
+
+// BM x BN tiles, WM x WN wavefronts, STAGES K-steps of 128 bytes in LDS.  Operands and scales go straight into LDS; a K-step is
+// requested STAGES - 1 steps before it is multiplied, into the stage that was read last.  A workgroup stays for several tiles, and
+// its requests run on through their boundaries: a tile of 1024 elements has eight K-steps, and starting anew (which expert, the
+// first K-step) took as long as half of them.  The list of row blocks is kept in LDS for that.
+template <int BM_BITS, int BN, int WM, int WN, int STAGES, bool EXACT>
 __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
   constexpr int BM = 1 << BM_BITS, WAVES = WM * WN;
   constexpr int MT = BM / WM / 16, NT = BN / WN / 16;  // 16 x 16 tiles of a wavefront
   constexpr int XL = BM / 8 / WAVES, WL = BN / 8 / WAVES;  // loads of a wavefront and K-step, 8 rows each
-  constexpr int kStage = (BM + BN) * kB;
+  constexpr int kLoads = XL + WL + 1;                      // ... and one of scales: of 64 rows, or of a wavefront's columns
+  constexpr int kRowScales = (BM + BN) * kB, kColumnScales = kRowScales + BM * 4;
+  constexpr int kStage = kColumnScales + WN * 256;
   static_assert(NT % 4 == 0 && XL >= 1 && WL >= 1 && kB % (BN / WN) == 0, "a wavefront's columns share a scale block");
+  static_assert(BM >= 64 && WAVES >= BM / 64 + WN, "a wavefront fetches the scales of 64 rows or of its columns");
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  int* const s_blocks = reinterpret_cast<int*>(smem + STAGES * kStage);  // [E] row blocks up to an expert and its own
+  int* const s_rows = s_blocks + a.E;                                    // [E] rows likewise
   const int lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
 
-  // 32 tiles at a time per XCD, four row blocks wide, so that they share both operands in its L2
-  const int xcd = blockIdx.x % kXcds, idx = blockIdx.x / kXcds;
-  const int t = ((idx / kCusPerXcd) * kXcds + xcd) * kCusPerXcd + idx % kCusPerXcd;
-  const int per = kPatchRows * a.tiles_n;
-  const int block = __builtin_amdgcn_readfirstlane(t / per * kPatchRows + t % kPatchRows);
-  const int n0 = __builtin_amdgcn_readfirstlane(t % per / kPatchRows * BN);
-  const Block at = find_block(a, block, BM_BITS);
-  if (at.rows == 0) return;
+  if (wave == 0) {
+    int carry_b = 0, carry_m = 0;
+    for (int base = 0; base < a.E; base += kWave) {
+      const int given = a.loads[min(base + lane, a.E - 1)];
+      const int m = base + lane < a.E ? max(given, 0) : 0;
+      const int incl_b = carry_b + wave_inclusive_scan((m + BM - 1) >> BM_BITS), incl_m = carry_m + wave_inclusive_scan(m);
+      if (base + lane < a.E) s_blocks[base + lane] = incl_b, s_rows[base + lane] = incl_m;
+      carry_b = read_lane(incl_b, kWave - 1);
+      carry_m = read_lane(incl_m, kWave - 1);
+    }
+  }
+  __syncthreads();
+  const int blocks = __builtin_amdgcn_readfirstlane(s_blocks[a.E - 1]);
+  // Tiles are dealt out in runs, one per XCD and round; four row blocks wide, so that a run shares both operands in its L2.
+  const int run = gridDim.x / kXcds, per = kPatchRows * a.tiles_n;
+  const long tiles = static_cast<long>(blocks) * a.tiles_n;
+  long t = static_cast<long>(blockIdx.x % kXcds) * run + blockIdx.x / kXcds;
+  struct Tile {
+    int e, row0, rows, n0;
+  };
+  auto tile_at = [&](int t) {
+    const int group = t / per, in = t - group * per, wide = min(kPatchRows, blocks - group * kPatchRows);
+    const int block = __builtin_amdgcn_readfirstlane(group * kPatchRows + in % wide);
+    int e = 0;
+    for (int base = 0; base < a.E; base += kWave) {
+      const unsigned long long hit = __ballot(base + lane < a.E && block < s_blocks[min(base + lane, a.E - 1)]);
+      if (hit != 0) {
+        e = base + __builtin_ctzll(hit);
+        break;
+      }
+    }
+    const int before = e > 0 ? s_blocks[e - 1] : 0, first = e > 0 ? s_rows[e - 1] : 0;
+    const int seat0 = (block - before) << BM_BITS, row0 = first + seat0;
+    Tile at;
+    at.e = __builtin_amdgcn_readfirstlane(e);
+    at.row0 = __builtin_amdgcn_readfirstlane(row0);
+    at.rows = __builtin_amdgcn_readfirstlane(max(0, min(min(BM, s_rows[e] - row0), a.P - row0)));
+    at.n0 = __builtin_amdgcn_readfirstlane(in / wide * BN);
+    return at;
+  };
+  if (t >= tiles) return;
 
-  const i32x4 rx = make_rsrc(static_cast<const uint8_t*>(a.x) + static_cast<size_t>(at.row0) * a.pitch, static_cast<size_t>(at.rows) * a.pitch);
-  const i32x4 rw = make_rsrc(a.w + (static_cast<size_t>(at.e) * a.N + n0) * a.K, static_cast<size_t>(min(BN, a.N - n0)) * a.K);
   // Slot s of LDS row r holds chunk s ^ key(r) of that row.  The keys make any 16 rows that are read together at one chunk cover
   // all banks: 16 neighbours of x; of w the rows 8 g + r + constant, g and r in 0..3 (see the columns below).
   uint32_t ox[XL], ow[WL];
-  const int sub = lane >> 3, slot = lane & 7;
+  auto x_chunk = [&](int l, int i) { return (l & 7) ^ ((((wave * XL + i) * 8 + (l >> 3)) >> 1) & 7); };
+  auto w_chunk = [&](int l, int i) {
+    const int r = (wave * WL + i) * 8 + (l >> 3);
+    return (l & 7) ^ (((r >> 1) & 1) | ((r >> 3) & 3) << 1);
+  };
 #pragma unroll
-  for (int i = 0; i < XL; ++i) {
-    const int r = (wave * XL + i) * 8 + sub;
-    ox[i] = r < at.rows ? r * a.pitch + (slot ^ ((r >> 1) & 7)) * 16 : kNowhere;
-  }
+  for (int i = 0; i < XL; ++i) ox[i] = ((wave * XL + i) * 8 + (lane >> 3)) * a.pitch + x_chunk(lane, i) * 16;
 #pragma unroll
-  for (int i = 0; i < WL; ++i) {
-    const int r = (wave * WL + i) * 8 + sub;
-    ow[i] = r < a.N - n0 ? r * a.K + (slot ^ (((r >> 1) & 1) | ((r >> 3) & 3) << 1)) * 16 : kNowhere;
-  }
+  for (int i = 0; i < WL; ++i) ow[i] = ((wave * WL + i) * 8 + (lane >> 3)) * a.K + w_chunk(lane, i) * 16;
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem)));
-  auto request = [&](int kt) {
-    const uint32_t from = kt * kB, to = lds0 + (kt & 1) * kStage;
-    if (kt == a.KB - 1 && a.K % kB != 0) {  // a last K-step that K does not fill: chunks behind K read as zeros
+  // a last K-step that K does not fill (-1: there is none): its chunks behind K are turned to nowhere
+  const int part = __builtin_amdgcn_readfirstlane(a.K % kB != 0 ? a.KB - 1 : -1);
+  // What is requested next: K-step ahead_kt of a tile.  Rows and columns that do not exist are past the buffers' extents: they
+  // read as zeros and cost no request.  The first wavefronts bring the scales of 64 rows each, the next ones those of WN's columns.
+  int ahead_kt = 0;
+  uint32_t into = 0;  // the stage that the request fills
+  i32x4 rx, rw;
+  uint64_t scales_at;
+  int scales_bytes;
+  constexpr int kRowWaves = BM / 64;
+  const int scales_of = wave < kRowWaves + WN ? wave : 0;
+  const bool column_scales = scales_of >= kRowWaves;
+  const uint32_t scales_to = column_scales ? kColumnScales + (scales_of - kRowWaves) * 256 : kRowScales + scales_of * 256;
+  const uint64_t scales_step = column_scales ? 4 : static_cast<uint64_t>(a.P) * 4;
+  auto aim = [&](const Tile& at) {
+    ahead_kt = 0;
+    rx = make_rsrc(static_cast<const uint8_t*>(a.x) + static_cast<size_t>(at.row0) * a.pitch, static_cast<size_t>(at.rows) * a.pitch);
+    rw = make_rsrc(a.w + (static_cast<size_t>(at.e) * a.N + at.n0) * a.K, static_cast<size_t>(min(BN, a.N - at.n0)) * a.K);
+    const int column = min((at.n0 + (scales_of - kRowWaves) * (BN / WN)) / kB, a.NB - 1);
+    scales_at = column_scales ? reinterpret_cast<uint64_t>(a.sw + (static_cast<size_t>(at.e) * a.NB + column) * a.KB)
+                              : reinterpret_cast<uint64_t>(a.sx + at.row0 + scales_of * 64);
+    scales_bytes = column_scales ? 4 : max(0, min(64, at.rows - scales_of * 64)) * 4;
+  };
+  Tile at = tile_at(static_cast<int>(t));
+  aim(at);
+  auto request = [&] {
+    const uint32_t from = ahead_kt * kB, to = lds0 + into;
+    into = into == (STAGES - 1) * kStage ? 0 : into + kStage;
+    load_word_to_lds(make_rsrc(reinterpret_cast<const void*>(scales_at), scales_bytes), lane * 4, to + scales_to);
+    scales_at += scales_step;
+    if (ahead_kt != part) {
 #pragma unroll
-      for (int i = 0; i < XL; ++i) {
-        const int r = (wave * XL + i) * 8 + sub;
-        if (kt * kB + (slot ^ ((r >> 1) & 7)) * 16 >= a.K) ox[i] = kNowhere;
-      }
+      for (int i = 0; i < XL; ++i) load_to_lds(rx, ox[i], from, to + (wave * XL + i) * 1024);
 #pragma unroll
-      for (int i = 0; i < WL; ++i) {
-        const int r = (wave * WL + i) * 8 + sub;
-        if (kt * kB + (slot ^ (((r >> 1) & 1) | ((r >> 3) & 3) << 1)) * 16 >= a.K) ow[i] = kNowhere;
-      }
+      for (int i = 0; i < WL; ++i) load_to_lds(rw, ow[i], from, to + BM * kB + (wave * WL + i) * 1024);
+    } else {
+      int l = lane;
+      asm volatile("" : "+v"(l));  // (else what follows from it is kept in registers all through the K loop)
+#pragma unroll
+      for (int i = 0; i < XL; ++i)
+        load_to_lds(rx, from + x_chunk(l, i) * 16 >= static_cast<uint32_t>(a.K) ? kNowhere : ox[i], from, to + (wave * XL + i) * 1024);
+#pragma unroll
+      for (int i = 0; i < WL; ++i)
+        load_to_lds(rw, from + w_chunk(l, i) * 16 >= static_cast<uint32_t>(a.K) ? kNowhere : ow[i], from, to + BM * kB + (wave * WL + i) * 1024);
     }
-#pragma unroll
-    for (int i = 0; i < XL; ++i) load_to_lds(rx, ox[i], from, to + (wave * XL + i) * 1024);
-#pragma unroll
-    for (int i = 0; i < WL; ++i) load_to_lds(rw, ow[i], from, to + BM * kB + (wave * WL + i) * 1024);
+  };
+  // one K-step on, into the next tile of this workgroup at the end of one; false behind the last
+  auto step_ahead = [&] {
+    if (++ahead_kt < a.KB) return true;
+    t += gridDim.x;
+    if (t >= tiles) return false;
+    aim(tile_at(static_cast<int>(t)));
+    return true;
   };
 
   const int g = lane >> 4, c16 = lane & 15;
   // Row i of tile j's weight fragment is column (j / 4) 64 + (j / 2 % 2) 32 + (i / 4) 8 + (j % 2) 4 + i % 4: the results of
   // two tiles are then 8 neighbouring columns of a lane's row, and the four lanes of a row store 64 bytes side by side.
-  int wrow[4], xrow[MT];  // LDS offsets
-  uint32_t wkey[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int r = wn * (BN / WN) + (j >> 1) * 32 + (c16 >> 2) * 8 + (j & 1) * 4 + (c16 & 3);
-    wrow[j] = BM * kB + r * kB;
-    wkey[j] = ((r >> 1) & 1) | ((r >> 3) & 3) << 1;
-  }
-#pragma unroll
-  for (int i = 0; i < MT; ++i) xrow[i] = (wm * (BM / WM) + i * 16 + c16) * kB;
-  const uint32_t xkey = (c16 >> 1) & 7;
+  const int wr = wn * (BN / WN) + (c16 >> 2) * 8 + (c16 & 3), wkey = ((wr >> 1) & 1) | ((wr >> 3) & 3) << 1;
+  const int wlo = BM * kB + wr * kB + ((g ^ wkey) << 4), whi = BM * kB + wr * kB + (((g + 4) ^ wkey) << 4);  // chunks g and g + 4
+  const int xr = wm * (BM / WM) + c16, xkey = (c16 >> 1) & 7;
+  const int xlo = xr * kB + ((g ^ xkey) << 4), xhi = xr * kB + (((g + 4) ^ xkey) << 4);
+  auto column_of = [](int j) { return (j >> 2) * 64 + ((j >> 1) & 1) * 32 + (j & 1) * 4; };
 
-  const float* sx = a.sx + at.row0 + wm * (BM / WM) + c16;
-  const int last_row = a.P - 1 - (at.row0 + wm * (BM / WM) + c16);
-  const float* sw = a.sw + (static_cast<size_t>(at.e) * a.NB + min((n0 + wn * (BN / WN)) / kB, a.NB - 1)) * a.KB;
-  float sxv[MT], swv;
-  auto request_scales = [&](int kt) {
+  long done = t;
+  bool more = true;  // there is a K-step that has not been requested
 #pragma unroll
-    for (int i = 0; i < MT; ++i) sxv[i] = sx[static_cast<size_t>(kt) * a.P + min(i * 16, last_row)];
-    swv = sw[kt];
-  };
+  for (int q = 0; q < STAGES - 1; ++q)
+    if (more) {
+      request();
+      more = step_ahead();
+    }
+  using Operand = decltype(operand<EXACT>(i32x8{}));
+  uint32_t stage_at = 0;
+  f32x4 acc[MT][NT];
+  float s[MT];
+  Pipe<MT, NT> pipe;
+  for (;;) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      s[i] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+#pragma unroll 1
+    for (int kt = 0; kt < a.KB; ++kt) {
+      // (of the loads behind this K-step's all but STAGES - 2 steps' have been requested; behind the last request the count is less)
+      if (STAGES == 2 || !more) wait_loads_but<0>();
+      else wait_loads_but<(STAGES - 2) * kLoads>();
+      block_barrier();
+      const char* const stage = smem + stage_at;
+      stage_at = stage_at == (STAGES - 1) * kStage ? 0 : stage_at + kStage;
+      auto fragment = [&](int lo_at, int hi_at) {
+        const i32x4 lo = *reinterpret_cast<const i32x4*>(stage + lo_at), hi = *reinterpret_cast<const i32x4*>(stage + hi_at);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      };
+      i32x8 w = fragment(wlo, whi), x_read[MT];
+      float s_read[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        x_read[i] = fragment(xlo + i * 16 * kB, xhi + i * 16 * kB);
+        s_read[i] = *reinterpret_cast<const float*>(stage + kRowScales + (xr + i * 16) * 4);
+      }
+      const float scale = *reinterpret_cast<const float*>(stage + kColumnScales + wn * 256);
+      if (more) {
+        request();
+        more = step_ahead();
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      pipe.drain(acc, s);
+      Operand x[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        x[i] = operand<EXACT>(x_read[i]);
+        s[i] = s_read[i] * scale;
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const Operand at_hand = operand<EXACT>(w);
+        if (j + 1 < NT) w = fragment(wlo + column_of(j + 1) * kB, whi + column_of(j + 1) * kB);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) pipe.put(j * MT + i, multiply(at_hand, x[i]), acc, s);
+      }
+    }
+    pipe.drain(acc, s);
+    pipe.clear();
+    store_tile<MT, NT, EXACT>(a, Block{at.e, at.row0, at.rows}, wm * (BM / WM), at.n0 + wn * (BN / WN), acc);
+    done += gridDim.x;
+    if (done >= tiles) return;
+    at = tile_at(static_cast<int>(done));
+  }
+}
+
+// Few rows per expert: the weights are streamed once and set the time.  A workgroup takes 16 NT columns and 16 MT rows; its
+// W wavefronts take K-steps in turn (D of them in flight, weights straight into the fragments' registers) and add up their
+// sums through LDS.  Rows that are not 8-bit yet are quantized on the way in: the 32 elements that a lane holds of its row's
+// block are exactly its fragment, so that costs two exchanges among the row's four lanes and no launch of its own.
+template <int XDT, int MT, int NT, int W, int D, bool EXACT>
+__global__ __launch_bounds__(W * 64) void fp8_few_rows_kernel(Fp8Args a) {
+  constexpr bool kQuantized = XDT < 0;
+  constexpr int kBytes = kQuantized ? 1 : elem_bytes(XDT == BRT_F32 ? BRT_F32 : BRT_F16);
+  constexpr int kLoads = 2 * kBytes;  // 16-byte loads for a lane's 32 elements
+  constexpr int kBits = MT == 1 ? 4 : MT == 2 ? 5 : 6;
+  __shared__ f32x4 s_part[W > 1 ? W : 1][NT * MT][64];
+  const int lane = lane_id(), g = lane >> 4, c16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int block = blockIdx.x / a.tiles_n, n0 = (blockIdx.x - block * a.tiles_n) * 16 * NT;
+  const Block at = find_block(a, block, kBits);
+  if (at.rows == 0) return;
+  const int pitch = a.pitch * kBytes;
+  const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<char*>(static_cast<const char*>(a.x)) + static_cast<size_t>(at.row0) * pitch, 0, at.rows * pitch, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(a.w) + (static_cast<size_t>(at.e) * a.N + n0) * a.K, 0, min(16 * NT, a.N - n0) * a.K, 0x00020000);
+  const float* sw = a.sw + (static_cast<size_t>(at.e) * a.NB + n0 / kB) * a.KB;
+
+  // the biases of the tiles that this wavefront finishes: fetched ahead of the weights, not behind the last barrier
+  constexpr int kFinished = (MT * NT + W - 1) / W;
+  float bias[kFinished][4];
+#pragma unroll
+  for (int f = 0; f < kFinished; ++f) biases<4>(a, at.e, n0 + (wave + f * W) % NT * 16 + g * 4, bias[f]);
 
   f32x4 acc[MT][NT];
 #pragma unroll
@@ -296,70 +540,185 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  request_scales(0);
-  request(0);
-  for (int kt = 0; kt < a.KB; ++kt) {
-    wait_loads_all();
-    block_barrier();
-    float s[MT];
+  for (int kb0 = wave; kb0 < a.KB; kb0 += W * D) {
+    u32x4 wv[D][NT][2], xv[D][MT][kLoads];
+    float scale[D], given[D][MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) s[i] = sxv[i] * swv;
-    if (kt + 1 < a.KB) {
-      request_scales(kt + 1);
-      request(kt + 1);
-    }
-    const char* const stage = smem + (kt & 1) * kStage;
-    decltype(operand<EXACT>(i32x8{})) x[MT];
+    for (int d = 0; d < D; ++d) {
+      const int kb = kb0 + d * W;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const i32x4 lo = *reinterpret_cast<const i32x4*>(stage + xrow[i] + ((g ^ xkey) << 4));
-      const i32x4 hi = *reinterpret_cast<const i32x4*>(stage + xrow[i] + (((g + 4) ^ xkey) << 4));
-      x[i] = operand<EXACT>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      for (int h = 0; h < 2; ++h) {  // the lane's chunks of 16: g and g + 4
+        const bool there = kb * kB + h * 64 + g * 16 < a.K;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          wv[d][j][h] = __builtin_amdgcn_raw_buffer_load_b128(rw, there ? (j * 16 + c16) * a.K + h * 64 + g * 16 : kNowhere, kb * kB, 0);
+      }
+      scale[d] = sw[min(kb, a.KB - 1)];
     }
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const char* const from = stage + wrow[j & 3] + (j >> 2) * 64 * kB;
-      const i32x4 lo = *reinterpret_cast<const i32x4*>(from + ((g ^ wkey[j & 3]) << 4));
-      const i32x4 hi = *reinterpret_cast<const i32x4*>(from + (((g + 4) ^ wkey[j & 3]) << 4));
-      const auto w = operand<EXACT>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    for (int d = 0; d < D; ++d) {
+      const int kb = kb0 + d * W;
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        const f32x4 part = multiply(w, x[i]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[i][j][q] = __builtin_fmaf(part[q], s[i], acc[i][j][q]);
+        for (int l = 0; l < kLoads; ++l) {
+          const int h = l / kBytes;
+          const bool there = kb * kB + h * 64 + g * 16 < a.K;
+          xv[d][i][l] = __builtin_amdgcn_raw_buffer_load_b128(
+              rx, there ? (i * 16 + c16) * pitch + (h * 64 + g * 16) * kBytes + (l % kBytes) * 16 : kNowhere, kb * kB * kBytes, 0);
+        }
+        if constexpr (kQuantized)
+          given[d][i] = a.sx[static_cast<size_t>(min(kb, a.KB - 1)) * a.P + at.row0 + min(i * 16 + c16, at.rows - 1)];
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      decltype(operand<EXACT>(i32x8{})) x[MT];
+      float s[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        i32x8 q;
+        if constexpr (kQuantized) {
+#pragma unroll
+          for (int l = 0; l < 2; ++l)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) q[4 * l + c] = static_cast<int>(xv[d][i][l][c]);
+          s[i] = given[d][i] * scale[d];
+        } else {
+          constexpr int NE = 16 / kBytes;
+          float v[32];
+          uint32_t top = 0;
+#pragma unroll
+          for (int l = 0; l < kLoads; ++l) {
+            float part[NE];
+            unpack<XDT, 16>(xv[d][i][l], part);
+#pragma unroll
+            for (int c = 0; c < NE; ++c) {
+              v[l * NE + c] = part[c];
+              top = max(top, magnitude(part[c]));
+            }
+          }
+          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, kWave)));
+          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, kWave)));
+          float own, inverse;
+          scale_of(top, &own, &inverse);
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            q[c] = static_cast<int>(pack4(v[4 * c] * inverse, v[4 * c + 1] * inverse, v[4 * c + 2] * inverse, v[4 * c + 3] * inverse));
+          s[i] = own * scale[d];
+        }
+        x[i] = operand<EXACT>(q);
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        i32x8 v;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[4 * h + c] = static_cast<int>(wv[d][j][h][c]);
+        const auto w = operand<EXACT>(v);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const f32x4 part = multiply(w, x[i]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) acc[i][j][q] = __builtin_fmaf(part[q], s[i], acc[i][j][q]);
+        }
       }
     }
   }
 
-  const bool whole = a.N % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int r = wm * (BM / WM) + i * 16 + c16;
-    if (r >= at.rows) continue;
+  for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < NT; j += 2) {
-      float v[8];
+    for (int j = 0; j < NT; ++j) s_part[wave][i * NT + j][lane] = acc[i][j];
+  __syncthreads();
+  const bool whole = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] = acc[i][j][q], v[4 + q] = acc[i][j + 1][q];
-      finish<8>(a, at.e, static_cast<size_t>(at.row0) + r, n0 + wn * (BN / WN) + (j >> 2) * 64 + ((j >> 1) & 1) * 32 + g * 8, whole, v);
-    }
+  for (int f = 0; f < kFinished; ++f) {
+    const int p = wave + f * W;
+    if (p >= MT * NT) break;
+    f32x4 sum = s_part[0][p][lane];
+#pragma unroll
+    for (int w = 1; w < W; ++w) sum += s_part[w][p][lane];
+    const int r = p / NT * 16 + c16;
+    float v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = sum[q];
+    if (r < at.rows) finish<4>(a, static_cast<size_t>(at.row0) + r, n0 + p % NT * 16 + g * 4, whole, bias[f], v);
   }
 }
 
-template <int BM_BITS, int BN, int WM, int WN, bool EXACT = false>
+template <int XDT, int MT, int NT, int W, int D, bool EXACT>
+int launch_few_rows(Fp8Args& a, hipStream_t st) {
+  constexpr int kRows = 16 * MT;
+  const long blocks = static_cast<long>(a.P) / kRows + std::min(a.E, a.P);
+  a.tiles_n = (a.N + 16 * NT - 1) / (16 * NT);
+  if (blocks * a.tiles_n >= (1l << 31)) return fail(BRT_E_UNSUPPORTED, "too many tiles");
+  hipLaunchKernelGGL((fp8_few_rows_kernel<XDT, MT, NT, W, D, EXACT>), dim3(static_cast<unsigned>(blocks * a.tiles_n)), dim3(W * 64), 0, st, a);
+  return check_launch("fp8_few_rows_kernel");
+}
+// Rows and columns of a workgroup, wavefronts that share K, K-steps in flight.  `tiles` of 16 columns is what there is to deal
+// out (the loads are on the device: every expert is taken to have rows where there are as many rows).  Few of them: as many
+// wavefronts as possible on each; many: more columns to a wavefront, which quantizes the rows once for all of them.
+template <int XDT, bool EXACT>
+int launch_few_rows(Fp8Args& a, hipStream_t st) {
+  const long tiles = static_cast<long>(std::min(a.E, a.P)) * ((a.N + 15) / 16);
+  if (a.P > 16 && a.P > 10l * a.E) {
+    if (tiles < 1024) return launch_few_rows<XDT, 2, 2, 8, 1, EXACT>(a, st);
+    return launch_few_rows<XDT, 2, 4, 4, 1, EXACT>(a, st);
+  }
+  if (tiles < 512) return launch_few_rows<XDT, 1, 1, 16, 1, EXACT>(a, st);
+  if (tiles < 1536) return launch_few_rows<XDT, 1, 2, 8, 1, EXACT>(a, st);
+  if (tiles < 4096) return launch_few_rows<XDT, 1, 4, 8, 1, EXACT>(a, st);
+  return launch_few_rows<XDT, 1, 4, 4, 1, EXACT>(a, st);
+}
+template <int XDT>
+int launch_few_rows(Fp8Args& a, hipStream_t st) {
+  return a.out_dtype == BRT_F32 ? launch_few_rows<XDT, true>(a, st) : launch_few_rows<XDT, false>(a, st);
+}
+// Which shapes the kernel for few rows takes: those of few tiles, whose time is a launch and the chain of loads behind it.  It needs
+// no launch to quantize the rows, but quantizes them again for every 16 to 64 columns (with the launch counted, us here / 64 x 128
+// or 64 x 64 tiles): 1 row 1024 -> 1024 4.0 / 8; 48 rows of 8 experts 1024 -> 4096 10.0 / 11.2; 64 rows 4096 -> 4096 15.3 / 18.8; 100
+// rows of 4 experts 8192 -> 1024 24.8 / 32.2; but 128 rows of 32 experts 1024 -> 4096 31.4 / 30.4, 200 of 64 768 -> 2048 23.9 / 22.3,
+// 190 of 8 1024 -> 4096 15.2 / 12.4.
+bool few_rows(int P, int E, int N) {
+  if (E > kMostExperts || P <= 16) return true;
+  const long used = std::min(E, P);
+  if (P <= 10l * E) return used * ((N + 15) / 16) <= 4096;
+  return P <= 128 && ((P + 31) / 32 + used - 1) * ((N + 31) / 32) <= 320;
+}
+
+template <int BM_BITS, int BN, int WM, int WN, int STAGES, bool EXACT = false>
 int launch_tiles(Fp8Args& a, hipStream_t st) {
-  constexpr int kLds = 2 * ((1 << BM_BITS) + BN) * kB;
-  const auto fn = fp8_tiles_kernel<BM_BITS, BN, WM, WN, EXACT>;
-  if (const int rc = allow_dynamic_lds(reinterpret_cast<const void*>(fn), kLds); rc != BRT_OK) return rc;
+  constexpr int kStage = ((1 << BM_BITS) + BN) * kB + (1 << BM_BITS) * 4 + WN * 256;
+  constexpr int kResident = STAGES * kStage <= 80 * 1024 - kMostExperts * 8 ? 2 : 1;  // workgroups of a CU
+  const auto fn = fp8_tiles_kernel<BM_BITS, BN, WM, WN, STAGES, EXACT>;
+  if (const int rc = allow_dynamic_lds(reinterpret_cast<const void*>(fn), STAGES * kStage + kMostExperts * 8); rc != BRT_OK) return rc;
   a.tiles_n = (a.N + BN - 1) / BN;
   // an expert adds at most one row block that it does not fill
-  const long blocks = (static_cast<long>(a.P) >> BM_BITS) + std::min(a.E, a.P);
-  const long tiles = (blocks + kPatchRows - 1) / kPatchRows * kPatchRows * a.tiles_n;
-  const long round = kXcds * kCusPerXcd;
-  const long grid = (tiles + round - 1) / round * round;
-  if (grid >= (1l << 31)) return fail(BRT_E_UNSUPPORTED, "too many tiles");
-  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(WM * WN * 64), kLds, st, a);
+  const long tiles = ((static_cast<long>(a.P) >> BM_BITS) + std::min(a.E, a.P)) * a.tiles_n;
+  if (tiles >= (1l << 31)) return fail(BRT_E_UNSUPPORTED, "too many tiles");
+  const long grid = std::min<long>((tiles + kXcds - 1) / kXcds * kXcds, kResident * kXcds * kCusPerXcd);
+  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(WM * WN * 64), STAGES * kStage + a.E * 8, st, a);
   return check_launch("fp8_tiles_kernel");
+}
+
+// Tiles by what there is to deal out, a list's last row blocks taken as half full (us; without the launch that quantizes):
+//   64 x 64, four stages, while they go once round the chip: 400 rows of 8 experts 1024 -> 4096 12.8, 64 x 128 tiles 15.2;
+//   64 x 128, three stages, while 128 x 256 tiles do not, and for less than 64 rows an expert: 1500 rows of 4 experts 768 -> 2048
+//   12.4, 64 x 64 16.4, 128 x 256 15.4; 2048 rows of 128 experts 1024 -> 2048 59, 128 x 256 61;
+//   256 x 256, two stages, from two rounds and 1024 rows an expert on: 16384 rows of 8 experts 4096 -> 4096 300, 128 x 256 330;
+//   128 x 256, three stages, otherwise: 8192 rows of 64 experts 1024 -> 4096 80, 128 x 128 84, 256 x 256 85; 16384 rows of 32
+//   experts 4096 -> 1024 110, 256 x 256 124.
+int launch_any_tiles(Fp8Args& a, hipStream_t st) {
+  const long used = std::min(a.E, a.P);
+  auto tiles = [&](int rows, int columns) { return (2l * a.P / rows + used + 1) / 2 * ((a.N + columns - 1) / columns); };
+  const bool once = tiles(64, 64) <= 640;
+  if (a.out_dtype == BRT_F32) return once ? launch_tiles<6, 64, 2, 1, 4, true>(a, st) : launch_tiles<7, 128, 2, 2, 2, true>(a, st);
+  if (once) return launch_tiles<6, 64, 2, 1, 4>(a, st);
+  if (tiles(128, 256) < 256 || a.P < 64l * a.E) return launch_tiles<6, 128, 2, 2, 3>(a, st);
+  if (a.P >= 1024l * a.E && tiles(256, 256) >= 512) return launch_tiles<8, 256, 4, 2, 2>(a, st);
+  return launch_tiles<7, 256, 2, 4, 3>(a, st);
 }
 
 }  // namespace
@@ -386,10 +745,15 @@ extern "C" int brt_hip_quantize_rows(const void* x, int P, int K, int dtype, voi
   return check_launch("quantize_rows_kernel");
 }
 
-extern "C" int brt_hip_grouped_gemm_fp8(const void* x, int pitch, const float* x_scales, const void* w, const float* w_scales,
-                                        const int32_t* loads, const void* bias, int bias_dtype, void* out, int out_dtype, int E,
-                                        int P, int N, int K, int activation, void* stream) {
+extern "C" int brt_hip_grouped_gemm_fp8_quantizes(int E, int P, int N) { return few_rows(P, E, N) ? 1 : 0; }
+
+extern "C" int brt_hip_grouped_gemm_fp8(const void* x, int x_dtype, int pitch, const float* x_scales, const void* w,
+                                        const float* w_scales, const int32_t* loads, const void* bias, int bias_dtype, void* out,
+                                        int out_dtype, int E, int P, int N, int K, int activation, void* stream) {
   if (E <= 0 || P < 0 || N < 0 || K < 0 || pitch < K) return fail(BRT_E_INVALID, "bad shape E=%d P=%d N=%d K=%d pitch=%d", E, P, N, K, pitch);
+  const bool quantized = x_scales != nullptr;
+  if (!quantized && x_dtype != BRT_F32 && x_dtype != BRT_F16 && x_dtype != BRT_BF16)
+    return fail(BRT_E_UNSUPPORTED, "dtype %d is not supported", x_dtype);
   if (out_dtype != BRT_F32 && out_dtype != BRT_F16 && out_dtype != BRT_BF16) return fail(BRT_E_UNSUPPORTED, "dtype %d is not supported", out_dtype);
   if (bias && bias_dtype != BRT_F32 && bias_dtype != BRT_F16 && bias_dtype != BRT_BF16)
     return fail(BRT_E_UNSUPPORTED, "bias dtype %d is not supported", bias_dtype);
@@ -397,16 +761,22 @@ extern "C" int brt_hip_grouped_gemm_fp8(const void* x, int pitch, const float* x
     return fail(BRT_E_UNSUPPORTED, "activation %d is not supported", activation);
   if (P == 0 || N == 0) return BRT_OK;
   if (K == 0) return fail(BRT_E_UNSUPPORTED, "rows of no elements");
-  if (!x || !x_scales || !w || !w_scales || !loads || !out) return fail(BRT_E_INVALID, "null argument");
+  if (!x || !w || !w_scales || !loads || !out) return fail(BRT_E_INVALID, "null argument");
   if (K % 16 != 0 || pitch % 16 != 0 || !aligned(x, 16) || !aligned(w, 16))
     return fail(BRT_E_UNSUPPORTED, "rows must be whole, aligned units of 16 elements (K=%d)", K);
-  if (pitch > (1 << 22)) return fail(BRT_E_UNSUPPORTED, "rows of more than 4 Mi elements");  // (256 of them are addressed by 31 bits)
+  if (pitch > (1 << 20)) return fail(BRT_E_UNSUPPORTED, "rows of more than 1 Mi elements");  // (256 of them are addressed by 31 bits)
+  if (!quantized && !few_rows(P, E, N)) return fail(BRT_E_UNSUPPORTED, "rows for the wide tiles are quantized beforehand");
   Fp8Args a{};
   a.x = x; a.sx = x_scales; a.w = static_cast<const uint8_t*>(w); a.sw = w_scales; a.loads = loads;
   a.bias = bias; a.bias_dtype = bias_dtype; a.out = out; a.out_dtype = out_dtype; a.act = activation;
   a.pitch = pitch; a.E = E; a.P = P; a.N = N; a.K = K;
   a.KB = (K + kB - 1) / kB; a.NB = (N + kB - 1) / kB;
-  if (out_dtype == BRT_F32) return launch_tiles<7, 128, 2, 2, true>(a, as_stream(stream));
-  if (P > 160 * static_cast<long>(E) && N > 128) return launch_tiles<8, 256, 4, 2>(a, as_stream(stream));
-  return launch_tiles<7, 128, 2, 2>(a, as_stream(stream));
+  hipStream_t st = as_stream(stream);
+  if (few_rows(P, E, N)) {
+    if (quantized) return launch_few_rows<-1>(a, st);
+    if (x_dtype == BRT_F32) return launch_few_rows<BRT_F32>(a, st);
+    if (x_dtype == BRT_F16) return launch_few_rows<BRT_F16>(a, st);
+    return launch_few_rows<BRT_BF16>(a, st);
+  }
+  return launch_any_tiles(a, st);
 }

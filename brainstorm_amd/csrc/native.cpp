@@ -1041,11 +1041,15 @@ PyObject* grouped_linear_fp8(const Args& a) {
     if (!aligned16(rows)) rows = rows.clone();
     pitch = in_place ? x.stride(0) : K;
     scales = x_scales.t().contiguous();
+  } else if (brt_hip_grouped_gemm_fp8_quantizes(E, P, N)) {
+    data_type(x, "x data type");
+    rows = dense(x), pitch = K;
+    if (!aligned16(rows)) rows = rows.clone();
   } else {
     const Blocks b = quantized(x, "x");
     rows = b.q, scales = b.scales, pitch = b.q.size(1);
   }
-  check(brt_hip_grouped_gemm_fp8(ptr(rows), pitch, fptr(scales), ptr(weight), fptr(weight_scales), iptr(loads), ptr(bias),
+  check(brt_hip_grouped_gemm_fp8(ptr(rows), code_of(rows.scalar_type()), pitch, fptr(scales), ptr(weight), fptr(weight_scales), iptr(loads), ptr(bias),
                                  bias.defined() ? code_of(bias.scalar_type()) : BRT_F32, ptr(out), code_of(out.scalar_type()), E, P, N, K,
                                  a.integer(5), stream_of(x)));
   return out_blocks ? as_rows(quantized(out, "out"), N) : wrap(out);

@@ -511,7 +511,8 @@ int brt_hip_combine_by_rows_grad(const void* grad, const void* rows, const float
  *
  * brt_hip_grouped_gemm_fp8: for the rows r of expert e (packed by expert, rows behind the last one's are not written)
  *     out[r,n] = act(sum_kb x_scales[kb,r] * w_scales[e,n/128,kb] * (sum over block kb of x[r,k] * w[e,n,k]) + bias[e,n]),
- *   x rows of `pitch` >= K bytes, w [E,N,K], w_scales [E,ceil(N/128),KB], bias [E,N] of bias_dtype or NULL, out [P,N] of
+ *   x e4m3 rows of `pitch` >= K elements with x_scales; or, where brt_hip_grouped_gemm_fp8_quantizes(E, P, N) is 1 (few rows per
+ *   expert) and x_scales is NULL, rows of x_dtype, which the kernel quantizes itself to the same bits.  w [E,N,K], w_scales [E,ceil(N/128),KB], bias [E,N] of bias_dtype or NULL, out [P,N] of
  *   out_dtype.  The blocks are added in fp32, in order; the result is rounded once.  A block's sum for an fp32 result is one of
  *   exact products; for a 16-bit result it is the 8-bit matrix instruction's, which drops the bits of a product that lie more
  *   than 13 below the largest one of 16 (1.3e-5 of the result's norm on normal data).
@@ -519,9 +520,10 @@ int brt_hip_combine_by_rows_grad(const void* grad, const void* rows, const float
  * K is a multiple of 16, and x, q and w are 16-byte aligned; N is any number.
  */
 int brt_hip_quantize_rows(const void* x, int P, int K, int dtype, void* q, int pitch, float* scales, void* stream);
-int brt_hip_grouped_gemm_fp8(const void* x, int pitch, const float* x_scales, const void* w, const float* w_scales,
-                             const int32_t* loads, const void* bias, int bias_dtype, void* out, int out_dtype, int E,
-                             int P, int N, int K, int activation, void* stream);
+int brt_hip_grouped_gemm_fp8(const void* x, int x_dtype, int pitch, const float* x_scales, const void* w,
+                             const float* w_scales, const int32_t* loads, const void* bias, int bias_dtype, void* out,
+                             int out_dtype, int E, int P, int N, int K, int activation, void* stream);
+int brt_hip_grouped_gemm_fp8_quantizes(int E, int P, int N);
 
 /*
  * brt_hip_grouped_gemm / _f32out / _routed / _routed_f32out / _by_rows on fp32 rows of x (16-byte aligned), which the

@@ -136,6 +136,8 @@ CASES = [  # rows, in, out, experts
     (1, 16, 1, 1), (1, 128, 64, 1), (1, 2048, 520, 4), (2, 1040, 129, 3), (5, 272, 136, 8), (17, 144, 72, 2), (48, 1024, 512, 8),
     (33, 512, 4, 1), (64, 640, 260, 1), (100, 384, 256, 130), (129, 256, 136, 1), (300, 2064, 200, 2), (700, 128, 384, 4),
     (513, 528, 264, 1), (777, 1152, 520, 2), (1500, 400, 300, 3),
+    # every kind of tile, with lists that workgroups walk in several tiles: see launch_any_tiles
+    (200, 256, 8200, 8), (2600, 144, 1030, 2), (3000, 272, 3000, 60), (3100, 128, 4104, 3), (2200, 256, 16400, 2), (900, 384, 2056, 120),
 ]
 
 
@@ -305,7 +307,7 @@ def test_arguments_are_checked_before_anything_runs():
     assert lib.brt_hip_quantize_rows(None, 4, 128, 0, None, 128, None, None) == -1
     assert lib.brt_hip_quantize_rows(None, 0, 128, 0, None, 128, None, None) == 0
     call = lambda E=2, P=4, N=64, K=128, pitch=128, act=0, out=0: lib.brt_hip_grouped_gemm_fp8(  # noqa: E731
-        None, pitch, None, None, None, None, None, 0, None, out, E, P, N, K, act, None)
+        None, 0, pitch, None, None, None, None, None, 0, None, out, E, P, N, K, act, None)
     assert call() == -1 and call(E=0) == -1 and call(pitch=64) == -1 and call(act=5) == -4 and call(out=7) == -4
     assert call(P=0) == 0 and call(N=0) == 0 and call(K=0, pitch=0) == -4
     assert lib.brt_hip_gate_topk_grad(None, None, None, None, None, 4, 4, 5, 0, 1, None) == -1
