@@ -124,7 +124,7 @@ class CompactRoute:
     matrix the reference would have produced, generated on first read."""
 
     __slots__ = ("path_ids", "weights", "loads", "counts", "seat_rows", "row_entries", "k", "cells",
-                 "paths", "single_path", "indices", "combined_into", "__weakref__")
+                 "paths", "single_path", "indices", "combined_into", "differentiable", "__weakref__")
 
     def __init__(self, path_ids, weights, loads, counts, seat_rows, row_entries, paths, indices):
         self.path_ids, self.weights = path_ids, weights
@@ -134,6 +134,7 @@ class CompactRoute:
         self.single_path = self.k == 1
         self.indices = indices       # lazily filled [cells, paths] seat indices (what the stacks carry)
         self.combined_into = None    # the tensor an expert kernel already stored the combined rows to
+        self.differentiable = False  # the combine carries gradients (set by a fabric built so)
 
     def owns(self, route_indices, loads) -> bool:
         return route_indices is self.indices and loads is self.loads

@@ -89,7 +89,8 @@ struct Fp8Args {
   const float* sw;     // [E, NB, KB]
   const int* loads;    // [E]
   const void* bias;    // [E, N] of bias_dtype or null
-  void* out;           // [P, N] of out_dtype
+  void* out;           // [P, N] of out_dtype, or with out_scales e4m3 [P, NB * 128]
+  float* out_scales;   // [NB][P] or null
   int pitch, bias_dtype, out_dtype, act;
   int E, P, N, K, KB, NB, tiles_n;
 };
@@ -296,11 +297,71 @@ __device__ __forceinline__ void store_tile(const Fp8Args& a, const Block& at, in
   else with_act(std::integral_constant<int, BRT_BF16>{});
 }
 
+// The same results rounded to bf16 and quantized: what quantize_rows makes of them, without their way through memory.  A scale
+// block is the columns of one wavefront (NT = 8) or of two neighbours (NT = 4), which exchange their largest values through
+// `exchange` ([WN][BM] words); every wavefront of the workgroup calls it.
+template <int ACT, int MT, int NT, int BM, int WN>
+__device__ __forceinline__ void store_blocks(const Fp8Args& a, const Block& at, int r0, int n0, int wn, uint32_t* exchange, f32x4 (&acc)[MT][NT]) {
+  static_assert(NT == 8 || (NT == 4 && WN % 2 == 0), "a block of 128 columns belongs to one wavefront or two");
+  const int lane = lane_id(), g = lane >> 4, c16 = lane & 15;
+  uint32_t top[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) top[i] = 0;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int n = n0 + (j >> 2) * 64 + ((j >> 1) & 1) * 32 + g * 8 + (j & 1) * 4;
+    float bias[4];
+    biases<4>(a, at.e, min(n, a.N - 1), bias);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        // (columns behind the last are zero; the value is held as the bf16 it was rounded to)
+        const float v = n + q < a.N ? bf16_to_float(float_to_bf16(apply_act<ACT>(acc[i][j][q] + bias[q]))) : 0.0f;
+        acc[i][j][q] = v;
+        top[i] = max(top[i], magnitude(v));
+      }
+    __builtin_amdgcn_sched_barrier(0);  // (the biases of all columns at once do not fit beside the accumulators)
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    top[i] = max(top[i], static_cast<uint32_t>(__shfl_xor(static_cast<int>(top[i]), 16, kWave)));
+    top[i] = max(top[i], static_cast<uint32_t>(__shfl_xor(static_cast<int>(top[i]), 32, kWave)));
+  }
+  if constexpr (NT == 4) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+      if (g == 0) exchange[wn * BM + r0 + i * 16 + c16] = top[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MT; ++i) top[i] = max(top[i], exchange[(wn ^ 1) * BM + r0 + i * 16 + c16]);
+  }
+  const int nb = n0 / kB;
+  uint8_t* const out = static_cast<uint8_t*>(a.out);
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int r = r0 + i * 16 + c16;
+    if (r >= at.rows || nb >= a.NB) continue;
+    const size_t row = static_cast<size_t>(at.row0) + r;
+    float scale, inverse;
+    scale_of(top[i], &scale, &inverse);
+    if (g == 0 && n0 % kB == 0) a.out_scales[static_cast<size_t>(nb) * a.P + row] = scale;
+#pragma unroll
+    for (int j = 0; j < NT; j += 2) {
+      u32x2 o;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        o[h] = pack4(acc[i][j + h][0] * inverse, acc[i][j + h][1] * inverse, acc[i][j + h][2] * inverse, acc[i][j + h][3] * inverse);
+      *reinterpret_cast<u32x2*>(out + row * (static_cast<size_t>(a.NB) * kB) + n0 + (j >> 2) * 64 + ((j >> 1) & 1) * 32 + g * 8) = o;
+    }
+  }
+}
+
 // BM x BN tiles, WM x WN wavefronts, STAGES K-steps of 128 bytes in LDS.  Operands and scales go straight into LDS; a K-step is
 // requested STAGES - 1 steps before it is multiplied, into the stage that was read last.  A workgroup stays for several tiles, and
 // its requests run on through their boundaries: a tile of 1024 elements has eight K-steps, and starting anew (which expert, the
 // first K-step) took as long as half of them.  The list of row blocks is kept in LDS for that.
-template <int BM_BITS, int BN, int WM, int WN, int STAGES, bool EXACT>
+template <int BM_BITS, int BN, int WM, int WN, int STAGES, bool GO_ROUND, bool EXACT, bool BLOCKS>
 __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
   constexpr int BM = 1 << BM_BITS, WAVES = WM * WN;
   constexpr int MT = BM / WM / 16, NT = BN / WN / 16;  // 16 x 16 tiles of a wavefront
@@ -313,6 +374,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   int* const s_blocks = reinterpret_cast<int*>(smem + STAGES * kStage);  // [E] row blocks up to an expert and its own
   int* const s_rows = s_blocks + a.E;                                    // [E] rows likewise
+  uint32_t* const s_tops = reinterpret_cast<uint32_t*>(s_rows + a.E);    // [WN][BM], where results are quantized
   const int lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
@@ -376,7 +438,10 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
   const int part = __builtin_amdgcn_readfirstlane(a.K % kB != 0 ? a.KB - 1 : -1);
   // What is requested next: K-step ahead_kt of a tile.  Rows and columns that do not exist are past the buffers' extents: they
   // read as zeros and cost no request.  The first wavefronts bring the scales of 64 rows each, the next ones those of WN's columns.
-  int ahead_kt = 0;
+  // With GO_ROUND a tile begins with the K-step of its number in the row of tiles: with all of them at one place of K, weight rows
+  // that are a power of two apart come from the same few memory channels (300 rows of 32 experts 4096 -> 4096 149 -> 103 us, 4224 ->
+  // 4096 100 either way).  Where weights are read from the L2 several times it costs 4 % and gains nothing.
+  int ahead_kt = 0, ahead_left = 0;
   uint32_t into = 0;  // the stage that the request fills
   i32x4 rx, rw;
   uint64_t scales_at;
@@ -387,12 +452,14 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
   const uint32_t scales_to = column_scales ? kColumnScales + (scales_of - kRowWaves) * 256 : kRowScales + scales_of * 256;
   const uint64_t scales_step = column_scales ? 4 : static_cast<uint64_t>(a.P) * 4;
   auto aim = [&](const Tile& at) {
-    ahead_kt = 0;
+    ahead_kt = GO_ROUND ? at.n0 / BN % a.KB : 0;
+    ahead_left = a.KB;
     rx = make_rsrc(static_cast<const uint8_t*>(a.x) + static_cast<size_t>(at.row0) * a.pitch, static_cast<size_t>(at.rows) * a.pitch);
     rw = make_rsrc(a.w + (static_cast<size_t>(at.e) * a.N + at.n0) * a.K, static_cast<size_t>(min(BN, a.N - at.n0)) * a.K);
     const int column = min((at.n0 + (scales_of - kRowWaves) * (BN / WN)) / kB, a.NB - 1);
     scales_at = column_scales ? reinterpret_cast<uint64_t>(a.sw + (static_cast<size_t>(at.e) * a.NB + column) * a.KB)
                               : reinterpret_cast<uint64_t>(a.sx + at.row0 + scales_of * 64);
+    if constexpr (GO_ROUND) scales_at += ahead_kt * scales_step;
     scales_bytes = column_scales ? 4 : max(0, min(64, at.rows - scales_of * 64)) * 4;
   };
   Tile at = tile_at(static_cast<int>(t));
@@ -420,7 +487,13 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
   };
   // one K-step on, into the next tile of this workgroup at the end of one; false behind the last
   auto step_ahead = [&] {
-    if (++ahead_kt < a.KB) return true;
+    if (GO_ROUND ? --ahead_left > 0 : ahead_kt + 1 < a.KB) {
+      if (++ahead_kt == a.KB && GO_ROUND) {
+        ahead_kt = 0;
+        scales_at -= a.KB * scales_step;
+      }
+      return true;
+    }
     t += gridDim.x;
     if (t >= tiles) return false;
     aim(tile_at(static_cast<int>(t)));
@@ -436,7 +509,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
   const int xlo = xr * kB + ((g ^ xkey) << 4), xhi = xr * kB + (((g + 4) ^ xkey) << 4);
   auto column_of = [](int j) { return (j >> 2) * 64 + ((j >> 1) & 1) * 32 + (j & 1) * 4; };
 
-  long done = t;
+  long done = t;  // (the same walk, for the tile that is multiplied)
   bool more = true;  // there is a K-step that has not been requested
 #pragma unroll
   for (int q = 0; q < STAGES - 1; ++q)
@@ -498,7 +571,17 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
     }
     pipe.drain(acc, s);
     pipe.clear();
-    store_tile<MT, NT, EXACT>(a, Block{at.e, at.row0, at.rows}, wm * (BM / WM), at.n0 + wn * (BN / WN), acc);
+    const Block rows_at{at.e, at.row0, at.rows};
+    if constexpr (BLOCKS) {
+      auto blocks = [&](auto act) {
+        store_blocks<decltype(act)::value, MT, NT, BM, WN>(a, rows_at, wm * (BM / WM), at.n0 + wn * (BN / WN), wn, s_tops, acc);
+      };
+      if (a.act == BRT_ACT_GELU) blocks(std::integral_constant<int, BRT_ACT_GELU>{});
+      else if (a.act == BRT_ACT_RELU) blocks(std::integral_constant<int, BRT_ACT_RELU>{});
+      else blocks(std::integral_constant<int, BRT_ACT_NONE>{});
+    } else {
+      store_tile<MT, NT, EXACT>(a, rows_at, wm * (BM / WM), at.n0 + wn * (BN / WN), acc);
+    }
     done += gridDim.x;
     if (done >= tiles) return;
     at = tile_at(static_cast<int>(done));
@@ -688,37 +771,59 @@ bool few_rows(int P, int E, int N) {
   return P <= 128 && ((P + 31) / 32 + used - 1) * ((N + 31) / 32) <= 320;
 }
 
-template <int BM_BITS, int BN, int WM, int WN, int STAGES, bool EXACT = false>
+template <int BM_BITS, int BN, int WM, int WN, int STAGES, bool GO_ROUND, bool EXACT, bool BLOCKS>
 int launch_tiles(Fp8Args& a, hipStream_t st) {
   constexpr int kStage = ((1 << BM_BITS) + BN) * kB + (1 << BM_BITS) * 4 + WN * 256;
-  constexpr int kResident = STAGES * kStage <= 80 * 1024 - kMostExperts * 8 ? 2 : 1;  // workgroups of a CU
-  const auto fn = fp8_tiles_kernel<BM_BITS, BN, WM, WN, STAGES, EXACT>;
-  if (const int rc = allow_dynamic_lds(reinterpret_cast<const void*>(fn), STAGES * kStage + kMostExperts * 8); rc != BRT_OK) return rc;
+  constexpr int kTops = BLOCKS && BN / WN < kB ? WN * (1 << BM_BITS) * 4 : 0;  // (a block's largest values pass between wavefronts)
+  constexpr int kMost = STAGES * kStage + kMostExperts * 8 + kTops;
+  constexpr int kResident = kMost <= 80 * 1024 ? 2 : 1;  // workgroups of a CU
+  const auto fn = fp8_tiles_kernel<BM_BITS, BN, WM, WN, STAGES, GO_ROUND, EXACT, BLOCKS>;
+  if (const int rc = allow_dynamic_lds(reinterpret_cast<const void*>(fn), kMost); rc != BRT_OK) return rc;
   a.tiles_n = (a.N + BN - 1) / BN;
   // an expert adds at most one row block that it does not fill
   const long tiles = ((static_cast<long>(a.P) >> BM_BITS) + std::min(a.E, a.P)) * a.tiles_n;
   if (tiles >= (1l << 31)) return fail(BRT_E_UNSUPPORTED, "too many tiles");
   const long grid = std::min<long>((tiles + kXcds - 1) / kXcds * kXcds, kResident * kXcds * kCusPerXcd);
-  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(WM * WN * 64), STAGES * kStage + a.E * 8, st, a);
+  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(WM * WN * 64), STAGES * kStage + a.E * 8 + kTops, st, a);
   return check_launch("fp8_tiles_kernel");
+}
+template <int BM_BITS, int BN, int WM, int WN, int STAGES, bool GO_ROUND = false>
+int launch_tiles(Fp8Args& a, hipStream_t st) {
+  if (a.out_scales != nullptr) return launch_tiles<BM_BITS, BN, WM, WN, STAGES, GO_ROUND, false, true>(a, st);
+  return launch_tiles<BM_BITS, BN, WM, WN, STAGES, GO_ROUND, false, false>(a, st);
 }
 
 // Tiles by what there is to deal out, a list's last row blocks taken as half full (us; without the launch that quantizes):
-//   64 x 64, four stages, while they go once round the chip: 400 rows of 8 experts 1024 -> 4096 12.8, 64 x 128 tiles 15.2;
+//   64 x 64, four stages, while they go once round the chip: 400 rows of 8 experts 1024 -> 4096 9.8, 64 x 128 12;
 //   64 x 128, three stages, while 128 x 256 tiles do not, and for less than 64 rows an expert: 1500 rows of 4 experts 768 -> 2048
-//   12.4, 64 x 64 16.4, 128 x 256 15.4; 2048 rows of 128 experts 1024 -> 2048 59, 128 x 256 61;
-//   256 x 256, two stages, from two rounds and 1024 rows an expert on: 16384 rows of 8 experts 4096 -> 4096 300, 128 x 256 330;
-//   128 x 256, three stages, otherwise: 8192 rows of 64 experts 1024 -> 4096 80, 128 x 128 84, 256 x 256 85; 16384 rows of 32
-//   experts 4096 -> 1024 110, 256 x 256 124.
+//   9, 64 x 64 13, 128 x 256 12; 2048 rows of 128 experts 1024 -> 2048 56, 128 x 256 58;
+//   128 x 256 and 256 x 256 by the rounds over the CUs that they take, at 1.05 and 1.75 us a K-step and 4 and 6 a tile: 8192 rows of
+//   64 experts 1024 -> 4096 80 and 85, 8192 of 32 4096 -> 1024 (two rounds and one) 86 and 76, 16384 of 8 4096 -> 4096 315 and 290.
+enum TileKind { k64x64, k64x128, k128x128, k128x256, k256x256 };
+TileKind tile_kind(int E, int P, int N, int K, int out_dtype) {
+  const long used = std::min(E, P);
+  auto tiles = [&](int rows, int columns) { return (2l * P / rows + used + 1) / 2 * ((N + columns - 1) / columns); };
+  if (tiles(64, 64) <= 640) return k64x64;
+  if (out_dtype == BRT_F32) return k128x128;
+  if (tiles(128, 256) < 256 || P < 64l * E) return k64x128;
+  const long cus = kXcds * kCusPerXcd, steps = (K + kB - 1) / kB;
+  const long wide = (tiles(256, 256) + cus - 1) / cus * (35 * steps + 120), half = (tiles(128, 256) + cus - 1) / cus * (21 * steps + 80);
+  return wide < half ? k256x256 : k128x256;
+}
+bool quantizes_result(int E, int P, int N, int K, int out_dtype) {
+  return !few_rows(P, E, N) && out_dtype == BRT_BF16 && tile_kind(E, P, N, K, out_dtype) != k64x64;
+}
 int launch_any_tiles(Fp8Args& a, hipStream_t st) {
-  const long used = std::min(a.E, a.P);
-  auto tiles = [&](int rows, int columns) { return (2l * a.P / rows + used + 1) / 2 * ((a.N + columns - 1) / columns); };
-  const bool once = tiles(64, 64) <= 640;
-  if (a.out_dtype == BRT_F32) return once ? launch_tiles<6, 64, 2, 1, 4, true>(a, st) : launch_tiles<7, 128, 2, 2, 2, true>(a, st);
-  if (once) return launch_tiles<6, 64, 2, 1, 4>(a, st);
-  if (tiles(128, 256) < 256 || a.P < 64l * a.E) return launch_tiles<6, 128, 2, 2, 3>(a, st);
-  if (a.P >= 1024l * a.E && tiles(256, 256) >= 512) return launch_tiles<8, 256, 4, 2, 2>(a, st);
-  return launch_tiles<7, 256, 2, 4, 3>(a, st);
+  TileKind kind = tile_kind(a.E, a.P, a.N, a.K, a.out_dtype);
+  // (quantizing 256 x 256 results needs more registers than there are: 8192 rows of 32 experts 1024 -> 4096 + GELU 101 us, 128 x 256 BLK)
+  if (kind == k256x256 && a.out_scales != nullptr) kind = k128x256;
+  switch (kind) {
+    case k64x64: return a.out_dtype == BRT_F32 ? launch_tiles<6, 64, 2, 1, 4, false, true, false>(a, st) : launch_tiles<6, 64, 2, 1, 4, false, false, false>(a, st);
+    case k64x128: return launch_tiles<6, 128, 2, 2, 3, true>(a, st);
+    case k128x128: return launch_tiles<7, 128, 2, 2, 2, false, true, false>(a, st);
+    case k128x256: return launch_tiles<7, 256, 2, 4, 3>(a, st);
+    default: return launch_tiles<8, 256, 4, 2, 2, false, false, false>(a, st);
+  }
 }
 
 }  // namespace
@@ -747,9 +852,13 @@ extern "C" int brt_hip_quantize_rows(const void* x, int P, int K, int dtype, voi
 
 extern "C" int brt_hip_grouped_gemm_fp8_quantizes(int E, int P, int N) { return few_rows(P, E, N) ? 1 : 0; }
 
+extern "C" int brt_hip_grouped_gemm_fp8_blocks(int E, int P, int N, int K, int out_dtype) {
+  return quantizes_result(E, P, N, K, out_dtype) ? 1 : 0;
+}
+
 extern "C" int brt_hip_grouped_gemm_fp8(const void* x, int x_dtype, int pitch, const float* x_scales, const void* w,
                                         const float* w_scales, const int32_t* loads, const void* bias, int bias_dtype, void* out,
-                                        int out_dtype, int E, int P, int N, int K, int activation, void* stream) {
+                                        int out_dtype, float* out_scales, int E, int P, int N, int K, int activation, void* stream) {
   if (E <= 0 || P < 0 || N < 0 || K < 0 || pitch < K) return fail(BRT_E_INVALID, "bad shape E=%d P=%d N=%d K=%d pitch=%d", E, P, N, K, pitch);
   const bool quantized = x_scales != nullptr;
   if (!quantized && x_dtype != BRT_F32 && x_dtype != BRT_F16 && x_dtype != BRT_BF16)
@@ -765,10 +874,12 @@ extern "C" int brt_hip_grouped_gemm_fp8(const void* x, int x_dtype, int pitch, c
   if (K % 16 != 0 || pitch % 16 != 0 || !aligned(x, 16) || !aligned(w, 16))
     return fail(BRT_E_UNSUPPORTED, "rows must be whole, aligned units of 16 elements (K=%d)", K);
   if (pitch > (1 << 20)) return fail(BRT_E_UNSUPPORTED, "rows of more than 1 Mi elements");  // (256 of them are addressed by 31 bits)
+  if (out_scales && (!quantizes_result(E, P, N, K, out_dtype) || !aligned(out, 16)))
+    return fail(BRT_E_UNSUPPORTED, "results of this shape are not quantized by the product's kernel");
   if (!quantized && !few_rows(P, E, N)) return fail(BRT_E_UNSUPPORTED, "rows for the wide tiles are quantized beforehand");
   Fp8Args a{};
   a.x = x; a.sx = x_scales; a.w = static_cast<const uint8_t*>(w); a.sw = w_scales; a.loads = loads;
-  a.bias = bias; a.bias_dtype = bias_dtype; a.out = out; a.out_dtype = out_dtype; a.act = activation;
+  a.bias = bias; a.bias_dtype = bias_dtype; a.out = out; a.out_dtype = out_dtype; a.out_scales = out_scales; a.act = activation;
   a.pitch = pitch; a.E = E; a.P = P; a.N = N; a.K = K;
   a.KB = (K + kB - 1) / kB; a.NB = (N + kB - 1) / kB;
   hipStream_t st = as_stream(stream);

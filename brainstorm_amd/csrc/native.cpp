@@ -226,6 +226,7 @@ variable_list gate(const Tensor& given, int64_t k, bool softmax, bool hot_mask) 
 
 struct GateTopk : Function<GateTopk> {
   static variable_list forward(AutogradContext* ctx, const Tensor& given, int64_t k, bool softmax, bool hot_mask) {
+    ctx->set_materialize_grads(false);  // (the ids' would be a fill of zeros in every pass)
     variable_list made = gate(given, k, softmax, hot_mask);
     ctx->mark_non_differentiable(hot_mask ? variable_list{made[0], made[2]} : variable_list{made[0]});
     ctx->save_for_backward({given, made[0], made[1]});
@@ -1027,9 +1028,14 @@ PyObject* grouped_linear_fp8(const Args& a) {
     if (out_blocks || (typed && type != out.scalar_type())) runtime_error("out is given: it says its type, and holds no blocks");
     if (data_type(out, "output data type") < 0 || out.sizes() != at::IntArrayRef({P, N}) || !out.is_contiguous())
       runtime_error("out must be a contiguous [rows, out_features] tensor");
-  } else {
-    out = empty({P, N}, type, x);
   }
+  if (out_blocks && N % 16 != 0) not_implemented("a result in blocks has a multiple of 16 columns");
+  const int out_type = out.defined() ? code_of(out.scalar_type()) : code_of(type);
+  Blocks made;  // the result, where the product's kernel quantizes it
+  if (out_blocks && brt_hip_grouped_gemm_fp8_blocks(E, P, N, K, out_type))
+    made = {empty({P, blocks_of(N) * kScaleBlock}, at::kByte, x), empty({blocks_of(N), P}, at::kFloat, x)};
+  else if (!out.defined())
+    out = empty({P, N}, type, x);
   const Tensor weight = dense(w), weight_scales = dense(w_scales), loads = dense(loads_given);
   const Tensor bias = bias_given.defined() ? dense(bias_given) : bias_given;
   Tensor rows, scales;
@@ -1050,9 +1056,9 @@ PyObject* grouped_linear_fp8(const Args& a) {
     rows = b.q, scales = b.scales, pitch = b.q.size(1);
   }
   check(brt_hip_grouped_gemm_fp8(ptr(rows), code_of(rows.scalar_type()), pitch, fptr(scales), ptr(weight), fptr(weight_scales), iptr(loads), ptr(bias),
-                                 bias.defined() ? code_of(bias.scalar_type()) : BRT_F32, ptr(out), code_of(out.scalar_type()), E, P, N, K,
-                                 a.integer(5), stream_of(x)));
-  return out_blocks ? as_rows(quantized(out, "out"), N) : wrap(out);
+                                 bias.defined() ? code_of(bias.scalar_type()) : BRT_F32, ptr(made.q.defined() ? made.q : out), out_type,
+                                 fptr(made.scales), E, P, N, K, a.integer(5), stream_of(x)));
+  return !out_blocks ? wrap(out) : as_rows(made.q.defined() ? made : quantized(out, "out"), N);
 }
 
 // ---- values on the host ------------------------------------------------------------------------------

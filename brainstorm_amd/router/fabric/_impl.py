@@ -396,10 +396,14 @@ class FusedDispatchFabric(DispatchFabric):
     (``route_by_path``): no ``[cells, paths]`` mask or seat matrix is written or read; the matrix on
     the tag stack is generated only if something reads it.  The rows are sized as with
     ``static_rows`` and moved by ``dispatch_by_rows``, or with ``defer_dispatch`` gathered by the
-    expert's first grouped GEMM; top-k routes with k > 1 are taken as well."""
+    expert's first grouped GEMM; top-k routes with k > 1 are taken as well.
+    ``differentiable=True`` (an extension, with ``compact_route=True``) makes the layer trainable: the dispatched rows carry
+    the gradient of the cells, and the combine of this route those of the expert's rows and of the score (where it weights
+    them).  Nothing is deferred then, and a residual is copied instead of written."""
 
     def __init__(self, flow_num: int, route_logic="1d", transform=False, **kwargs):
         kwargs["index_format"] = "seat_index"
+        differentiable = bool(kwargs.pop("differentiable", False))
         defer = bool(kwargs.pop("defer_dispatch", False))
         static_rows = bool(kwargs.pop("static_rows", False))
         compact = bool(kwargs.pop("compact_route", False))
@@ -407,6 +411,9 @@ class FusedDispatchFabric(DispatchFabric):
         self.defer_dispatch = defer
         self.static_rows = static_rows
         self.compact_route = compact
+        self.differentiable = differentiable
+        if differentiable and not compact:
+            raise ValueError("differentiable=True needs compact_route=True")
         self._host_caps_key = ()   # the capacity buffer the host copy below was read from
         self._host_caps_list = None
 
@@ -491,13 +498,16 @@ class FusedDispatchFabric(DispatchFabric):
         indices = lazy_tensor(_lib.native().matrix(cells, paths, torch.int32, data), fill_dense)
         route = c_router.CompactRoute(decision.path_ids, decision.scores, loads, counts, seat_rows,
                                       row_entries, paths, indices)
+        route.differentiable = differentiable = getattr(self, "differentiable", False)
         c_router.remember_route(loads, route)
         self.__dict__["_route"] = route
         self.capture_flow_stats(in_flows, indices, loads)  # (reads the dense matrix when capturing)
         level = len(tags) - 1
         extra = dict(extra or {})
         extra[_route_key(level)] = route
-        if (self.defer_dispatch and data.dim() == 2 and data.shape[1] % 8 == 0
+        if differentiable:
+            routed = c_router.dispatch_by_rows(data, row_entries, k, seat_rows=seat_rows)
+        elif (self.defer_dispatch and data.dim() == 2 and data.shape[1] % 8 == 0
                 and data.dtype in (torch.bfloat16, torch.float32)):
             routed = _lib.native().matrix(rows, data.shape[1], None, data)
             extra[_deferred_key(level)] = DeferredState(data, route, routed, _deferred_key(level))
@@ -511,6 +521,8 @@ class FusedDispatchFabric(DispatchFabric):
         if isinstance(hot_mask, CompactHotMask):
             if self._takes_compact(in_flows, runtime_capacities):
                 return self._forward_compact(in_flows, hot_mask, score)
+            if getattr(self, "differentiable", False):
+                raise NotImplementedError("a differentiable dispatch takes one flow of cells of whole, aligned 16-byte units")
             hot_mask = hot_mask.dense()  # a shape this path does not take: the mask, as the reference
         if not self._in_one_step(in_flows, runtime_capacities, hot_mask):
             return super().forward(in_flow, hot_mask, runtime_capacities, score, route)
@@ -604,6 +616,14 @@ class FusedCombineFabric(CombineFabric):
             return residual
         if data.size(0) != route.row_entries.numel():
             raise RuntimeError("the expert output does not have the rows of the dispatched layout")
+        if route.differentiable:
+            if gates is not None and (gates.dim() != 2 or gates.size(1) < route.paths):
+                raise RuntimeError(f"the score does not have a column for each of {route.paths} paths")
+            out = c_router.combine_by_rows(data, route.path_ids, route.seat_rows, gates=gates, row_entries=route.row_entries)
+            if residual is None:
+                return out
+            has_row = (route.seat_rows > 0).any(dim=1).view([-1] + [1] * (out.dim() - 1))
+            return torch.where(has_row, out, residual.view_as(out).to(out.dtype))
         if residual is not None and not residual.is_contiguous():
             raise RuntimeError("the residual must be contiguous (it is updated in place)")
         if route.k == 1 and gates is None:

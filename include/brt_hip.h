@@ -517,13 +517,17 @@ int brt_hip_combine_by_rows_grad(const void* grad, const void* rows, const float
  *   exact products; for a 16-bit result it is the 8-bit matrix instruction's, which drops the bits of a product that lie more
  *   than 13 below the largest one of 16 (1.3e-5 of the result's norm on normal data).
  *
+ *   With out_scales, where brt_hip_grouped_gemm_fp8_blocks(E, P, N, K, out_dtype) is 1, the result is rounded to out_dtype and
+ *   quantized as brt_hip_quantize_rows would quantize it: out is e4m3 [P,ceil(N/128)*128], out_scales [ceil(N/128),P].
+ *
  * K is a multiple of 16, and x, q and w are 16-byte aligned; N is any number.
  */
 int brt_hip_quantize_rows(const void* x, int P, int K, int dtype, void* q, int pitch, float* scales, void* stream);
 int brt_hip_grouped_gemm_fp8(const void* x, int x_dtype, int pitch, const float* x_scales, const void* w,
                              const float* w_scales, const int32_t* loads, const void* bias, int bias_dtype, void* out,
-                             int out_dtype, int E, int P, int N, int K, int activation, void* stream);
+                             int out_dtype, float* out_scales, int E, int P, int N, int K, int activation, void* stream);
 int brt_hip_grouped_gemm_fp8_quantizes(int E, int P, int N);
+int brt_hip_grouped_gemm_fp8_blocks(int E, int P, int N, int K, int out_dtype);
 
 /*
  * brt_hip_grouped_gemm / _f32out / _routed / _routed_f32out / _by_rows on fp32 rows of x (16-byte aligned), which the

@@ -168,16 +168,21 @@ def test_products(rows, k, n, experts, form, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,k,n,experts", [(3, 256, 512, 2), (200, 256, 384, 2), (900, 512, 512, 2), (1000, 384, 136, 1)])
-def test_result_in_blocks_is_the_quantized_result(rows, k, n, experts):
-    if n % 16:
-        n += 16 - n % 16
-    x, (w, ws) = normal(1, rows, k, dtype=torch.bfloat16).cuda(), (t.cuda() for t in weights(2, experts, n, k))
-    loads = loads_of(3, rows, experts).cuda()
-    out = grouped_linear_fp8(x, w, ws, loads, activation="gelu")
-    q, scales = grouped_linear_fp8(x, w, ws, loads, activation="gelu", out_blocks=True)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("activation", ["gelu", "relu", None])
+@pytest.mark.parametrize("rows,k,n,experts", [(3, 256, 512, 2), (200, 256, 384, 2), (900, 512, 512, 2), (1000, 384, 144, 1), (3000, 272, 3008, 60),
+                                              (2600, 144, 1040, 2), (3100, 128, 4112, 3), (2200, 256, 16400, 2)])
+def test_result_in_blocks_is_the_quantized_result(rows, k, n, experts, activation, dtype):
+    x, (w, ws) = normal(1, rows, k, dtype=TYPES[dtype]).cuda(), (t.cuda() for t in weights(2, experts, n, k))
+    loads, bias = loads_of(3, rows, experts).cuda(), normal(4, experts, n).cuda()
+    out = grouped_linear_fp8(x, w, ws, loads, bias=bias, activation=activation)
+    q, scales = grouped_linear_fp8(x, w, ws, loads, bias=bias, activation=activation, out_blocks=True)
     want_q, want_scales = quantize_rows(out)
-    assert torch.equal(scales, want_scales) and torch.equal(q.contiguous().view(torch.uint8), want_q.contiguous().view(torch.uint8))
+    assert q.shape == out.shape and torch.equal(scales, want_scales)
+    assert torch.equal(q.contiguous().view(torch.uint8), want_q.contiguous().view(torch.uint8))
+    # columns behind the last one are zeros: the next product reads whole blocks
+    padded = torch.as_strided(q.view(torch.uint8), (rows, q.stride(0)), (q.stride(0), 1))
+    assert not padded[:, n:].any()
 
 
 @pytest.mark.gpu
@@ -290,6 +295,8 @@ def test_refusals():
         ok(x=x.double())
     with pytest.raises(KeyError):
         ok(activation="tanh")
+    with pytest.raises(NotImplementedError, match="multiple of 16 columns"):
+        ok(w=w[:, :100].contiguous(), ws=ws, out_blocks=True)
     with pytest.raises(NotImplementedError, match="units of 16"):
         quantize_rows(torch.zeros(4, 40, device="cuda"))
     with pytest.raises(RuntimeError, match="CUDA tensor"):
@@ -307,7 +314,7 @@ def test_arguments_are_checked_before_anything_runs():
     assert lib.brt_hip_quantize_rows(None, 4, 128, 0, None, 128, None, None) == -1
     assert lib.brt_hip_quantize_rows(None, 0, 128, 0, None, 128, None, None) == 0
     call = lambda E=2, P=4, N=64, K=128, pitch=128, act=0, out=0: lib.brt_hip_grouped_gemm_fp8(  # noqa: E731
-        None, 0, pitch, None, None, None, None, None, 0, None, out, E, P, N, K, act, None)
+        None, 0, pitch, None, None, None, None, None, 0, None, out, None, E, P, N, K, act, None)
     assert call() == -1 and call(E=0) == -1 and call(pitch=64) == -1 and call(act=5) == -4 and call(out=7) == -4
     assert call(P=0) == 0 and call(N=0) == 0 and call(K=0, pitch=0) == -4
     assert lib.brt_hip_gate_topk_grad(None, None, None, None, None, 4, 4, 5, 0, 1, None) == -1
@@ -323,3 +330,32 @@ def test_arguments_are_checked_before_anything_runs():
     back = lib.brt_hip_combine_by_rows_grad
     assert back(None, None, None, None, None, None, None, None, 4, 1, 8, 4, 1, 2, None) == -4
     assert back(None, None, None, None, None, None, 16, None, 4, 1, 8, 4, 0, 0, None) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cells", [1, 17, 300, 3000])
+def test_a_served_layer_of_all_operators(cells):
+    """Gate, route, dispatch, an expert FFN of two such products and the combine, against the same steps in 64 bits with the hidden
+    rows rounded to bf16 as the layer holds them (a value near a border of e4m3 may be rounded to the other side: 1.4e-2 of the
+    norm is half of what rounding to e4m3 itself costs)."""
+    import brt._C.router as c_router
+
+    experts, d, d_ff, k = 4, 256, 400, 2
+    w1, s1 = weights(1, experts, d_ff, d)
+    w2, s2 = weights(2, experts, d, d_ff)
+    x, scores = normal(3, cells, d, dtype=torch.bfloat16), normal(4, cells, experts)
+    dev = [t.cuda() for t in (w1, s1, w2, s2)]
+    ids, weight = c_router.gate_topk(scores.cuda(), k, softmax=True)
+    loads, _, seat_rows, row_entries = c_router.route_by_path(ids, experts)
+    rows = c_router.dispatch_by_rows(x.cuda(), row_entries, k)
+    hidden, scales = grouped_linear_fp8(rows, dev[0], dev[1], loads, activation="gelu", out_blocks=True)
+    y = grouped_linear_fp8(hidden, dev[2], dev[3], loads, x_scales=scales)
+    out = c_router.combine_by_rows(y, ids, seat_rows, weight)
+
+    loads = loads.cpu()
+    xq, xs = quantized_here(rows.cpu())
+    h, _ = product_in_64(xq, xs, w1, s1, loads, activation="gelu")
+    hq, hs = quantized_here(h.to(torch.bfloat16))
+    want, _ = product_in_64(hq, hs, w2, s2, loads)
+    want = (want[seat_rows.cpu().long() - 1] * weight.cpu().double()[:, :, None]).sum(1)
+    assert float((out.cpu().double() - want).norm() / want.norm()) <= 1.4e-2

@@ -398,3 +398,57 @@ def test_a_training_step_of_all_three_on_a_stream_and_replayed():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, eager))
         check(held, *new)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("capacity", [24, 9])
+@pytest.mark.parametrize("k,weighted", [(1, False), (1, True), (2, True)])
+def test_a_layer_of_routers_that_trains(k, weighted, capacity):
+    """Scatter router, experts of plain torch modules on their rows, gather router: the gradients of cells, score and experts against
+    autograd over a loop in 64 bits; cells without a row keep the residual."""
+    from brt import Annotator, to_grid_tensor, to_torch_tensor
+    from brt.router import GatherRouter, ScatterRouter
+
+    cells, paths, d = 70, 4, 16
+    scatter = ScatterRouter(protocol_type="topk", protocol_kwargs={"top_k": k}, fabric_type="fused_dispatch",
+                            fabric_kwargs={"compact_route": True, "differentiable": True, "supported_capacities": capacity}).cuda()
+    gather = GatherRouter(fabric_type="fused_combine", fabric_kwargs={"transform": weighted}).cuda()
+    experts = [normal(10 + e, d, d).requires_grad_() for e in range(paths)]
+    x = normal(1, cells, d).requires_grad_()
+    score = torch.softmax(normal(2, cells, paths), 1).requires_grad_()
+    residual = normal(3, cells, d).requires_grad_()
+    routed = scatter(Annotator([0])(x), score)
+    rows, tags, loads, extra = to_torch_tensor(routed, retrieve_attr=True)
+    counts = loads[-1].tolist()
+    parts = torch.split(rows, counts + [rows.shape[0] - sum(counts)])
+    y = torch.cat([part @ expert for part, expert in zip(parts, experts)] + [parts[-1]])
+    out = to_torch_tensor(gather(to_grid_tensor(y, tags, loads, extra), residual, score))
+    back = normal(4, cells, d)
+    leaves = [x, residual] + experts + ([score] if weighted else [])
+    found = torch.autograd.grad(out, leaves, back)
+
+    x64, r64, s64 = (t.detach().double().requires_grad_() for t in (x, residual, score))
+    e64 = [t.detach().double().requires_grad_() for t in experts]
+    top = torch.topk(score.detach(), k, dim=1).indices
+    taken, want, seats = [0] * paths, [], top.tolist()
+    kept = [[False] * k for _ in range(cells)]
+    for t in range(cells):
+        for j, e in enumerate(seats[t]):
+            kept[t][j] = taken[e] < capacity
+            taken[e] += 1
+    for t in range(cells):
+        terms = [(x64[t] @ e64[e]) * (s64[t, e] if weighted else 1.0) for j, e in enumerate(seats[t]) if kept[t][j]]
+        want.append(sum(terms) if terms else r64[t])
+    want = torch.stack(want) + 0 * r64  # (where every cell has a row, nothing depends on the residual)
+    assert capacity == 24 or any(not any(row) for row in kept)
+    wanted = torch.autograd.grad(want, [x64, r64] + e64 + ([s64] if weighted else []), back.double())
+    torch.testing.assert_close(out.double(), want.detach(), rtol=1e-5, atol=2e-5)
+    for a, b in zip(found, wanted):
+        torch.testing.assert_close(a.double(), b, rtol=1e-4, atol=1e-4)
+
+
+def test_a_differentiable_fabric_needs_the_compact_route():
+    from brt.router import ScatterRouter
+
+    with pytest.raises(ValueError, match="compact_route"):
+        ScatterRouter(protocol_type="topk", fabric_type="fused_dispatch", fabric_kwargs={"differentiable": True})
