@@ -158,7 +158,7 @@ SIGNATURES = {
     "brt_hip_grouped_gemm_fp8": (
         _c_int,
         [_c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_int, _c_int,
-         _c_int, _c_int, _c_int, _c_ptr],
+         _c_int, _c_int, _c_int, _c_int, _c_ptr],
     ),
     "brt_hip_grouped_gemm_fp8_blocks": (_c_int, [_c_int] * 5),
     "brt_hip_gate_topk_grad": (

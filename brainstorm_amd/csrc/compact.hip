@@ -506,7 +506,7 @@ __global__ __launch_bounds__(kBlock) void combine_by_rows_kernel(RowsArgs a) {
           }
         }
       }
-      if constexpr (IN_DT != OUT_DT && LS == 6) {
+      if constexpr (IN_DT != OUT_DT && OUT_DT == BRT_F32 && LS == 6) {
         // 16-bit rows into an fp32 result, a whole wavefront per row: whole-line streaming stores
         const bool row_ok = live && (use[0] || !a.is_residual);  // the same for the whole wavefront
 #pragma unroll
@@ -676,8 +676,9 @@ int combine_rows(const void* src, void* dst, const float* weights, const void* g
                  int in_dtype, int out_dtype, void* stream) {
   if (T < 0 || k <= 0 || cell < 0 || P < 0) return fail(BRT_E_INVALID, "bad shape T=%d k=%d cell=%d P=%d", T, k, cell, P);
   if (k > kMaxK) return fail(BRT_E_UNSUPPORTED, "more than %d paths per cell", kMaxK);
+  const bool narrows = in_dtype == BRT_F32 && (out_dtype == BRT_F16 || out_dtype == BRT_BF16);
   if ((in_dtype != BRT_F32 && in_dtype != BRT_F16 && in_dtype != BRT_BF16) ||
-      (out_dtype != in_dtype && out_dtype != BRT_F32))
+      (out_dtype != in_dtype && out_dtype != BRT_F32 && !narrows))
     return fail(BRT_E_UNSUPPORTED, "dtype pair %d -> %d is not supported", in_dtype, out_dtype);
   if (static_cast<long>(T) * k >= (1l << 31)) return fail(BRT_E_UNSUPPORTED, "T*k >= 2^31");
   if (T == 0 || cell == 0) return BRT_OK;
@@ -704,7 +705,9 @@ int combine_rows(const void* src, void* dst, const float* weights, const void* g
   if (k == 1) BRT_LAUNCH_K(IN, OUT, 1)      \
   else if (k == 2) BRT_LAUNCH_K(IN, OUT, 2) \
   else BRT_LAUNCH_K(IN, OUT, kMaxK)
-  if (in_dtype == BRT_F32) BRT_LAUNCH(BRT_F32, BRT_F32)
+  if (in_dtype == BRT_F32 && out_dtype == BRT_F32) BRT_LAUNCH(BRT_F32, BRT_F32)
+  else if (in_dtype == BRT_F32 && out_dtype == BRT_F16) BRT_LAUNCH(BRT_F32, BRT_F16)
+  else if (in_dtype == BRT_F32) BRT_LAUNCH(BRT_F32, BRT_BF16)
   else if (in_dtype == BRT_F16 && out_dtype == BRT_F16) BRT_LAUNCH(BRT_F16, BRT_F16)
   else if (in_dtype == BRT_F16) BRT_LAUNCH(BRT_F16, BRT_F32)
   else if (out_dtype == BRT_BF16) BRT_LAUNCH(BRT_BF16, BRT_BF16)

@@ -755,7 +755,7 @@ Tensor cells_of_rows(const Tensor& given, const Tensor& ids_given, const Tensor&
     out = empty(rows_of(in, T), o.typed ? o.out_type : in.scalar_type(), in);
   }
   const int out_type = code_of(out.scalar_type());
-  if (out_type < 0 || (out_type != in_type && out_type != BRT_F32)) not_implemented("output data type is not supported");
+  if (out_type < 0 || (out_type != in_type && out_type != BRT_F32 && in_type != BRT_F32)) not_implemented("output data type is not supported");
   Tensor gates = o.gates;
   if (gates.defined()) {
     on_device(gates, "gates");
@@ -789,10 +789,12 @@ struct CombineByRows : Function<CombineByRows> {
     return differentiable_once(6, grads, saved, [&](variable_list& made) {
       if (!grads[0].defined()) return;
       const Tensor rows = saved[0].defined() ? dense(saved[0]) : Tensor(), weights = saved[1].defined() ? dense(saved[1]) : Tensor();
-      const Tensor ids = dense(saved[2]), seats = dense(saved[3]), entries = dense(saved[4]), grad = dense(grads[0]);
-      const c10::DeviceGuard guard(grad.device());
+      const Tensor ids = dense(saved[2]), seats = dense(saved[3]), entries = dense(saved[4]);
+      const c10::DeviceGuard guard(ids.device());
       const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
       const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
+      // (fp32 rows with a 16-bit result: the kernel takes gradients of the rows' type, or fp32)
+      const Tensor grad = dense(grads[0].scalar_type() == type ? grads[0] : grads[0].to(at::kFloat));
       const int64_t T = ids.size(0), k = ids.size(1), P = shape[0];
       int64_t cell = 1;
       for (size_t d = 1; d < shape.size(); ++d) cell *= shape[d];
@@ -998,7 +1000,7 @@ PyObject* quantize_rows(const Args& a) {  // x
   return as_rows(quantized(x, "x"), x.dim() == 2 ? x.size(1) : 0);
 }
 
-// x, weight, weight_scales, loads, bias, activation, x_scales, out, out_dtype, out_blocks
+// x, weight, weight_scales, loads, bias, activation, x_scales, out, out_dtype, out_blocks, exact (None: as fp32 results ask)
 PyObject* grouped_linear_fp8(const Args& a) {
   const Tensor x = a.tensor(0), w = a.tensor(1), w_scales = a.tensor(2), loads_given = a.tensor(3), bias_given = a.tensor_or_none(4);
   const Tensor x_scales = a.tensor_or_none(6);
@@ -1057,7 +1059,8 @@ PyObject* grouped_linear_fp8(const Args& a) {
   }
   check(brt_hip_grouped_gemm_fp8(ptr(rows), code_of(rows.scalar_type()), pitch, fptr(scales), ptr(weight), fptr(weight_scales), iptr(loads), ptr(bias),
                                  bias.defined() ? code_of(bias.scalar_type()) : BRT_F32, ptr(made.q.defined() ? made.q : out), out_type,
-                                 fptr(made.scales), E, P, N, K, a.integer(5), stream_of(x)));
+                                 fptr(made.scales), E, P, N, K, a.integer(5),
+                                 a.none(10) ? out_type == BRT_F32 : a.flag(10), stream_of(x)));
   return !out_blocks ? wrap(out) : as_rows(made.q.defined() ? made : quantized(out, "out"), N);
 }
 
@@ -1298,7 +1301,7 @@ PyMethodDef methods[] = {
     BRT_ENTRY(grouped_linear_f32, 16), BRT_ENTRY(cast_f32_to_bf16, 1), BRT_ENTRY(branch_key, 5),        BRT_ENTRY(int_list, 1),
     BRT_ENTRY(ordinary, 3),         BRT_ENTRY(plain, 1),            BRT_ENTRY(of_class, 2),            BRT_ENTRY(matrix, 4),
     BRT_ENTRY(grid, 5),                BRT_ENTRY(split_rows, 4),
-    BRT_ENTRY(quantize_rows, 1), BRT_ENTRY(grouped_linear_fp8, 10),
+    BRT_ENTRY(quantize_rows, 1), BRT_ENTRY(grouped_linear_fp8, 11),
     BRT_ENTRY(sum_rows_by_index, 3), BRT_ENTRY(combine_flows, 2), BRT_ENTRY(one_value, 2),         BRT_ENTRY(unique_tags, 1),      BRT_ENTRY(calls, 0),            {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "brt_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

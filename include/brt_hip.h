@@ -448,7 +448,7 @@ int brt_hip_combine_by_index(const void* in_data, void* out_data, const void* in
  *   in ascending path id, of weights[t,j] * src[seat_rows[t,j]-1] (weights NULL = 1), in fp32 from 0
  *   with product and sum rounded separately: the order and roundings of brt_hip_combine.  Cells
  *   without a row keep dst when is_residual != 0 and are zeroed otherwise.  k <= 8; dtypes as
- *   brt_hip_combine.
+ *   brt_hip_combine, and fp32 rows into a 16-bit result, rounded once.
  */
 int brt_hip_gate_topk(const void* scores, int T, int E, int k, int dtype, int softmax,
                       int32_t* path_ids, float* weights, int32_t* hot_mask, void* stream);
@@ -513,9 +513,9 @@ int brt_hip_combine_by_rows_grad(const void* grad, const void* rows, const float
  *     out[r,n] = act(sum_kb x_scales[kb,r] * w_scales[e,n/128,kb] * (sum over block kb of x[r,k] * w[e,n,k]) + bias[e,n]),
  *   x e4m3 rows of `pitch` >= K elements with x_scales; or, where brt_hip_grouped_gemm_fp8_quantizes(E, P, N) is 1 (few rows per
  *   expert) and x_scales is NULL, rows of x_dtype, which the kernel quantizes itself to the same bits.  w [E,N,K], w_scales [E,ceil(N/128),KB], bias [E,N] of bias_dtype or NULL, out [P,N] of
- *   out_dtype.  The blocks are added in fp32, in order; the result is rounded once.  A block's sum for an fp32 result is one of
- *   exact products; for a 16-bit result it is the 8-bit matrix instruction's, which drops the bits of a product that lie more
- *   than 13 below the largest one of 16 (1.3e-5 of the result's norm on normal data).
+ *   out_dtype.  The blocks are added in fp32, in order; the result is rounded once.  With `exact` a block's sum is one
+ *   of exact products; else it is the 8-bit matrix instruction's, which drops the bits of a product that lie more than 13 below
+ *   the largest one of 16 (1.3e-5 of the result's norm on normal data).  exact needs an fp32 result.
  *
  *   With out_scales, where brt_hip_grouped_gemm_fp8_blocks(E, P, N, K, out_dtype) is 1, the result is rounded to out_dtype and
  *   quantized as brt_hip_quantize_rows would quantize it: out is e4m3 [P,ceil(N/128)*128], out_scales [ceil(N/128),P].
@@ -525,7 +525,8 @@ int brt_hip_combine_by_rows_grad(const void* grad, const void* rows, const float
 int brt_hip_quantize_rows(const void* x, int P, int K, int dtype, void* q, int pitch, float* scales, void* stream);
 int brt_hip_grouped_gemm_fp8(const void* x, int x_dtype, int pitch, const float* x_scales, const void* w,
                              const float* w_scales, const int32_t* loads, const void* bias, int bias_dtype, void* out,
-                             int out_dtype, float* out_scales, int E, int P, int N, int K, int activation, void* stream);
+                             int out_dtype, float* out_scales, int E, int P, int N, int K, int activation, int exact,
+                             void* stream);
 int brt_hip_grouped_gemm_fp8_quantizes(int E, int P, int N);
 int brt_hip_grouped_gemm_fp8_blocks(int E, int P, int N, int K, int out_dtype);
 

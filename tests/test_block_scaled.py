@@ -76,10 +76,10 @@ def product_in_64(xq, xs, w, ws, loads, bias=None, activation=None):
     return want, size
 
 
-def assert_near(got, want, size, kb, gelu=False):
+def assert_near(got, want, size, kb, gelu=False, exact=None):
     got, kept = got.cpu(), ~want.isnan()
     info = torch.finfo(got.dtype)
-    exact = got.dtype == torch.float32
+    exact = got.dtype == torch.float32 if exact is None else exact
     off = ((128 + kb + 3) * 2.0 ** -23 + (0.0 if exact else 2.0 ** -9)) * size * (1.13 if gelu else 1.0) + (4.3e-6 if gelu else 0.0)
     bound = off + info.eps / 2 * (want.abs() + off) + info.tiny * info.eps
     far = ((got.double() - want).abs() / bound)[kept]
@@ -183,6 +183,21 @@ def test_result_in_blocks_is_the_quantized_result(rows, k, n, experts, activatio
     # columns behind the last one are zeros: the next product reads whole blocks
     padded = torch.as_strided(q.view(torch.uint8), (rows, q.stride(0)), (q.stride(0), 1))
     assert not padded[:, n:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n,experts", [(5, 1024, 520, 2), (200, 512, 256, 2), (1500, 384, 300, 3), (3000, 272, 3000, 60), (3100, 128, 4104, 3)])
+def test_fp32_results_of_the_8_bit_instruction(rows, k, n, experts):
+    x, (w, ws) = normal(1, rows, k, dtype=torch.bfloat16), weights(2, experts, n, k)
+    loads = loads_of(3, rows, experts)
+    xq, xs = quantized_here(x)
+    want, size = product_in_64(xq, xs, w, ws, loads)
+    got = grouped_linear_fp8(x.cuda(), w.cuda(), ws.cuda(), loads.cuda(), out_dtype=torch.float32, exact=False)
+    assert_near(got, want, size, -(-k // 128), exact=False)
+    # rounded to 16 bits it is the 16-bit result
+    assert torch.equal(got.bfloat16(), grouped_linear_fp8(x.cuda(), w.cuda(), ws.cuda(), loads.cuda()))
+    with pytest.raises(NotImplementedError, match="exact products"):
+        grouped_linear_fp8(x.cuda(), w.cuda(), ws.cuda(), loads.cuda(), exact=True)
 
 
 @pytest.mark.gpu
@@ -314,7 +329,7 @@ def test_arguments_are_checked_before_anything_runs():
     assert lib.brt_hip_quantize_rows(None, 4, 128, 0, None, 128, None, None) == -1
     assert lib.brt_hip_quantize_rows(None, 0, 128, 0, None, 128, None, None) == 0
     call = lambda E=2, P=4, N=64, K=128, pitch=128, act=0, out=0: lib.brt_hip_grouped_gemm_fp8(  # noqa: E731
-        None, 0, pitch, None, None, None, None, None, 0, None, out, None, E, P, N, K, act, None)
+        None, 0, pitch, None, None, None, None, None, 0, None, out, None, E, P, N, K, act, 0, None)
     assert call() == -1 and call(E=0) == -1 and call(pitch=64) == -1 and call(act=5) == -4 and call(out=7) == -4
     assert call(P=0) == 0 and call(N=0) == 0 and call(K=0, pitch=0) == -4
     assert lib.brt_hip_gate_topk_grad(None, None, None, None, None, 4, 4, 5, 0, 1, None) == -1

@@ -96,6 +96,29 @@ def test_combine_gradients(cells, paths, k, capacity, d, weighted, dtype, out):
         near(found[1], products.sum(2), products.abs().sum(2), d)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", ["f16", "bf16"])
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("cells,paths,k,capacity,d", SHAPES)
+def test_fp32_rows_combined_into_16_bits(cells, paths, k, capacity, d, weighted, out):
+    """The fp32 sum of the rows, rounded once; and its gradients."""
+    out = TYPES[out]
+    ids, seat_rows, row_entries = make_route(cells, paths, k, capacity, cells + 2, keep=0.8)
+    y, w = normal(1, row_entries.numel(), d).requires_grad_(), normal(2, cells, k) if weighted else None
+    got = c_router.combine_by_rows(y, ids, seat_rows, w, out_dtype=out, row_entries=row_entries)
+    wide = c_router.combine_by_rows(y.detach(), ids, seat_rows, w)
+    assert got.dtype == out and torch.equal(got, wide.to(out))
+    kept = torch.full((cells, d), 3.0, dtype=out, device="cuda")
+    c_router.combine_by_rows(y.detach(), ids, seat_rows, w, kept)
+    has = (seat_rows > 0).any(1)
+    assert torch.equal(kept[has], got[has]) and bool((kept[~has] == 3.0).all())
+    grad = normal(3, cells, d, dtype=out)
+    (dy,) = torch.autograd.grad(got, y, grad)
+    entry = (row_entries.long() - 1).clamp(min=0)
+    want = grad.double()[entry // k] * (1.0 if w is None else w.double().reshape(-1)[entry][:, None])
+    near(dy, torch.where((row_entries > 0)[:, None], want, 0.0), want.abs(), 1)
+
+
 GATES = [(1, 1, 1), (1, 4, 4), (5, 3, 2), (63, 8, 2), (130, 60, 3), (257, 64, 1), (33, 100, 4), (70, 128, 2), (9, 1000, 8), (17, 1024, 2), (12, 513, 13)]
 
 
