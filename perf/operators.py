@@ -327,8 +327,9 @@ def _own_serve(state):
     loads, _, seat_rows, row_entries = c_router.route_by_path(ids, case["experts"], state["capacities"], rows=_row_count(case))
     rows = c_router.dispatch_by_rows(x, row_entries, case["top_k"])
     hidden, scales = grouped_linear_fp8(rows, state["w1"], state["ws1"], loads, activation="gelu", out_blocks=True)
-    y = grouped_linear_fp8(hidden, state["w2"], state["ws2"], loads, x_scales=scales, out_dtype=x.dtype)
-    return {"out": c_router.combine_by_rows(y, ids, seat_rows, weights), "loads": loads}
+    # (the experts' rows stay in 32 bits until they are added up)
+    y = grouped_linear_fp8(hidden, state["w2"], state["ws2"], loads, x_scales=scales, out_dtype=torch.float32, exact=False)
+    return {"out": c_router.combine_by_rows(y, ids, seat_rows, weights, out_dtype=x.dtype), "loads": loads}
 
 
 def _own(state):
