@@ -511,12 +511,19 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
 
   long done = t;  // (the same walk, for the tile that is multiplied)
   bool more = true;  // there is a K-step that has not been requested
-#pragma unroll
-  for (int q = 0; q < STAGES - 1; ++q)
+  auto request_ahead = [&] {
     if (more) {
       request();
       more = step_ahead();
     }
+  };
+  // A K-step begins with its requests, but with 256 rows with the fragments' reads, which the requests' arrivals would hold up
+  // (16384 rows of 8 experts 4096 -> 4096 385 us the other way round, 327 so; 64 x 64 tiles 15 % the other way).  A wavefront without
+  // rows only fetches (8192 rows of 64 experts 1024 -> 4096 86.6 -> 84.6 us, 400 of 8 15.5 -> 14.8, in 256-row tiles 20.2 -> 16.8).
+  constexpr bool kRequestsFirst = BM <= 128;
+#pragma unroll
+  for (int q = 0; q < STAGES - 1; ++q)
+    request_ahead();
   using Operand = decltype(operand<EXACT>(i32x8{}));
   uint32_t stage_at = 0;
   f32x4 acc[MT][NT];
@@ -529,6 +536,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    const bool live = at.rows > wm * (BM / WM);
 #pragma unroll 1
     for (int kt = 0; kt < a.KB; ++kt) {
       // (of the loads behind this K-step's all but STAGES - 2 steps' have been requested; behind the last request the count is less)
@@ -541,6 +549,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
         const i32x4 lo = *reinterpret_cast<const i32x4*>(stage + lo_at), hi = *reinterpret_cast<const i32x4*>(stage + hi_at);
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
       };
+      if (kRequestsFirst || !live) request_ahead();
+      if (!live) continue;
       i32x8 w = fragment(wlo, whi), x_read[MT];
       float s_read[MT];
 #pragma unroll
@@ -549,10 +559,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
         s_read[i] = *reinterpret_cast<const float*>(stage + kRowScales + (xr + i * 16) * 4);
       }
       const float scale = *reinterpret_cast<const float*>(stage + kColumnScales + wn * 256);
-      if (more) {
-        request();
-        more = step_ahead();
-      }
+      if constexpr (!kRequestsFirst) request_ahead();
       __builtin_amdgcn_sched_barrier(0);
       pipe.drain(acc, s);
       Operand x[MT];
