@@ -28,6 +28,7 @@ constexpr float kMax = 448.0f;     // the largest e4m3 value
 constexpr float kLeast = 0x1p-100f;  // blocks whose largest value is below this are scaled as if it were this
 constexpr int kXcds = 8, kCusPerXcd = 32;
 constexpr int kPatchRows = 4;
+constexpr int kMostRows = 1 << 25;   // 64 times as many are added up in 32 bits
 constexpr int kMostExperts = 512;  // whose row blocks a workgroup keeps in LDS
 constexpr uint32_t kNowhere = 0x7ffffff0u;  // an offset past every extent: reads as zero, costs no request
 
@@ -161,22 +162,22 @@ __device__ __forceinline__ auto operand(const i32x8& v) {
 struct Block {
   int e, row0, rows;
 };
-// The expert and the rows of row block `block` of the list (blocks of `1 << bits` rows); rows 0: there is no such block.
+// The expert and the rows of row block `block` of the list (blocks of `1 << bits` rows); rows 0: there is no such block.  Loads are
+// taken as what they can be: none below zero, no rows behind the P that there are (which are few enough for 32-bit sums).
 __device__ __forceinline__ Block find_block(const Fp8Args& a, int block, int bits) {
   const int lane = lane_id();
   int carry_b = 0, carry_m = 0;
   for (int base = 0; base < a.E; base += kWave) {
     const int given = a.loads[min(base + lane, a.E - 1)];
-    const int m = base + lane < a.E ? max(given, 0) : 0;
+    const int m = base + lane < a.E ? min(max(given, 0), a.P) : 0;
     const int b = (m + (1 << bits) - 1) >> bits;
-    const int incl_b = carry_b + wave_inclusive_scan(b), incl_m = carry_m + wave_inclusive_scan(m);
+    const int incl_b = carry_b + wave_inclusive_scan(b), incl_m = min(carry_m + wave_inclusive_scan(m), a.P);
     const unsigned long long hit = __ballot(block < incl_b);
     if (hit != 0) {
       const int src = __builtin_ctzll(hit);
       const int seat0 = (block - (read_lane(incl_b, src) - read_lane(b, src))) << bits;
-      const int load = read_lane(m, src);
-      const int row0 = read_lane(incl_m, src) - load + seat0;
-      return {base + src, row0, max(0, min(min(1 << bits, load - seat0), a.P - row0))};
+      const int before = src > 0 ? read_lane(incl_m, src - 1) : carry_m, row0 = before + seat0;
+      return {base + src, row0, max(0, min(1 << bits, read_lane(incl_m, src) - row0))};
     }
     carry_b = read_lane(incl_b, kWave - 1);
     carry_m = read_lane(incl_m, kWave - 1);
@@ -383,15 +384,15 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
     int carry_b = 0, carry_m = 0;
     for (int base = 0; base < a.E; base += kWave) {
       const int given = a.loads[min(base + lane, a.E - 1)];
-      const int m = base + lane < a.E ? max(given, 0) : 0;
-      const int incl_b = carry_b + wave_inclusive_scan((m + BM - 1) >> BM_BITS), incl_m = carry_m + wave_inclusive_scan(m);
+      const int m = base + lane < a.E ? min(max(given, 0), a.P) : 0;  // (loads as in find_block)
+      const int incl_b = carry_b + wave_inclusive_scan((m + BM - 1) >> BM_BITS), incl_m = min(carry_m + wave_inclusive_scan(m), a.P);
       if (base + lane < a.E) s_blocks[base + lane] = incl_b, s_rows[base + lane] = incl_m;
       carry_b = read_lane(incl_b, kWave - 1);
       carry_m = read_lane(incl_m, kWave - 1);
     }
   }
   __syncthreads();
-  const int blocks = __builtin_amdgcn_readfirstlane(s_blocks[a.E - 1]);
+  const int blocks = min(__builtin_amdgcn_readfirstlane(s_blocks[a.E - 1]), (a.P >> BM_BITS) + min(a.E, a.P));
   // Tiles are dealt out in runs, one per XCD and round; four row blocks wide, so that a run shares both operands in its L2.
   const int run = gridDim.x / kXcds, per = kPatchRows * a.tiles_n;
   const long tiles = static_cast<long>(blocks) * a.tiles_n;
@@ -415,7 +416,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
     Tile at;
     at.e = __builtin_amdgcn_readfirstlane(e);
     at.row0 = __builtin_amdgcn_readfirstlane(row0);
-    at.rows = __builtin_amdgcn_readfirstlane(max(0, min(min(BM, s_rows[e] - row0), a.P - row0)));
+    at.rows = __builtin_amdgcn_readfirstlane(max(0, min(BM, s_rows[e] - row0)));
     at.n0 = __builtin_amdgcn_readfirstlane(in / wide * BN);
     return at;
   };
@@ -522,8 +523,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
   // rows only fetches (8192 rows of 64 experts 1024 -> 4096 86.6 -> 84.6 us, 400 of 8 15.5 -> 14.8, in 256-row tiles 20.2 -> 16.8).
   constexpr bool kRequestsFirst = BM <= 128;
 #pragma unroll
-  for (int q = 0; q < STAGES - 1; ++q)
-    request_ahead();
+  for (int q = 0; q < STAGES - 1; ++q) request_ahead();
   using Operand = decltype(operand<EXACT>(i32x8{}));
   uint32_t stage_at = 0;
   f32x4 acc[MT][NT];
@@ -822,7 +822,7 @@ bool quantizes_result(int E, int P, int N, int K, int out_dtype) {
 }
 int launch_any_tiles(Fp8Args& a, hipStream_t st) {
   TileKind kind = tile_kind(a.E, a.P, a.N, a.K, a.exact != 0);
-  // (quantizing 256 x 256 results needs more registers than there are: 8192 rows of 32 experts 1024 -> 4096 + GELU 101 us, 128 x 256 BLK)
+  // (quantizing 256 x 256 results needs more registers than there are: 8192 rows of 32 experts 1024 -> 4096 + GELU 101 us, 128 x 256 88)
   if (kind == k256x256 && a.out_scales != nullptr) kind = k128x256;
   switch (kind) {
     case k64x64: return a.exact ? launch_tiles<6, 64, 2, 1, 4, false, true, false>(a, st) : launch_tiles<6, 64, 2, 1, 4, false, false, false>(a, st);
@@ -882,6 +882,7 @@ extern "C" int brt_hip_grouped_gemm_fp8(const void* x, int x_dtype, int pitch, c
   if (!x || !w || !w_scales || !loads || !out) return fail(BRT_E_INVALID, "null argument");
   if (K % 16 != 0 || pitch % 16 != 0 || !aligned(x, 16) || !aligned(w, 16))
     return fail(BRT_E_UNSUPPORTED, "rows must be whole, aligned units of 16 elements (K=%d)", K);
+  if (P >= kMostRows) return fail(BRT_E_UNSUPPORTED, "more than %d rows", kMostRows - 1);
   if (pitch > (1 << 20)) return fail(BRT_E_UNSUPPORTED, "rows of more than 1 Mi elements");  // (256 of them are addressed by 31 bits)
   if (out_scales && (!quantizes_result(E, P, N, K, out_dtype) || !aligned(out, 16)))
     return fail(BRT_E_UNSUPPORTED, "results of this shape are not quantized by the product's kernel");

@@ -985,6 +985,7 @@ Blocks quantized(const Tensor& given, const char* name) {
   Tensor in = dense(given);
   if (!aligned16(in)) in = in.clone();
   const int64_t P = in.size(0), K = in.size(1), KB = blocks_of(K);
+  if (P >= int64_t{1} << 31 || K >= int64_t{1} << 31) not_implemented("a dimension of 2^31 and more");
   Blocks b{empty({P, KB * kScaleBlock}, at::kByte, in), empty({KB, P}, at::kFloat, in)};
   check(brt_hip_quantize_rows(ptr(in), P, K, type, ptr(b.q), KB * kScaleBlock, fptr(b.scales), stream_of(in)));
   return b;
@@ -1011,6 +1012,8 @@ PyObject* grouped_linear_fp8(const Args& a) {
   if (x.dim() != 2 || w.dim() != 3 || w.size(2) != x.size(1)) runtime_error("x must be [rows, in_features], weight [experts, out_features, in_features]");
   if (w.scalar_type() != at::kFloat8_e4m3fn) not_implemented("weight must be float8_e4m3fn");
   const int64_t P = x.size(0), K = x.size(1), E = w.size(0), N = w.size(1), KB = blocks_of(K);
+  for (const int64_t n : {P, K, E, N})
+    if (n >= int64_t{1} << 31) not_implemented("a dimension of 2^31 and more");
   if (w_scales.scalar_type() != at::kFloat || w_scales.sizes() != at::IntArrayRef({E, blocks_of(N), KB}))
     runtime_error("weight_scales must be fp32 [experts, blocks of out_features, blocks of in_features]");
   if (loads_given.numel() != E) runtime_error("one load per expert is needed");
@@ -1044,7 +1047,7 @@ PyObject* grouped_linear_fp8(const Args& a) {
   int64_t pitch;
   if (in_blocks) {
     if (x_scales.scalar_type() != at::kFloat || x_scales.sizes() != at::IntArrayRef({P, KB})) runtime_error("x_scales must be fp32 [rows, blocks]");
-    const bool in_place = P > 0 && (x.stride(1) == 1 || K == 1) && x.stride(0) >= K && x.stride(0) % 16 == 0 && aligned16(x);
+    const bool in_place = P > 0 && (x.stride(1) == 1 || K == 1) && x.stride(0) >= K && x.stride(0) % 16 == 0 && x.stride(0) <= 1 << 20 && aligned16(x);
     rows = in_place ? x : x.contiguous();
     if (!aligned16(rows)) rows = rows.clone();
     pitch = in_place ? x.stride(0) : K;

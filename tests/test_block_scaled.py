@@ -239,6 +239,55 @@ def test_strides_types_and_loads_that_do_not_fit():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [7, 300, 3000])
+def test_loads_that_name_more_rows_than_there_are(rows):
+    """Rows behind the last one do not exist, whatever the loads say: results of the first rows are those of loads that fit."""
+    k, n, experts = 128, 1040, 5
+    w, ws = (t.cuda() for t in weights(1, experts, n, k))
+    x = normal(2, rows, k, dtype=torch.bfloat16).cuda()
+    first = rows // 3
+    fits = torch.tensor([first, 0, rows - first, 0, 0], dtype=torch.int32, device="cuda")
+    want = grouped_linear_fp8(x, w, ws, fits)
+    most = 2 ** 31 - 1
+    for odd in ([first, -5, most, most, most], [first, 0, rows, rows, 1], [first, -most - 1, rows - first, 7, -1]):
+        got = grouped_linear_fp8(x, w, ws, torch.tensor(odd, dtype=torch.int32, device="cuda"))
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_many_experts():
+    """More than the list in LDS holds: the kernel for few rows takes them, with any number of rows."""
+    k, n, experts = 144, 72, 600
+    w, ws = weights(1, experts, n, k)
+    for rows in (5, 40000):
+        x, loads = normal(2, rows, k, dtype=torch.bfloat16), loads_of(3, rows, experts)
+        xq, xs = quantized_here(x)
+        want, size = product_in_64(xq, xs, w, ws, loads)
+        assert_near(grouped_linear_fp8(x.cuda(), w.cuda(), ws.cuda(), loads.cuda()), want, size, 2)
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once_and_scales_beyond_the_ordinary():
+    """Two streams at the same time; scales of e4m3 weights up to the largest fp32 can be multiplied with, and zero."""
+    k, n = 512, 512
+    w, ws = (t.cuda() for t in weights(1, 2, n, k))
+    ws[0, 1], ws[1, 0] = 0.0, 3e30
+    xs = [normal(s, 900, k, dtype=torch.bfloat16).cuda() for s in (2, 3)]
+    loads = torch.tensor([400, 500], dtype=torch.int32, device="cuda")
+    want = [grouped_linear_fp8(x, w, ws, loads) for x in xs]
+    assert not want[0][:400, 128:256].any() and torch.isfinite(want[0].float()).all()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for _ in range(5):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(grouped_linear_fp8(xs[i], w, ws, loads))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+
+
+@pytest.mark.gpu
 def test_no_rows():
     w, ws = (t.cuda() for t in weights(1, 2, 64, 128))
     none = torch.zeros(2, dtype=torch.int32, device="cuda")
@@ -331,6 +380,12 @@ def test_arguments_are_checked_before_anything_runs():
     call = lambda E=2, P=4, N=64, K=128, pitch=128, act=0, out=0: lib.brt_hip_grouped_gemm_fp8(  # noqa: E731
         None, 0, pitch, None, None, None, None, None, 0, None, out, None, E, P, N, K, act, 0, None)
     assert call() == -1 and call(E=0) == -1 and call(pitch=64) == -1 and call(act=5) == -4 and call(out=7) == -4
+    assert lib.brt_hip_grouped_gemm_fp8(16, 0, 1 << 21, 16, 16, 16, 16, None, 0, 16, 0, None, 2, 4, 64, 1 << 21, 0, 0, None) == -4
+    assert lib.brt_hip_grouped_gemm_fp8(16, 0, 128, 16, 16, 16, 16, None, 0, 16, 0, None, 2, 1 << 25, 64, 128, 0, 0, None) == -4
+    assert lib.brt_hip_grouped_gemm_fp8(16, 0, 128, 16, 16, 16, 16, None, 0, 16, 0, 16, 2, 4, 64, 128, 0, 0, None) == -4
+    assert lib.brt_hip_grouped_gemm_fp8(16, 0, 128, 16, 16, 16, 16, None, 0, 16, 2, None, 2, 4, 64, 128, 0, 1, None) == -4
+    assert lib.brt_hip_grouped_gemm_fp8(16, 2, 128, None, 16, 16, 16, None, 0, 16, 2, None, 2, 4000, 640, 128, 0, 0, None) == -4
+    assert lib.brt_hip_grouped_gemm_fp8(8, 0, 128, 16, 16, 16, 16, None, 0, 16, 0, None, 2, 4, 64, 128, 0, 0, None) == -4
     assert call(P=0) == 0 and call(N=0) == 0 and call(K=0, pitch=0) == -4
     assert lib.brt_hip_gate_topk_grad(None, None, None, None, None, 4, 4, 5, 0, 1, None) == -1
     assert lib.brt_hip_gate_topk_grad(None, None, None, None, None, 4, 2000, 1, 0, 1, None) == -4
