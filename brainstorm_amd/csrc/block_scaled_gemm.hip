@@ -28,7 +28,7 @@ constexpr float kMax = 448.0f;     // the largest e4m3 value
 constexpr float kLeast = 0x1p-100f;  // blocks whose largest value is below this are scaled as if it were this
 constexpr int kXcds = 8, kCusPerXcd = 32;
 constexpr int kPatchRows = 4;
-constexpr int kMostRows = 1 << 25;   // 64 times as many are added up in 32 bits
+constexpr int kMostRows = 1 << 24;   // 65 times as many are added up in 32 bits
 constexpr int kMostExperts = 512;  // whose row blocks a workgroup keeps in LDS
 constexpr uint32_t kNowhere = 0x7ffffff0u;  // an offset past every extent: reads as zero, costs no request
 
@@ -384,15 +384,16 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
     int carry_b = 0, carry_m = 0;
     for (int base = 0; base < a.E; base += kWave) {
       const int given = a.loads[min(base + lane, a.E - 1)];
-      const int m = base + lane < a.E ? min(max(given, 0), a.P) : 0;  // (loads as in find_block)
-      const int incl_b = carry_b + wave_inclusive_scan((m + BM - 1) >> BM_BITS), incl_m = min(carry_m + wave_inclusive_scan(m), a.P);
+      const int m = base + lane < a.E ? min(max(given, 0), a.P) : 0;  // (loads as in find_block; here no block is without rows)
+      const int sum_m = carry_m + wave_inclusive_scan(m), incl_m = min(sum_m, a.P);
+      const int incl_b = carry_b + wave_inclusive_scan((incl_m - min(sum_m - m, a.P) + BM - 1) >> BM_BITS);
       if (base + lane < a.E) s_blocks[base + lane] = incl_b, s_rows[base + lane] = incl_m;
       carry_b = read_lane(incl_b, kWave - 1);
       carry_m = read_lane(incl_m, kWave - 1);
     }
   }
   __syncthreads();
-  const int blocks = min(__builtin_amdgcn_readfirstlane(s_blocks[a.E - 1]), (a.P >> BM_BITS) + min(a.E, a.P));
+  const int blocks = __builtin_amdgcn_readfirstlane(s_blocks[a.E - 1]);
   // Tiles are dealt out in runs, one per XCD and round; four row blocks wide, so that a run shares both operands in its L2.
   const int run = gridDim.x / kXcds, per = kPatchRows * a.tiles_n;
   const long tiles = static_cast<long>(blocks) * a.tiles_n;
@@ -416,7 +417,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
     Tile at;
     at.e = __builtin_amdgcn_readfirstlane(e);
     at.row0 = __builtin_amdgcn_readfirstlane(row0);
-    at.rows = __builtin_amdgcn_readfirstlane(max(0, min(BM, s_rows[e] - row0)));
+    at.rows = __builtin_amdgcn_readfirstlane(min(BM, s_rows[e] - row0));
     at.n0 = __builtin_amdgcn_readfirstlane(in / wide * BN);
     return at;
   };

@@ -976,6 +976,18 @@ constexpr int64_t kScaleBlock = 128;
 int64_t blocks_of(int64_t n) { return (n + kScaleBlock - 1) / kScaleBlock; }
 bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
+// Whether the elements of two tensors span addresses in common.
+bool shares_memory(const Tensor& a, const Tensor& b) {
+  auto span = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    const auto first = reinterpret_cast<uintptr_t>(t.data_ptr());
+    return std::pair<uintptr_t, uintptr_t>(first, t.numel() == 0 ? first : first + (last + 1) * t.element_size());
+  };
+  const auto s = span(a), t = span(b);
+  return s.first < t.second && t.first < s.second;
+}
+
 struct Blocks {
   Tensor q, scales;  // [rows, pitch] bytes, [blocks, rows]
 };
@@ -1033,6 +1045,8 @@ PyObject* grouped_linear_fp8(const Args& a) {
     if (out_blocks || (typed && type != out.scalar_type())) runtime_error("out is given: it says its type, and holds no blocks");
     if (data_type(out, "output data type") < 0 || out.sizes() != at::IntArrayRef({P, N}) || !out.is_contiguous())
       runtime_error("out must be a contiguous [rows, out_features] tensor");
+    for (const Tensor* t : std::initializer_list<const Tensor*>{&x, &w, &w_scales, &loads_given, &bias_given, &x_scales})
+      if (t->defined() && shares_memory(out, *t)) runtime_error("out shares memory with an operand");
   }
   if (out_blocks && N % 16 != 0) not_implemented("a result in blocks has a multiple of 16 columns");
   const int out_type = out.defined() ? code_of(out.scalar_type()) : code_of(type);

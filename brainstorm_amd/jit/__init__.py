@@ -84,9 +84,10 @@ def grouped_linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scales: tor
     ``W_e[n, k] = weight[e, n, k] * weight_scales[e, n // 128, k // 128]``, ``weight`` float8_e4m3fn ``[experts, out_features,
     in_features]`` (in_features a multiple of 16) and fp32 scales.  ``x`` is quantized as :func:`quantize_rows` does it, or comes
     that way (float8_e4m3fn with ``x_scales``).  The products of a block are summed by the matrix units, scaled by ``x_scale *
-    weight_scale`` in fp32 and summed in order of the blocks; bias, activation and one rounding follow.
+    weight_scale`` in fp32 and summed in an order that the shape fixes; bias, activation and one rounding follow.
 
-    The result has ``x``'s type (``out_dtype``, or bf16 for 8-bit rows); a given ``out`` is filled in place.  Rows behind the
+    The result has ``x``'s type (``out_dtype``, or bf16 for 8-bit rows); a given ``out`` is filled in place
+    (memory of its own: it is written while the operands are read).  Rows behind the
     last expert's are not written.  ``out_blocks=True`` gives ``(q, scales)``, the quantized result, rounded to that type
     first (out_features a multiple of 16): the rows of the next such product.  Results are cut off from autograd, as those of
     :func:`grouped_linear`.

@@ -252,6 +252,11 @@ def test_loads_that_name_more_rows_than_there_are(rows):
     for odd in ([first, -5, most, most, most], [first, 0, rows, rows, 1], [first, -most - 1, rows - first, 7, -1]):
         got = grouped_linear_fp8(x, w, ws, torch.tensor(odd, dtype=torch.int32, device="cuda"))
         assert torch.equal(got, want)
+    # ... and where the loads are added up in several passes
+    w, ws = w[:1].expand(130, -1, -1).contiguous(), ws[:1].expand(130, -1, -1).contiguous()
+    want = grouped_linear_fp8(x, w[:1], ws[:1], torch.tensor([rows], dtype=torch.int32, device="cuda"))
+    for load in (rows, most):
+        assert torch.equal(grouped_linear_fp8(x, w, ws, torch.full((130,), load, dtype=torch.int32, device="cuda")), want)
 
 
 @pytest.mark.gpu
@@ -353,6 +358,13 @@ def test_refusals():
         ok(out=torch.zeros(n, 8, device="cuda").t())
     with pytest.raises(RuntimeError, match="out is given"):
         ok(out=torch.zeros(8, n, device="cuda"), out_blocks=True)
+    both = torch.zeros(16, n, device="cuda")
+    with pytest.raises(RuntimeError, match="shares memory"):
+        ok(w=w[:, :, :n].contiguous(), ws=ws[:, :, :1], x=both[4:12], out=both[:8])
+    assert torch.equal(ok(w=w[:, :, :n].contiguous(), ws=ws[:, :, :1], x=both[8:], out=both[:8]), torch.zeros(8, n, device="cuda"))
+    with pytest.raises(RuntimeError, match="shares memory"):
+        table = torch.zeros(2, n, device="cuda")
+        ok(x=x[:2], bias=table, out=table)
     with pytest.raises(NotImplementedError):
         ok(out_dtype=torch.float64)
     with pytest.raises(NotImplementedError):
@@ -381,7 +393,7 @@ def test_arguments_are_checked_before_anything_runs():
         None, 0, pitch, None, None, None, None, None, 0, None, out, None, E, P, N, K, act, 0, None)
     assert call() == -1 and call(E=0) == -1 and call(pitch=64) == -1 and call(act=5) == -4 and call(out=7) == -4
     assert lib.brt_hip_grouped_gemm_fp8(16, 0, 1 << 21, 16, 16, 16, 16, None, 0, 16, 0, None, 2, 4, 64, 1 << 21, 0, 0, None) == -4
-    assert lib.brt_hip_grouped_gemm_fp8(16, 0, 128, 16, 16, 16, 16, None, 0, 16, 0, None, 2, 1 << 25, 64, 128, 0, 0, None) == -4
+    assert lib.brt_hip_grouped_gemm_fp8(16, 0, 128, 16, 16, 16, 16, None, 0, 16, 0, None, 2, 1 << 24, 64, 128, 0, 0, None) == -4
     assert lib.brt_hip_grouped_gemm_fp8(16, 0, 128, 16, 16, 16, 16, None, 0, 16, 0, 16, 2, 4, 64, 128, 0, 0, None) == -4
     assert lib.brt_hip_grouped_gemm_fp8(16, 0, 128, 16, 16, 16, 16, None, 0, 16, 2, None, 2, 4, 64, 128, 0, 1, None) == -4
     assert lib.brt_hip_grouped_gemm_fp8(16, 2, 128, None, 16, 16, 16, None, 0, 16, 2, None, 2, 4000, 640, 128, 0, 0, None) == -4
