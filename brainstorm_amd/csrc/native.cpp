@@ -229,19 +229,23 @@ struct GateTopk : Function<GateTopk> {
     ctx->set_materialize_grads(false);  // (the ids' would be a fill of zeros in every pass)
     variable_list made = gate(given, k, softmax, hot_mask);
     ctx->mark_non_differentiable(hot_mask ? variable_list{made[0], made[2]} : variable_list{made[0]});
-    ctx->save_for_backward({given, made[0], made[1]});
-    ctx->saved_data["softmax"] = softmax;
+    // scores and weights are read for the softmax only: without it they may be written to before the backward pass
+    ctx->save_for_backward({softmax ? given : Tensor(), made[0], softmax ? made[1] : Tensor()});
+    ctx->saved_data["shape"] = given.sizes().vec();
+    ctx->saved_data["type"] = static_cast<int64_t>(given.scalar_type());
     return made;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
     return differentiable_once(4, grads, saved, [&](variable_list& made) {
       if (!grads[1].defined()) return;
-      const Tensor score = dense(saved[0]), ids = saved[1], weights = saved[2], grad = dense(grads[1]);
-      const c10::DeviceGuard guard(score.device());
-      made[0] = empty(score.sizes(), score.scalar_type(), score);
-      check(brt_hip_gate_topk_grad(ptr(score), iptr(ids), fptr(weights), fptr(grad), ptr(made[0]), score.size(0), score.size(1),
-                                   ids.size(1), code_of(score.scalar_type()), ctx->saved_data["softmax"].toBool(), stream_of(score)));
+      const Tensor score = saved[0].defined() ? dense(saved[0]) : Tensor(), ids = saved[1], weights = saved[2], grad = dense(grads[1]);
+      const c10::DeviceGuard guard(ids.device());
+      const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+      const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
+      made[0] = empty(shape, type, ids);
+      check(brt_hip_gate_topk_grad(ptr(score), iptr(ids), fptr(weights), fptr(grad), ptr(made[0]), shape[0], shape[1], ids.size(1),
+                                   code_of(type), score.defined(), stream_of(ids)));
     });
   }
 };

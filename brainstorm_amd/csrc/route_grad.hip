@@ -52,7 +52,7 @@ __global__ __launch_bounds__(kBlock) void gate_grad_kernel(GateGradArgs a) {
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
     const int u = s * lpr + glane;
-    unpack<DT, kBytes>(from[min(u, units - 1)], p[s]);
+    if (a.softmax) unpack<DT, kBytes>(from[min(u, units - 1)], p[s]);
 #pragma unroll
     for (int v = 0; v < V; ++v) g[s][v] = 0.0f;
   }
@@ -347,7 +347,7 @@ extern "C" int brt_hip_gate_topk_grad(const void* scores, const int32_t* path_id
   if (E > 1024) return fail(BRT_E_UNSUPPORTED, "more than 1024 paths");
   if (static_cast<long>(T) * E >= (1l << 31)) return fail(BRT_E_UNSUPPORTED, "T*E >= 2^31");
   if (T == 0) return BRT_OK;
-  if (!scores || !grad_scores || (k > 0 && (!path_ids || !grad || (softmax && !weights)))) return fail(BRT_E_INVALID, "null argument");
+  if ((softmax && !scores) || !grad_scores || (k > 0 && (!path_ids || !grad || (softmax && !weights)))) return fail(BRT_E_INVALID, "null argument");
   GateGradArgs a{scores, path_ids, weights, grad, grad_scores, T, E, k, softmax, 0};
   const int per = 16 / elem_bytes(dtype);
   const bool units = E % per == 0 && aligned(scores, 16) && aligned(grad_scores, 16);

@@ -477,7 +477,7 @@ int brt_hip_combine_by_rows_gated(const void* src, void* dst, const void* gates,
  *
  * brt_hip_gate_topk_grad: grad_scores [T,E] (of dtype) from grad [T,k], the gradient of the weights that
  *   brt_hip_gate_topk gave for path_ids: with softmax p * (grad at the chosen columns - sum_j grad[t,j] weights[t,j]),
- *   p the softmax of the row; else grad at the chosen columns, zero elsewhere (weights may be NULL).  E <= 1024.
+ *   p the softmax of the row; else grad at the chosen columns, zero elsewhere (scores and weights may be NULL).  E <= 1024.
  *
  * brt_hip_dispatch_by_rows_grad: of grad_rows [P,cell], the gradient of dispatch_by_rows' result,
  *   grad_cells[t] = sum_j weights[t,j] * grad_rows[seat_rows[t,j]-1] over the entries with a row, j ascending (weights

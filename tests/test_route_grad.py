@@ -240,6 +240,24 @@ def test_gate_gradient_of_masked_scores():
 
 
 @pytest.mark.gpu
+def test_what_a_gate_without_softmax_keeps():
+    """Its gradient reads neither scores nor weights: both may be written to before the backward pass; with softmax that is an error."""
+    given = normal(1, 20, 8).requires_grad_()
+    for softmax in (False, True):
+        scores = given * 1.0
+        ids, weights = c_router.gate_topk(scores, 2, softmax, differentiable=True)
+        weights /= 2.0
+        with torch.no_grad():
+            scores.zero_()
+        if softmax:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(weights.sum(), given)
+        else:
+            (got,) = torch.autograd.grad(weights.sum(), given)
+            assert torch.equal(got, torch.zeros_like(given).scatter_(1, ids.long(), 0.5))
+
+
+@pytest.mark.gpu
 def test_only_what_is_asked_for():
     cells, k, d = 50, 2, 64
     ids, seat_rows, row_entries = make_route(cells, 4, k, 20, 1)
