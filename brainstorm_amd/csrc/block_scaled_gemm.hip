@@ -396,12 +396,18 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
   const int blocks = __builtin_amdgcn_readfirstlane(s_blocks[a.E - 1]);
   // Tiles are dealt out in runs, one per XCD and round; four row blocks wide, so that a run shares both operands in its L2.
   const int run = gridDim.x / kXcds, per = kPatchRows * a.tiles_n;
-  const long tiles = static_cast<long>(blocks) * a.tiles_n;
+  // Where a last round has work for half of the workgroups at most, its tiles are dealt out by the halves of their rows: those have
+  // one wavefront of each SIMD at work (the second halves of tiles that have none are left out; nothing follows them).
+  constexpr bool kHalves = WAVES == 8 && WM * WN / 2 == 4;
+  const long real = static_cast<long>(blocks) * a.tiles_n, whole = kHalves && real % gridDim.x * 2 <= gridDim.x ? real / gridDim.x * gridDim.x : real;
+  const long tiles = whole + 2 * (real - whole);
   long t = static_cast<long>(blockIdx.x % kXcds) * run + blockIdx.x / kXcds;
   struct Tile {
     int e, row0, rows, n0;
   };
-  auto tile_at = [&](int t) {
+  auto tile_at = [&](long at_walk) {
+    const int over = static_cast<int>(at_walk - whole);
+    const int t = static_cast<int>(over < 0 ? at_walk : whole + (over >> 1)), half = over < 0 ? 0 : BM / 2;
     const int group = t / per, in = t - group * per, wide = min(kPatchRows, blocks - group * kPatchRows);
     const int block = __builtin_amdgcn_readfirstlane(group * kPatchRows + in % wide);
     int e = 0;
@@ -413,11 +419,11 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
       }
     }
     const int before = e > 0 ? s_blocks[e - 1] : 0, first = e > 0 ? s_rows[e - 1] : 0;
-    const int seat0 = (block - before) << BM_BITS, row0 = first + seat0;
+    const int seat0 = ((block - before) << BM_BITS) + (over & 1 ? half : 0), row0 = first + seat0;
     Tile at;
     at.e = __builtin_amdgcn_readfirstlane(e);
     at.row0 = __builtin_amdgcn_readfirstlane(row0);
-    at.rows = __builtin_amdgcn_readfirstlane(min(BM, s_rows[e] - row0));
+    at.rows = __builtin_amdgcn_readfirstlane(min(BM - half, s_rows[e] - row0));
     at.n0 = __builtin_amdgcn_readfirstlane(in / wide * BN);
     return at;
   };
@@ -464,7 +470,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
     if constexpr (GO_ROUND) scales_at += ahead_kt * scales_step;
     scales_bytes = column_scales ? 4 : max(0, min(64, at.rows - scales_of * 64)) * 4;
   };
-  Tile at = tile_at(static_cast<int>(t));
+  Tile at = tile_at(t);
+  if (at.rows <= 0) return;
   aim(at);
   auto request = [&] {
     const uint32_t from = ahead_kt * kB, to = lds0 + into;
@@ -498,7 +505,9 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
     }
     t += gridDim.x;
     if (t >= tiles) return false;
-    aim(tile_at(static_cast<int>(t)));
+    const Tile next = tile_at(t);
+    if (next.rows <= 0) return false;
+    aim(next);
     return true;
   };
 
@@ -592,7 +601,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
     }
     done += gridDim.x;
     if (done >= tiles) return;
-    at = tile_at(static_cast<int>(done));
+    at = tile_at(done);
+    if (at.rows <= 0) return;
   }
 }
 
