@@ -255,7 +255,7 @@ __device__ __forceinline__ void finish8(const Fp8Args& a, size_t row, int n, boo
   const size_t at = row * a.N + n;
   char* const to = static_cast<char*>(a.out) + at * elem_bytes(OUT);
   if (whole) {
-    pack_store<OUT, 8>(to, v);
+    pack_store<OUT, 8, true>(to, v);
   } else {
 #pragma unroll
     for (int q = 0; q < 8; ++q)
