@@ -822,24 +822,27 @@ int launch_tiles(Fp8Args& a, hipStream_t st) {
 //   64 x 64, four stages, while they go once round the chip: 400 rows of 8 experts 1024 -> 4096 9.8, 64 x 128 12;
 //   64 x 128, three stages, while 128 x 256 tiles do not, and for less than 64 rows an expert: 1500 rows of 4 experts 768 -> 2048
 //   9, 64 x 64 13, 128 x 256 12; 2048 rows of 128 experts 1024 -> 2048 56, 128 x 256 58;
-//   128 x 256 and 256 x 256 by the rounds over the CUs that they take, at 1.05 and 1.75 us a K-step and 4 and 6 a tile: 8192 rows of
-//   64 experts 1024 -> 4096 80 and 85, 8192 of 32 4096 -> 1024 (two rounds and one) 86 and 76, 16384 of 8 4096 -> 4096 315 and 290.
+//   128 x 256 and 256 x 256 by the rounds over the CUs that they take (one, or the share of one and half of one), at 1.05 and 1.75 us a
+//   K-step and 4 and 6.5 a tile, 6.5 and 12.5 with fp32 results: 16384 rows of 64 experts 1024 -> 4096 119 and 129, 8192 of 32 1024
+//   -> 4096 63 and 68, 8192 of 32 4096 -> 1024 61 and 57, 16384 of 8 4096 -> 4096 294 and 268, 16384 of 16 1024 -> 2048 fp32 74 and 83.
 enum TileKind { k64x64, k64x128, k128x128, k128x256, k256x256 };
-TileKind tile_kind(int E, int P, int N, int K, bool exact) {
+TileKind tile_kind(int E, int P, int N, int K, int out_dtype, bool exact) {
   const long used = std::min(E, P);
   auto tiles = [&](int rows, int columns) { return (2l * P / rows + used + 1) / 2 * ((N + columns - 1) / columns); };
   if (tiles(64, 64) <= 640) return k64x64;
   if (exact) return k128x128;
   if (tiles(128, 256) < 256 || P < 64l * E) return k64x128;
   const long cus = kXcds * kCusPerXcd, steps = (K + kB - 1) / kB;
-  const long wide = (tiles(256, 256) + cus - 1) / cus * (35 * steps + 120), half = (tiles(128, 256) + cus - 1) / cus * (21 * steps + 80);
+  const bool f32 = out_dtype == BRT_F32;
+  auto rounds = [&](long n) { return n <= cus ? cus : n + cus / 2; };  // (in CUs; a tile's time in twentieths of a microsecond)
+  const long wide = rounds(tiles(256, 256)) * (35 * steps + (f32 ? 250 : 130)), half = rounds(tiles(128, 256)) * (21 * steps + (f32 ? 130 : 80));
   return wide < half ? k256x256 : k128x256;
 }
 bool quantizes_result(int E, int P, int N, int K, int out_dtype) {
-  return !few_rows(P, E, N) && out_dtype == BRT_BF16 && tile_kind(E, P, N, K, false) != k64x64;
+  return !few_rows(P, E, N) && out_dtype == BRT_BF16 && tile_kind(E, P, N, K, out_dtype, false) != k64x64;
 }
 int launch_any_tiles(Fp8Args& a, hipStream_t st) {
-  TileKind kind = tile_kind(a.E, a.P, a.N, a.K, a.exact != 0);
+  TileKind kind = tile_kind(a.E, a.P, a.N, a.K, a.out_dtype, a.exact != 0);
   // (quantizing 256 x 256 results needs more registers than there are: 8192 rows of 32 experts 1024 -> 4096 + GELU 101 us, 128 x 256 88)
   if (kind == k256x256 && a.out_scales != nullptr) kind = k128x256;
   switch (kind) {
