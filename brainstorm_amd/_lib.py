@@ -264,6 +264,7 @@ def call_count() -> int:
     """Calls into the library that queued device work since the process started, read-backs of a few words
     among them.  Every such call is one kernel launch, except the compact route, the tag-index gather and the throttled
     top-1 route, which are two, and index generation and throttling, which are one or two by the size of the mask.
+    A product in 8 bits is one launch, or two where its rows are quantized first; a gradient of the route is one.
     Tests use the difference around a layer to pin how many launches a route costs."""
     return _calls + (_native.calls() if _native is not None else 0)
 
