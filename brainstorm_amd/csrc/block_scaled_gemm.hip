@@ -222,29 +222,31 @@ __device__ __forceinline__ void finish(const Fp8Args& a, size_t row, int n, bool
   }
 }
 
-// The products of a K-step on their way into the accumulators: while one is on the matrix pipe, the one two before it is scaled
-// and added.  What is left of a K-step is added while the next one's fragments come, with its scales still.  (sched_barrier keeps
-// the order: left alone the compiler puts each addition behind its product and waits for it.)
+// The products of a K-step on their way into the accumulators: while one is on the matrix pipe, the one three before it is scaled
+// and added (two before it: 16384 rows of 8 experts 4096 -> 4096 271 us, three 256, four to six the same).  What is left of a K-step
+// is added while the next one's fragments come, with its scales still.  (sched_barrier keeps the order: left alone the compiler puts
+// each addition behind its product and waits for it.)
 template <int MT, int NT>
 struct Pipe {
-  f32x4 held[4];
+  static constexpr int kBehind = 3;
+  f32x4 held[kBehind + 1];
   __device__ __forceinline__ Pipe() { clear(); }
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int p = 0; p < 4; ++p) held[p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p = 0; p <= kBehind; ++p) held[p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
   __device__ __forceinline__ void add(int p, f32x4 (&acc)[MT][NT], const float (&s)[MT]) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) acc[p % MT][p / MT][q] = __builtin_fmaf(held[p & 3][q], s[p % MT], acc[p % MT][p / MT][q]);
+    for (int q = 0; q < 4; ++q) acc[p % MT][p / MT][q] = __builtin_fmaf(held[p % (kBehind + 1)][q], s[p % MT], acc[p % MT][p / MT][q]);
   }
   __device__ __forceinline__ void put(int p, const f32x4& product, f32x4 (&acc)[MT][NT], const float (&s)[MT]) {
-    held[p & 3] = product;
-    if (p >= 2) add(p - 2, acc, s);
+    held[p % (kBehind + 1)] = product;
+    if (p >= kBehind) add(p - kBehind, acc, s);
     __builtin_amdgcn_sched_barrier(0);
   }
   __device__ __forceinline__ void drain(f32x4 (&acc)[MT][NT], const float (&s)[MT]) {
-    add(MT * NT - 2, acc, s);
-    add(MT * NT - 1, acc, s);
+#pragma unroll
+    for (int p = MT * NT - kBehind; p < MT * NT; ++p) add(p, acc, s);
   }
 };
 
@@ -256,7 +258,8 @@ __device__ __forceinline__ void finish8(const Fp8Args& a, size_t row, int n, boo
   const size_t at = row * a.N + n;
   char* const to = static_cast<char*>(a.out) + at * elem_bytes(OUT);
   if (whole) {
-    pack_store<OUT, 8, true>(to, v);
+    // (streaming stores: 16384 rows of 8 experts 4096 -> 4096 bf16 292 -> 274 us; fp32 results of 16384 rows 1024 -> 2048 69 -> 75)
+    pack_store<OUT, 8, OUT != BRT_F32>(to, v);
   } else {
 #pragma unroll
     for (int q = 0; q < 8; ++q)
@@ -364,9 +367,9 @@ __device__ __forceinline__ void store_blocks(const Fp8Args& a, const Block& at, 
 // its requests run on through their boundaries: a tile of 1024 elements has eight K-steps, and starting anew (which expert, the
 // first K-step) took as long as half of them.  The list of row blocks is kept in LDS for that.
 //
-// Bound by the matrix pipe beside the additions and the requests: 16384 rows of 8 experts 4096 -> 4096 274 us (2.0 PFLOP/s; the same
-// instructions from registers alone 3.6, without the requests 2.3); by the weights' way from memory with fewer rows: 8192 of 64 experts
-// 1024 -> 4096 80 us, of which the weights' 268 MB are 52.
+// Bound by the matrix pipe beside the additions and the requests: 16384 rows of 8 experts 4096 -> 4096 256 us (2.15 PFLOP/s; the same
+// instructions from registers alone 3.6, the requests cost 40 to 60 of it); by the weights' way from memory with fewer rows: 8192 of 64 experts
+// 1024 -> 4096 75 us, of which the weights' 268 MB are 52.
 template <int BM_BITS, int BN, int WM, int WN, int STAGES, bool GO_ROUND, bool EXACT, bool BLOCKS>
 __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
   constexpr int BM = 1 << BM_BITS, WAVES = WM * WN;
@@ -569,26 +572,29 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
       i32x8 w = fragment(wlo, whi), x_read[MT];
       float s_read[MT];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        x_read[i] = fragment(xlo + i * 16 * kB, xhi + i * 16 * kB);
-        s_read[i] = *reinterpret_cast<const float*>(stage + kRowScales + (xr + i * 16) * 4);
-      }
+      for (int i = 0; i < MT; ++i) x_read[i] = fragment(xlo + i * 16 * kB, xhi + i * 16 * kB);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) s_read[i] = *reinterpret_cast<const float*>(stage + kRowScales + (xr + i * 16) * 4);
       const float scale = *reinterpret_cast<const float*>(stage + kColumnScales + wn * 256);
       if constexpr (!kRequestsFirst) request_ahead();
       __builtin_amdgcn_sched_barrier(0);
       pipe.drain(acc, s);
       Operand x[MT];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        x[i] = operand<EXACT>(x_read[i]);
-        s[i] = s_read[i] * scale;
-      }
+      for (int i = 0; i < MT; ++i) x[i] = operand<EXACT>(x_read[i]);
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const Operand at_hand = operand<EXACT>(w);
         if (j + 1 < NT) w = fragment(wlo + column_of(j + 1) * kB, whi + column_of(j + 1) * kB);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) pipe.put(j * MT + i, multiply(at_hand, x[i]), acc, s);
+        for (int i = 0; i < MT; ++i) {
+          const int p = j * MT + i;
+          if (p == pipe.kBehind) {  // (not earlier: the first products wait for their own fragments only)
+#pragma unroll
+            for (int r = 0; r < MT; ++r) s[r] = s_read[r] * scale;
+          }
+          pipe.put(p, multiply(at_hand, x[i]), acc, s);
+        }
       }
     }
     pipe.drain(acc, s);
@@ -822,20 +828,23 @@ int launch_tiles(Fp8Args& a, hipStream_t st) {
 //   64 x 64, four stages, while they go once round the chip: 400 rows of 8 experts 1024 -> 4096 9.8, 64 x 128 12;
 //   64 x 128, three stages, while 128 x 256 tiles do not, and for less than 64 rows an expert: 1500 rows of 4 experts 768 -> 2048
 //   9, 64 x 64 13, 128 x 256 12; 2048 rows of 128 experts 1024 -> 2048 56, 128 x 256 58;
-//   128 x 256 and 256 x 256 by the rounds over the CUs that they take (one, or the share of one and half of one), at 1.05 and 1.75 us a
-//   K-step and 4 and 6.5 a tile, 6.5 and 12.5 with fp32 results: 16384 rows of 64 experts 1024 -> 4096 119 and 129, 8192 of 32 1024
-//   -> 4096 63 and 68, 8192 of 32 4096 -> 1024 61 and 57, 16384 of 8 4096 -> 4096 294 and 268, 16384 of 16 1024 -> 2048 fp32 74 and 83.
+//   128 x 256 and 256 x 256 by the rounds over the CUs that they take (one, or the share of one and half of one), at 1.05 and 1.6 us a
+//   K-step and 4 and 7.5 a tile, 6.5 and 13.5 with fp32 results: 16384 rows of 64 experts 1024 -> 4096 118 and 126, 8192 of 32 1024
+//   -> 4096 61 and 63, 8192 of 32 4096 -> 1024 59 and 53, 16384 of 8 4096 -> 4096 303 and 267, 16384 of 16 1024 -> 2048 fp32 69 and 81.
 enum TileKind { k64x64, k64x128, k128x128, k128x256, k256x256 };
 TileKind tile_kind(int E, int P, int N, int K, int out_dtype, bool exact) {
   const long used = std::min(E, P);
-  auto tiles = [&](int rows, int columns) { return (2l * P / rows + used + 1) / 2 * ((N + columns - 1) / columns); };
+  auto tiles = [&](int rows, int columns) {
+    const long blocks = used == 1 ? (P + rows - 1) / rows : (2l * P / rows + used + 1) / 2;
+    return blocks * ((N + columns - 1) / columns);
+  };
   if (tiles(64, 64) <= 640) return k64x64;
   if (exact) return k128x128;
   if (tiles(128, 256) < 256 || P < 64l * E) return k64x128;
   const long cus = kXcds * kCusPerXcd, steps = (K + kB - 1) / kB;
   const bool f32 = out_dtype == BRT_F32;
   auto rounds = [&](long n) { return n <= cus ? cus : n + cus / 2; };  // (in CUs; a tile's time in twentieths of a microsecond)
-  const long wide = rounds(tiles(256, 256)) * (35 * steps + (f32 ? 250 : 130)), half = rounds(tiles(128, 256)) * (21 * steps + (f32 ? 130 : 80));
+  const long wide = rounds(tiles(256, 256)) * (32 * steps + (f32 ? 270 : 150)), half = rounds(tiles(128, 256)) * (21 * steps + (f32 ? 130 : 80));
   return wide < half ? k256x256 : k128x256;
 }
 bool quantizes_result(int E, int P, int N, int K, int out_dtype) {
