@@ -260,6 +260,28 @@ def test_loads_that_name_more_rows_than_there_are(rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("k", [144, 1024])
+@pytest.mark.parametrize("loads", [[4600, 0], [4290, 310], [256 * 17, 248], [4000, 129], [2100, 128, 2200, 172], [1, 4599]])
+def test_a_last_round_of_few_tiles(loads, k):
+    """288 to 320 tiles of 256 x 256, or 576 to 624 of 128 x 256: the last round's are dealt out by halves, of which the second may be empty."""
+    n, rows = 4096, 4600
+    w, ws = weights(1, len(loads), n, k)
+    loads = torch.tensor(loads, dtype=torch.int32)
+    x = normal(2, rows, k, dtype=torch.bfloat16)
+    xq, xs = quantized_here(x)
+    want, size = product_in_64(xq, xs, w, ws, loads)
+    for dtype in (torch.bfloat16, torch.float16):
+        out = torch.full((rows, n), 7.0, dtype=dtype, device="cuda")
+        assert_near(grouped_linear_fp8(x.cuda(), w.cuda(), ws.cuda(), loads.cuda(), out=out), want, size, -(-k // 128))
+        assert bool((out[int(loads.sum()):] == 7.0).all())
+    q, scales = grouped_linear_fp8(x.cuda(), w.cuda(), ws.cuda(), loads.cuda(), out_blocks=True)
+    last = int(loads.sum())
+    plain = quantize_rows(grouped_linear_fp8(x.cuda(), w.cuda(), ws.cuda(), loads.cuda())[:last])
+    assert torch.equal(scales[:last], plain[1])  # (both kinds of tiles add up the blocks from the first on)
+    assert torch.equal(q[:last].view(torch.uint8), plain[0].view(torch.uint8))
+
+
+@pytest.mark.gpu
 def test_many_experts():
     """More than the list in LDS holds: the kernel for few rows takes them, with any number of rows."""
     k, n, experts = 144, 72, 600
