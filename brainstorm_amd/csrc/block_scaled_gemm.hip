@@ -826,8 +826,9 @@ int launch_tiles(Fp8Args& a, hipStream_t st) {
 
 // Tiles by what there is to deal out, a list's last row blocks taken as half full (us; without the launch that quantizes):
 //   64 x 64, four stages, while they go once round the chip: 400 rows of 8 experts 1024 -> 4096 9.8, 64 x 128 12;
-//   64 x 128, three stages, while 128 x 256 tiles do not, and for less than 64 rows an expert: 1500 rows of 4 experts 768 -> 2048
-//   9, 64 x 64 13, 128 x 256 12; 2048 rows of 128 experts 1024 -> 2048 56, 128 x 256 58;
+//   64 x 128, three stages, likewise (two workgroups on a CU), and for less than 64 rows an expert: 1500 rows of 4 experts 768 -> 2048
+//   9, 64 x 64 13, 128 x 256 11, 2500 of 16 4096 -> 1024 25, 128 x 256 34, but 4096 of 8 4096 -> 1024 47 and 36, 6000 of 16 1024 ->
+//   1024 18 and 13; 2048 rows of 128 experts 1024 -> 2048 56, 128 x 256 58;
 //   128 x 256 and 256 x 256 by the rounds over the CUs that they take (one, or the share of one and half of one), at 1.05 and 1.6 us a
 //   K-step and 4 and 7.5 a tile, 6.5 and 13.5 with fp32 results: 16384 rows of 64 experts 1024 -> 4096 118 and 126, 8192 of 32 1024
 //   -> 4096 61 and 63, 8192 of 32 4096 -> 1024 59 and 53, 16384 of 8 4096 -> 4096 303 and 267, 16384 of 16 1024 -> 2048 fp32 69 and 81.
@@ -840,7 +841,7 @@ TileKind tile_kind(int E, int P, int N, int K, int out_dtype, bool exact) {
   };
   if (tiles(64, 64) <= 640) return k64x64;
   if (exact) return k128x128;
-  if (tiles(128, 256) < 256 || P < 64l * E) return k64x128;
+  if (tiles(64, 128) <= 512 || P < 64l * E) return k64x128;
   const long cus = kXcds * kCusPerXcd, steps = (K + kB - 1) / kB;
   const bool f32 = out_dtype == BRT_F32;
   auto rounds = [&](long n) { return n <= cus ? cus : n + cus / 2; };  // (in CUs; a tile's time in twentieths of a microsecond)
