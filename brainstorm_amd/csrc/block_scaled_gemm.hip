@@ -824,9 +824,11 @@ int launch_tiles(Fp8Args& a, hipStream_t st) {
   return launch_tiles<BM_BITS, BN, WM, WN, STAGES, GO_ROUND, false, false>(a, st);
 }
 
-// Tiles by what there is to deal out, a list's last row blocks taken as half full (us; without the launch that quantizes):
-//   64 x 64, four stages, while they go once round the chip: 400 rows of 8 experts 1024 -> 4096 9.8, 64 x 128 12;
-//   64 x 128, three stages, likewise (two workgroups on a CU), and for less than 64 rows an expert: 1500 rows of 4 experts 768 -> 2048
+// Tiles by what there is to deal out, the experts' last row blocks taken as half full, and a mean load of less than 0.8 of a block as one
+// block (us; without the launch that quantizes):
+//   64 x 64, four stages, while they go once round the chip, two workgroups on a CU: 400 rows of 8 experts 1024 -> 4096 8.9, 64 x 128
+//   12.7, but 1000 of 8 512 -> 2048 10.9 and 7.6;
+//   64 x 128, three stages, likewise, and for less than 64 rows an expert: 1500 rows of 4 experts 768 -> 2048
 //   9, 64 x 64 13, 128 x 256 11, 2500 of 16 4096 -> 1024 25, 128 x 256 34, but 4096 of 8 4096 -> 1024 47 and 36, 6000 of 16 1024 ->
 //   1024 18 and 13; 2048 rows of 128 experts 1024 -> 2048 56, 128 x 256 58;
 //   128 x 256 and 256 x 256 by the rounds over the CUs that they take (one, or the share of one and half of one), at 1.05 and 1.6 us a
@@ -836,10 +838,10 @@ enum TileKind { k64x64, k64x128, k128x128, k128x256, k256x256 };
 TileKind tile_kind(int E, int P, int N, int K, int out_dtype, bool exact) {
   const long used = std::min(E, P);
   auto tiles = [&](int rows, int columns) {
-    const long blocks = used == 1 ? (P + rows - 1) / rows : (2l * P / rows + used + 1) / 2;
+    const long blocks = used == 1 ? (P + rows - 1) / rows : 5l * P <= 4l * rows * used ? used : (2l * P / rows + used + 1) / 2;
     return blocks * ((N + columns - 1) / columns);
   };
-  if (tiles(64, 64) <= 640) return k64x64;
+  if (tiles(64, 64) <= 512) return k64x64;
   if (exact) return k128x128;
   if (tiles(64, 128) <= 512 || P < 64l * E) return k64x128;
   const long cus = kXcds * kCusPerXcd, steps = (K + kB - 1) / kB;
