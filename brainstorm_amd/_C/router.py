@@ -731,10 +731,12 @@ def combine_by_rows(in_data: torch.Tensor, path_ids: torch.Tensor, seat_rows: to
     a row.  It is then a tensor of its own: ``out_data`` is not taken.  No gradients of these gradients."""
     if gates is not None and weights is not None:
         raise RuntimeError("weights or gates, not both")
-    if row_entries is not None and gates is not None:
-        weights, gates = torch.gather(gates, 1, path_ids.long()).to(torch.float32), None
-    if gates is not None and not (gates.dtype in _DT and gates.dim() == 2 and gates.size(0) == path_ids.size(0)
-                                  and gates.numel() < 1 << 31):
-        # what the kernel does not read in place: other types (fp64 gates), more rows than cells
-        weights, gates = torch.gather(gates, 1, path_ids.long()).to(torch.float32), None
+    if gates is not None and (row_entries is not None or not (
+            gates.dtype in _DT and gates.dim() == 2 and gates.size(0) == path_ids.size(0) and gates.numel() < 1 << 31)):
+        # gradients, and what the kernel does not read in place: other types (fp64 gates), more rows than cells
+        if gates.dim() != 2 or (gates.size(1) == 0 and path_ids.numel() > 0):
+            raise RuntimeError("gates must be [cells, paths] with at least one path")
+        # (an id outside the paths names none: its entry owns no row, and no weight or gradient of it is used)
+        weights = torch.gather(gates, 1, path_ids.long().clamp(0, gates.size(1) - 1)).to(torch.float32)
+        gates = None
     return _lib.native().combine_by_rows(in_data, path_ids, seat_rows, weights, out_data, out_dtype, gates, row_entries)

@@ -321,6 +321,58 @@ def test_gates_of_a_differentiable_combine():
     near(dgates, want, torch.zeros_like(want).scatter_(1, ids.long(), products.abs().sum(2)), d)
 
 
+def test_gates_are_not_read_at_ids_outside_the_paths(monkeypatch):
+    """An id below zero or beyond the paths names no path: the weight handed to the kernel comes from the row of the cell all the same,
+    and so does its gradient's place."""
+    from brainstorm_amd import _lib
+
+    class Handed:
+        @staticmethod
+        def combine_by_rows(in_data, path_ids, seat_rows, weights, out_data, out_dtype, gates, row_entries):
+            return weights
+
+    monkeypatch.setattr(_lib, "native", lambda: Handed)
+    ids = torch.tensor([[-1, 2], [3, 0], [2 ** 31 - 1, -2 ** 31]], dtype=torch.int32)
+    entries = torch.zeros(2, dtype=torch.int32)
+    for gates, row_entries in ((torch.arange(9.0).view(3, 3), entries), (torch.arange(9.0, dtype=torch.float64).view(3, 3), None),
+                               (torch.arange(12.0).view(4, 3), None)):
+        gates.requires_grad_()
+        weights = c_router.combine_by_rows(None, ids, None, gates=gates, row_entries=row_entries)
+        assert weights.dtype == torch.float32 and weights[0, 1] == 2.0 and weights[1, 1] == 3.0
+        (found,) = torch.autograd.grad(weights, gates, torch.tensor([[0.0, 1.0], [0.0, 1.0], [0.0, 0.0]]))
+        assert found[0, 2] == 1.0 and found[1, 0] == 1.0 and found.sum() == 2.0
+    with pytest.raises(RuntimeError, match="at least one path"):
+        c_router.combine_by_rows(None, ids, None, gates=torch.zeros(3, 0), row_entries=entries)
+    with pytest.raises(RuntimeError, match="at least one path"):
+        c_router.combine_by_rows(None, ids, None, gates=torch.zeros(9), row_entries=entries)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_gates_of_entries_without_a_path(dtype):
+    """Ids of -1 and beyond the paths, in the first cell and the last: result and gradients of the entries that have a path."""
+    cells, paths, k, d = 33, 5, 3, 16
+    ids, _, _ = make_route(cells, paths, k, 40, 1, keep=0.7)
+    ids[0, 0], ids[0, 1], ids[-1] = -1, paths, torch.tensor([2 ** 31 - 1, -2 ** 31, paths + 3])
+    _, _, seat_rows, row_entries = c_router.route_by_path(ids, paths, rows=cells * k)
+    assert not seat_rows[(ids < 0) | (ids >= paths)].any()
+    y = normal(1, row_entries.numel(), d).requires_grad_()
+    gates = normal(2, cells, paths, dtype=TYPES[dtype]).requires_grad_()
+    out = c_router.combine_by_rows(y, ids, seat_rows, gates=gates, row_entries=row_entries)
+    assert torch.equal(out, c_router.combine_by_rows(y.detach(), ids, seat_rows, gates=gates.detach()))
+    wide = gates.detach().double()  # (weights from outside the kernel)
+    assert torch.equal(out, c_router.combine_by_rows(y.detach(), ids, seat_rows, gates=wide))
+    back = normal(3, cells, d)
+    dy, dgates = torch.autograd.grad(out, [y, gates], back)
+    column = ids.long().clamp(0, paths - 1)
+    products = of_entries(y.detach(), seat_rows) * back.double()[:, None]
+    zero = torch.zeros(cells, paths, dtype=torch.float64, device="cuda")
+    near(dgates, zero.scatter_add(1, column, products.sum(2)), zero.scatter_add(1, column, products.abs().sum(2)), d)
+    entry = (row_entries.long() - 1).clamp(min=0)
+    want = back.double()[entry // k] * gates.detach().double().gather(1, column).reshape(-1)[entry][:, None]
+    near(dy, torch.where((row_entries > 0)[:, None], want, 0.0), want.abs(), 1)
+
+
 @pytest.mark.gpu
 def test_gradients_of_gradients_are_refused():
     cells, k, d = 20, 1, 16
