@@ -186,9 +186,12 @@ __device__ __forceinline__ Block find_block(const Fp8Args& a, int block, int bit
   return {0, 0, 0};
 }
 
+// Activations hand NaN on: a row that holds NaN or an infinity has results of NaN, not zeros that look sound, in blocks too.
+template <int ACT>
+__device__ __forceinline__ float activated(float v) { return apply_act<ACT, true>(v); }
 __device__ __forceinline__ float activated(float v, int act) {
-  if (act == BRT_ACT_GELU) return gelu_erf(v);
-  if (act == BRT_ACT_RELU) return fmaxf(v, 0.0f);
+  if (act == BRT_ACT_GELU) return activated<BRT_ACT_GELU>(v);
+  if (act == BRT_ACT_RELU) return activated<BRT_ACT_RELU>(v);
   return v;
 }
 
@@ -254,7 +257,7 @@ struct Pipe {
 template <int ACT, int OUT>
 __device__ __forceinline__ void finish8(const Fp8Args& a, size_t row, int n, bool whole, const float (&bias)[8], float (&v)[8]) {
 #pragma unroll
-  for (int q = 0; q < 8; ++q) v[q] = apply_act<ACT>(v[q] + bias[q]);
+  for (int q = 0; q < 8; ++q) v[q] = activated<ACT>(v[q] + bias[q]);
   const size_t at = row * a.N + n;
   char* const to = static_cast<char*>(a.out) + at * elem_bytes(OUT);
   if (whole) {
@@ -322,7 +325,7 @@ __device__ __forceinline__ void store_blocks(const Fp8Args& a, const Block& at, 
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         // (columns behind the last are zero; the value is held as the bf16 it was rounded to)
-        const float v = n + q < a.N ? bf16_to_float(float_to_bf16(apply_act<ACT>(acc[i][j][q] + bias[q]))) : 0.0f;
+        const float v = n + q < a.N ? bf16_to_float(float_to_bf16(activated<ACT>(acc[i][j][q] + bias[q]))) : 0.0f;
         acc[i][j][q] = v;
         top[i] = max(top[i], magnitude(v));
       }

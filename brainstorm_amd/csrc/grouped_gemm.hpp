@@ -66,6 +66,14 @@ __device__ __forceinline__ int routed_cell(const GemmArgs& a, int e, int row, in
 // Against the erf form in double the result is within 4.3e-6 absolute everywhere, two orders below
 // half a bf16 step at the values where that bound is reached.  The clamp keeps +-inf inputs from
 // turning inf * 0 into NaN.  Cost per element: seven multiply-adds, one exp2, min, max, one more fma.
+//   Of NaN fmaxf(v, 0) makes 0, and so does GELU (the clamp has made its tail 0).  KEEP_NAN takes the maximum that hands NaN on (one
+// instruction, v_maximum3_f32); every other value has the same bits.
+template <bool KEEP_NAN>
+__device__ __forceinline__ float positive_part(float v) {
+  if constexpr (KEEP_NAN) return __builtin_elementwise_maximum(v, 0.0f);
+  else return fmaxf(v, 0.0f);
+}
+template <bool KEEP_NAN = false>
 __device__ __forceinline__ float gelu_erf(float v) {
   const float av = fminf(fabsf(v), 1e30f);
   float q = -1.262479145e-06f;
@@ -76,13 +84,13 @@ __device__ __forceinline__ float gelu_erf(float v) {
   q = __builtin_fmaf(q, av, -4.599574506e-01f);
   q = __builtin_fmaf(q, av, -1.150609374e+00f);
   q = __builtin_fmaf(q, av, -1.000043273e+00f);
-  return __builtin_fmaf(-av, __builtin_amdgcn_exp2f(q), fmaxf(v, 0.0f));
+  return __builtin_fmaf(-av, __builtin_amdgcn_exp2f(q), positive_part<KEEP_NAN>(v));
 }
 
-template <int ACT>
+template <int ACT, bool KEEP_NAN = false>
 __device__ __forceinline__ float apply_act(float v) {
-  if (ACT == BRT_ACT_GELU) return gelu_erf(v);
-  if (ACT == BRT_ACT_RELU) return fmaxf(v, 0.0f);
+  if (ACT == BRT_ACT_GELU) return gelu_erf<KEEP_NAN>(v);
+  if (ACT == BRT_ACT_RELU) return positive_part<KEEP_NAN>(v);
   return v;
 }
 

@@ -132,6 +132,30 @@ def test_blocks_with_nan_and_infinity_and_tiny_values():
     assert out[0].isnan().all() and out[1].isnan().all() and torch.isfinite(out[2:]).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", [None, "relu", "gelu"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,k,n,experts", [(6, 256, 64, 1), (40, 256, 72, 3), (200, 256, 384, 2), (1000, 384, 144, 1), (3000, 272, 3008, 60),
+                                              (3100, 128, 4112, 3), (2200, 256, 16400, 2)])
+def test_activations_hand_nan_on(rows, k, n, experts, dtype, activation):
+    """Rows that hold NaN or an infinity are NaN in every kind of kernel, also as blocks; the rows beside them keep their bits."""
+    w, ws = (t.cuda() for t in weights(2, experts, n, k))
+    loads, bias = loads_of(3, rows, experts).cuda(), normal(4, experts, n).cuda()
+    good = normal(1, rows, k, dtype=TYPES[dtype]).cuda()
+    x = good.clone()
+    bad = torch.tensor([0, rows // 2, rows - 1], device="cuda")
+    x[bad[0], 3], x[bad[1], k - 1], x[bad[2], k // 2] = float("nan"), float("inf"), float("-inf")
+    kept = torch.ones(rows, dtype=torch.bool, device="cuda").index_fill(0, bad, False)
+    out = grouped_linear_fp8(x, w, ws, loads, bias=bias, activation=activation)
+    assert out[bad].isnan().all()
+    assert torch.equal(out[kept], grouped_linear_fp8(good, w, ws, loads, bias=bias, activation=activation)[kept])
+    if n % 16 == 0:
+        q, scales = grouped_linear_fp8(x, w, ws, loads, bias=bias, activation=activation, out_blocks=True)
+        assert scales[bad].isnan().all() and q[bad].float().isnan().all()
+        want, want_scales = grouped_linear_fp8(good, w, ws, loads, bias=bias, activation=activation, out_blocks=True)
+        assert torch.equal(scales[kept], want_scales[kept]) and torch.equal(q[kept].view(torch.uint8), want[kept].view(torch.uint8))
+
+
 CASES = [  # rows, in, out, experts
     (1, 16, 1, 1), (1, 128, 64, 1), (1, 2048, 520, 4), (2, 1040, 129, 3), (5, 272, 136, 8), (17, 144, 72, 2), (48, 1024, 512, 8),
     (33, 512, 4, 1), (64, 640, 260, 1), (100, 384, 256, 130), (129, 256, 136, 1), (300, 2064, 200, 2), (700, 128, 384, 4),
