@@ -219,7 +219,12 @@ __global__ __launch_bounds__(kBlock) void dispatch_grad_kernel(RowsGradArgs a) {
         pack_store<DT, NE, kStream>(static_cast<u32x4*>(a.out) + cell * a.cpr + off, acc);
     }
   }
-  if (dots) store_dots<KMAX>(a, slot0, live, LPR, glane, dot);
+  if (dots) {
+    // an entry without a row was summed as 0 * x, which an x that is not finite makes NaN: its gradient is zero
+#pragma unroll
+    for (int j = 0; j < KMAX; ++j) dot[j] = has[j] ? dot[j] : 0.0f;
+    store_dots<KMAX>(a, slot0, live, LPR, glane, dot);
+  }
 }
 
 template <int DT, bool G32, int LS, int UPR, int KMAX>

@@ -222,6 +222,36 @@ def test_what_belongs_to_no_entry_is_not_looked_at():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("k,d", [(1, 8), (2, 32), (3, 264), (8, 1032)])
+def test_cells_that_are_not_finite_and_entries_without_a_row(k, d, dtype):
+    """The weight of an entry without a row has the gradient zero, whatever its cell and the gradient of its result hold."""
+    cells, paths, dtype = 24, 9, TYPES[dtype]
+    ids, _, _ = make_route(cells, paths, k, 40, 1)
+    ids[:3], ids[3:9, ::2] = -1, -1  # all entries of some cells have no row, every other one of some
+    _, _, seat_rows, row_entries = c_router.route_by_path(ids, paths, rows=cells * k)
+    given = normal(2, cells, d, dtype=dtype)
+    x = given.clone()
+    x[0], x[1, 5], x[3, 0], x[4], x[5, d - 1] = float("nan"), float("inf"), float("inf"), float("nan"), float("-inf")
+    w = normal(3, cells, k).requires_grad_()
+    grad = normal(4, row_entries.numel(), d, dtype=dtype)
+
+    def of_dispatch(x):
+        return torch.autograd.grad(c_router.dispatch_by_rows(x, row_entries, k, w, seat_rows=seat_rows), w, grad)[0]
+
+    dw, sound = of_dispatch(x), of_dispatch(given)
+    assert not dw[seat_rows == 0].any()
+    assert not torch.isfinite(dw[3:6][seat_rows[3:6] > 0]).any()
+    finite = torch.isfinite(x).all(1)
+    assert torch.equal(dw[finite], sound[finite])
+    # the combine's: rows and gradients that are not finite beside entries without a row
+    y = normal(5, row_entries.numel(), d, dtype=dtype)
+    out = c_router.combine_by_rows(y, ids, seat_rows, w, row_entries=row_entries)
+    (dw,) = torch.autograd.grad(out, w, x)
+    assert not dw[seat_rows == 0].any() and not torch.isfinite(dw[3:6][seat_rows[3:6] > 0]).any()
+
+
+@pytest.mark.gpu
 def test_gate_gradient_of_masked_scores():
     """Scores of -inf have no probability and no gradient; a row of nothing else is NaN, as its softmax is."""
     scores = normal(1, 4, 40)
