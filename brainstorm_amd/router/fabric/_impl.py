@@ -619,11 +619,16 @@ class FusedCombineFabric(CombineFabric):
         if route.differentiable:
             if gates is not None and (gates.dim() != 2 or gates.size(1) < route.paths):
                 raise RuntimeError(f"the score does not have a column for each of {route.paths} paths")
-            out = c_router.combine_by_rows(data, route.path_ids, route.seat_rows, gates=gates, row_entries=route.row_entries)
+            out = c_router.combine_by_rows(data, route.path_ids, route.seat_rows, gates=gates, row_entries=route.row_entries,
+                                           out_dtype=None if residual is None else residual.dtype)
             if residual is None:
                 return out
-            has_row = (route.seat_rows > 0).any(dim=1).view([-1] + [1] * (out.dim() - 1))
-            return torch.where(has_row, out, residual.view_as(out).to(out.dtype))
+            # the residual's type and shape, as when it is written in place
+            if residual.numel() != out.numel():
+                raise RuntimeError("the residual does not have the elements of the cells")
+            flat = (route.cells, out.numel() // route.cells)
+            has_row = (route.seat_rows > 0).any(dim=1, keepdim=True)
+            return torch.where(has_row, out.view(flat), residual.reshape(flat)).view(residual.shape)
         if residual is not None and not residual.is_contiguous():
             raise RuntimeError("the residual must be contiguous (it is updated in place)")
         if route.k == 1 and gates is None:

@@ -570,6 +570,39 @@ def test_a_layer_of_routers_that_trains(k, weighted, capacity):
         torch.testing.assert_close(a.double(), b, rtol=1e-4, atol=1e-4)
 
 
+def routed_layer(differentiable, k, weighted, capacity, x, score, residual):
+    """A scatter router, experts that scale their rows and a gather router with a residual."""
+    from brt import Annotator, to_grid_tensor, to_torch_tensor
+    from brt.router import GatherRouter, ScatterRouter
+
+    scatter = ScatterRouter(protocol_type="topk", protocol_kwargs={"top_k": k}, fabric_type="fused_dispatch",
+                            fabric_kwargs={"compact_route": True, "differentiable": differentiable, "supported_capacities": capacity}).cuda()
+    gather = GatherRouter(fabric_type="fused_combine", fabric_kwargs={"transform": weighted}).cuda()
+    rows, tags, loads, extra = to_torch_tensor(scatter(Annotator([0])(x), score), retrieve_attr=True)
+    return to_torch_tensor(gather(to_grid_tensor(rows * 0.75, tags, loads, extra), residual, score))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,kept", [("bf16", "f32"), ("f16", "f32"), ("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("k,weighted", [(1, False), (1, True), (2, True)])
+def test_a_residual_of_another_type(k, weighted, rows, kept):
+    """With or without gradients the result has the residual's type and shape, and the same bits; its gradients as the residual's."""
+    cells, paths, d = 70, 4, 16
+    x = normal(1, cells, d, dtype=TYPES[rows])
+    score = torch.softmax(normal(2, cells, paths), 1)
+    for shape in ((cells, d), (2, cells // 2, d)):
+        residual = normal(3, *shape, dtype=TYPES[kept])
+        want = routed_layer(False, k, weighted, 9, x, score, residual.clone())
+        leaves = [x.clone().requires_grad_(), residual.clone().requires_grad_()]
+        got = routed_layer(True, k, weighted, 9, leaves[0], score, leaves[1])
+        assert got.dtype == residual.dtype and got.shape == want.shape and torch.equal(got, want)
+        back = normal(4, *shape, dtype=TYPES[kept])
+        dx, dr = torch.autograd.grad(got, leaves, back)
+        bare = (want == residual).view(cells, d).all(1)
+        assert bool(bare.any()) and dx.dtype == x.dtype and dr.dtype == residual.dtype
+        assert torch.equal(dr.view(cells, d), torch.where(bare[:, None], back.view(cells, d), 0.0)) and not dx[bare].any() and bool(dx[~bare].any())
+
+
 def test_a_differentiable_fabric_needs_the_compact_route():
     from brt.router import ScatterRouter
 
