@@ -129,6 +129,12 @@ int data_type(const Tensor& t, const char* what) {
   return c;
 }
 Tensor dense(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
+bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+// ... and at an address that its rows can be read from in units of 16 bytes (a slice of a longer vector may start anywhere)
+Tensor dense_units(const Tensor& given) {
+  const Tensor t = dense(given);
+  return aligned16(t) ? t : t.clone();
+}
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 int32_t* iptr(const Tensor& t) { return static_cast<int32_t*>(ptr(t)); }
 float* fptr(const Tensor& t) { return static_cast<float*>(ptr(t)); }
@@ -703,8 +709,8 @@ struct DispatchByRows : Function<DispatchByRows> {
     const variable_list saved = ctx->get_saved_variables();
     return differentiable_once(5, grads, saved, [&](variable_list& made) {
       if (!grads[0].defined()) return;
-      const Tensor cells = saved[0].defined() ? dense(saved[0]) : Tensor(), weights = saved[1].defined() ? dense(saved[1]) : Tensor();
-      const Tensor seats = dense(saved[2]), grad = dense(grads[0]);
+      const Tensor cells = saved[0].defined() ? dense_units(saved[0]) : Tensor(), weights = saved[1].defined() ? dense(saved[1]) : Tensor();
+      const Tensor seats = dense(saved[2]), grad = dense_units(grads[0]);
       const c10::DeviceGuard guard(grad.device());
       const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
       const int64_t T = seats.size(0), k = seats.size(1), P = grad.size(0);
@@ -792,13 +798,13 @@ struct CombineByRows : Function<CombineByRows> {
     const variable_list saved = ctx->get_saved_variables();
     return differentiable_once(6, grads, saved, [&](variable_list& made) {
       if (!grads[0].defined()) return;
-      const Tensor rows = saved[0].defined() ? dense(saved[0]) : Tensor(), weights = saved[1].defined() ? dense(saved[1]) : Tensor();
+      const Tensor rows = saved[0].defined() ? dense_units(saved[0]) : Tensor(), weights = saved[1].defined() ? dense(saved[1]) : Tensor();
       const Tensor ids = dense(saved[2]), seats = dense(saved[3]), entries = dense(saved[4]);
       const c10::DeviceGuard guard(ids.device());
       const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
       const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
       // (fp32 rows with a 16-bit result: the kernel takes gradients of the rows' type, or fp32)
-      const Tensor grad = dense(grads[0].scalar_type() == type ? grads[0] : grads[0].to(at::kFloat));
+      const Tensor grad = dense_units(grads[0].scalar_type() == type ? grads[0] : grads[0].to(at::kFloat));
       const int64_t T = ids.size(0), k = ids.size(1), P = shape[0];
       int64_t cell = 1;
       for (size_t d = 1; d < shape.size(); ++d) cell *= shape[d];
@@ -978,7 +984,6 @@ PyObject* cast_f32_to_bf16(const Args& a) {
 // ---- products in 8 bits ------------------------------------------------------------------------------
 constexpr int64_t kScaleBlock = 128;
 int64_t blocks_of(int64_t n) { return (n + kScaleBlock - 1) / kScaleBlock; }
-bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
 // Whether the elements of two tensors span addresses in common.
 bool shares_memory(const Tensor& a, const Tensor& b) {
@@ -998,8 +1003,7 @@ struct Blocks {
 Blocks quantized(const Tensor& given, const char* name) {
   const int type = data_type(given, (std::string(name) + " data type").c_str());
   if (given.dim() != 2) runtime_error(std::string(name) + " must be [rows, elements]");
-  Tensor in = dense(given);
-  if (!aligned16(in)) in = in.clone();
+  const Tensor in = dense_units(given);
   const int64_t P = in.size(0), K = in.size(1), KB = blocks_of(K);
   if (P >= int64_t{1} << 31 || K >= int64_t{1} << 31) not_implemented("a dimension of 2^31 and more");
   Blocks b{empty({P, KB * kScaleBlock}, at::kByte, in), empty({KB, P}, at::kFloat, in)};
@@ -1066,14 +1070,12 @@ PyObject* grouped_linear_fp8(const Args& a) {
   if (in_blocks) {
     if (x_scales.scalar_type() != at::kFloat || x_scales.sizes() != at::IntArrayRef({P, KB})) runtime_error("x_scales must be fp32 [rows, blocks]");
     const bool in_place = P > 0 && (x.stride(1) == 1 || K == 1) && x.stride(0) >= K && x.stride(0) % 16 == 0 && x.stride(0) <= 1 << 20 && aligned16(x);
-    rows = in_place ? x : x.contiguous();
-    if (!aligned16(rows)) rows = rows.clone();
+    rows = in_place ? x : dense_units(x);
     pitch = in_place ? x.stride(0) : K;
     scales = x_scales.t().contiguous();
   } else if (brt_hip_grouped_gemm_fp8_quantizes(E, P, N)) {
     data_type(x, "x data type");
-    rows = dense(x), pitch = K;
-    if (!aligned16(rows)) rows = rows.clone();
+    rows = dense_units(x), pitch = K;
   } else {
     const Blocks b = quantized(x, "x");
     rows = b.q, scales = b.scales, pitch = b.q.size(1);

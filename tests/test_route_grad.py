@@ -570,6 +570,28 @@ def test_a_layer_of_routers_that_trains(k, weighted, capacity):
         torch.testing.assert_close(a.double(), b, rtol=1e-4, atol=1e-4)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32"), ("f32", "f16")])
+def test_gradients_at_any_address(dtype, out):
+    """What flattens the result behind a few other values hands back a slice that starts at any element: the same gradients."""
+    cells, paths, k, d = 37, 5, 2, 40
+    dtype, out = TYPES[dtype], TYPES[out]
+    ids, seat_rows, row_entries = make_route(cells, paths, k, 12, 1, keep=0.8)
+    x, w = normal(1, cells, d, dtype=dtype).requires_grad_(), normal(2, cells, k).requires_grad_()
+    y = normal(3, row_entries.numel(), d, dtype=dtype).requires_grad_()
+    scores = normal(4, cells, paths, dtype=dtype).requires_grad_()
+    for made, leaves in ((c_router.dispatch_by_rows(x, row_entries, k, w, seat_rows=seat_rows), [x, w]),
+                         (c_router.combine_by_rows(y, ids, seat_rows, w, out_dtype=out, row_entries=row_entries), [y, w]),
+                         (c_router.gate_topk(scores, k, True, differentiable=True)[1], [scores])):
+        grad = normal(5, made.numel(), dtype=made.dtype)
+        want = torch.autograd.grad(made, leaves, grad.view_as(made), retain_graph=True)
+        for before in (1, 3):
+            some = normal(6, before, dtype=made.dtype)
+            long = torch.cat([some, made.reshape(-1)])
+            got = torch.autograd.grad(long, leaves, torch.cat([some, grad]), retain_graph=True)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def routed_layer(differentiable, k, weighted, capacity, x, score, residual):
     """A scatter router, experts that scale their rows and a gather router with a residual."""
     from brt import Annotator, to_grid_tensor, to_torch_tensor
