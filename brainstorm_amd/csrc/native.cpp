@@ -157,7 +157,14 @@ at::DimVector rows_of(const Tensor& t, int64_t rows) {  // the shape of t with a
 
 // ---- gradients ---------------------------------------------------------------------------------------
 std::optional<Tensor> optional(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
-bool tracked(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
+// Whether a differentiable op records a backward pass for this operand.  The ops have no forward-mode gradients: a dual tensor's tangent is
+// refused where it would be lost.
+bool tracked(const Tensor& t) {
+  if (!t.defined()) return false;
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined())
+    not_implemented("forward-mode gradients of the routing ops are not implemented");
+  return t.requires_grad() && at::GradMode::is_enabled();
+}
 
 // The gradients of a backward pass for its `n` arguments, filled in by `fill` (what stays undefined has none).  The kernels
 // behind them have no gradients of their own: where a graph of the backward pass is asked for, differentiating it towards
@@ -735,7 +742,8 @@ PyObject* dispatch_by_rows(const Args& a) {  // in_data, row_entries, k, weights
   if (out.defined()) runtime_error("a differentiable dispatch makes its own result: seat_rows or out, not both");
   if (seats.dim() != 2 || seats.size(0) != in.size(0) || seats.size(1) != k) runtime_error("seat_rows must be [cells, k]");
   if (k > 8) not_implemented("more than 8 paths per cell");
-  return wrap(tracked(in) || tracked(weights) ? DispatchByRows::apply(in, optional(weights), entries, seats, k) : rows_of_cells(in, entries, k, weights, Tensor()));
+  const bool by_cells = tracked(in), by_weights = tracked(weights);
+  return wrap(by_cells || by_weights ? DispatchByRows::apply(in, optional(weights), entries, seats, k) : rows_of_cells(in, entries, k, weights, Tensor()));
 }
 
 struct CombineOptions {
@@ -828,7 +836,8 @@ PyObject* combine_by_rows(const Args& a) {  // in_data, path_ids, seat_rows, wei
   if (weights.defined()) same_device(weights, in, "weights");
   if (o.residual.defined() || o.gates.defined()) runtime_error("a differentiable combine takes neither out_data nor gates beside row_entries");
   if (in.dim() < 1 || entries.numel() != in.size(0)) runtime_error("row_entries must have one entry for every row");
-  if (!tracked(in) && !tracked(weights)) return wrap(cells_of_rows(in, ids, seats, weights, o));
+  const bool by_rows = tracked(in), by_weights = tracked(weights);
+  if (!by_rows && !by_weights) return wrap(cells_of_rows(in, ids, seats, weights, o));
   return wrap(CombineByRows::apply(in, optional(weights), ids, seats, entries, o.typed ? o.out_type : in.scalar_type()));
 }
 

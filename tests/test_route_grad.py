@@ -415,6 +415,36 @@ def test_gradients_of_gradients_are_refused():
 
 
 @pytest.mark.gpu
+def test_forward_mode_gradients_are_refused():
+    """A tangent is never dropped without an error; tensors without one go through, and duals through ops that are cut off anyway."""
+    import torch.autograd.forward_ad as forward
+
+    cells, k, d = 20, 2, 16
+    ids, seat_rows, row_entries = make_route(cells, 4, k, 20, 1)
+    x, w, scores = normal(1, cells, d), normal(2, cells, k), normal(3, cells, 4)
+    y, gates = normal(4, row_entries.numel(), d), normal(5, cells, 4)
+    calls = [
+        (lambda t: c_router.gate_topk(t, k, True, differentiable=True)[1], scores),
+        (lambda t: c_router.gate_topk(t, k, differentiable=True)[1], scores),
+        (lambda t: c_router.dispatch_by_rows(t, row_entries, k, w, seat_rows=seat_rows), x),
+        (lambda t: c_router.dispatch_by_rows(x, row_entries, k, t, seat_rows=seat_rows), w),
+        (lambda t: c_router.combine_by_rows(t, ids, seat_rows, w, row_entries=row_entries), y),
+        (lambda t: c_router.combine_by_rows(y, ids, seat_rows, t, row_entries=row_entries), w),
+        (lambda t: c_router.combine_by_rows(y, ids, seat_rows, gates=t, row_entries=row_entries), gates),
+    ]
+    for call, given in calls:
+        want = call(given)
+        with forward.dual_level():
+            dual = forward.make_dual(given, torch.ones_like(given))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(dual)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(forward.make_dual(given.clone().requires_grad_(), torch.ones_like(given)))
+            assert torch.equal(call(forward.unpack_dual(dual).primal), want) and torch.equal(call(given), want)
+            assert torch.equal(c_router.gate_topk(forward.make_dual(scores, scores), k, True)[1], c_router.gate_topk(scores, k, True)[1])
+
+
+@pytest.mark.gpu
 def test_refusals_of_the_differentiable_forms():
     cells, k, d = 20, 2, 16
     ids, seat_rows, row_entries = make_route(cells, 4, k, 20, 1)
