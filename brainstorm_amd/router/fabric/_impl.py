@@ -524,6 +524,9 @@ class FusedDispatchFabric(DispatchFabric):
             if getattr(self, "differentiable", False):
                 raise NotImplementedError("a differentiable dispatch takes one flow of cells of whole, aligned 16-byte units")
             hot_mask = hot_mask.dense()  # a shape this path does not take: the mask, as the reference
+        elif getattr(self, "differentiable", False) and torch.is_grad_enabled():
+            # a dense route carries no gradients, neither here nor through the combine
+            raise NotImplementedError("a differentiable dispatch takes the decision of a topk protocol for a device score of up to 1024 paths")
         if not self._in_one_step(in_flows, runtime_capacities, hot_mask):
             return super().forward(in_flow, hot_mask, runtime_capacities, score, route)
         # static rows, one flow, single-path route: index generation moves the rows itself

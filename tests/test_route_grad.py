@@ -660,3 +660,30 @@ def test_a_differentiable_fabric_needs_the_compact_route():
 
     with pytest.raises(ValueError, match="compact_route"):
         ScatterRouter(protocol_type="topk", fabric_type="fused_dispatch", fabric_kwargs={"differentiable": True})
+
+
+def test_a_differentiable_fabric_refuses_a_mask():
+    """Only the decision of a top-k protocol carries gradients; a mask would cut them off without a word."""
+    from brt import Annotator
+    from brt.router import ScatterRouter
+
+    kwargs = {"fabric_type": "fused_dispatch", "fabric_kwargs": {"compact_route": True, "differentiable": True}}
+    x = Annotator([0])(torch.ones(4, 8, requires_grad=True))
+    for protocol in ({"protocol_type": "switch_top1", "protocol_kwargs": {"one_hot": True}}, {"protocol_type": "topk"}):
+        with pytest.raises(NotImplementedError, match="topk protocol"):
+            ScatterRouter(**protocol, **kwargs)(x, torch.eye(4))  # (a score on the host: the protocol gives a mask)
+
+
+@pytest.mark.gpu
+def test_a_mask_goes_through_where_no_gradient_is_wanted():
+    from brt import Annotator, to_torch_tensor
+    from brt.router import ScatterRouter
+
+    x, mask = normal(1, 6, 8), torch.eye(6, 3, device="cuda")
+    made = []
+    with torch.no_grad():
+        for differentiable in (False, True):
+            scatter = ScatterRouter(protocol_type="switch_top1", fabric_type="fused_dispatch",
+                                    fabric_kwargs={"compact_route": True, "differentiable": differentiable}).cuda()
+            made.append(to_torch_tensor(scatter(Annotator([0])(x), mask)))
+    assert torch.equal(*made)
