@@ -598,9 +598,13 @@ class FusedCombineFabric(CombineFabric):
             gates = score if self.transform else None
             if isinstance(route, c_router.CompactRoute) and route.owns(route_indices, loads):
                 out = self._combine_compact(data, route, state, gates, residual)
-            elif route is not None and route.is_tag_index and route.owns(route_indices, loads):
+            elif isinstance(route, c_router.Route) and route.is_tag_index and route.owns(route_indices, loads):
                 out = self._combine_deferred(data, route, state, gates, residual)
             else:
+                lost = route if route is not None else c_router.route_of_loads(loads)
+                if getattr(lost, "differentiable", False) and torch.is_grad_enabled():
+                    raise RuntimeError("the rows of a differentiable dispatch come without their route: the combine would cut off their "
+                                       "gradients (the extra attributes, indices and loads of the routed flow go with the expert's rows)")
                 (out,) = c_router.combine_with_indices_and_loads(
                     data, route_indices, loads, gates, residual,
                     max_path_padding=self.max_path_padding, ever_padded=self.ever_padded, route=route)

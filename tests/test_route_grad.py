@@ -687,3 +687,33 @@ def test_a_mask_goes_through_where_no_gradient_is_wanted():
                                     fabric_kwargs={"compact_route": True, "differentiable": differentiable}).cuda()
             made.append(to_torch_tensor(scatter(Annotator([0])(x), mask)))
     assert torch.equal(*made)
+
+
+@pytest.mark.gpu
+def test_rows_without_their_route_are_refused():
+    """An expert that drops the extra attributes, or names other loads: the combine would cut the gradients off."""
+    from brt import Annotator, to_grid_tensor, to_torch_tensor
+    from brt.router import GatherRouter, ScatterRouter
+
+    x, score = normal(1, 12, 8).requires_grad_(), torch.softmax(normal(2, 12, 3), 1)
+    scatter = ScatterRouter(protocol_type="topk", fabric_type="fused_dispatch",
+                            fabric_kwargs={"compact_route": True, "differentiable": True}).cuda()
+    gather = GatherRouter(fabric_type="fused_combine").cuda()
+
+    def rows():
+        return to_torch_tensor(scatter(Annotator([0])(x), score), retrieve_attr=True)
+
+    data, tags, loads, extra = rows()
+    with pytest.raises(RuntimeError, match="without their route"):
+        gather(to_grid_tensor(data, tags, loads, None))
+    data, tags, loads, extra = rows()
+    with pytest.raises(RuntimeError, match="without their route"):
+        gather(to_grid_tensor(data, tags, loads[:-1] + [loads[-1].clone()], extra))
+    with torch.no_grad():
+        data, tags, loads, extra = rows()
+        assert torch.equal(to_torch_tensor(gather(to_grid_tensor(data, tags, loads, None))), x)
+        data, tags, loads, extra = rows()
+        assert torch.equal(to_torch_tensor(gather(to_grid_tensor(data, tags, loads[:-1] + [loads[-1].clone()], extra))), x)
+    data, tags, loads, extra = rows()
+    (dx,) = torch.autograd.grad(to_torch_tensor(gather(to_grid_tensor(data, tags, loads, extra))).sum(), x)
+    assert torch.equal(dx, torch.ones_like(x))
