@@ -155,6 +155,12 @@ at::DimVector rows_of(const Tensor& t, int64_t rows) {  // the shape of t with a
   return s;
 }
 
+int64_t row_elements(const Tensor& t) {  // also of a tensor without rows
+  int64_t n = 1;
+  for (int64_t d = 1; d < t.dim(); ++d) n *= t.size(d);
+  return n;
+}
+
 // ---- gradients ---------------------------------------------------------------------------------------
 std::optional<Tensor> optional(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 // Whether a differentiable op records a backward pass for this operand.  The ops have no forward-mode gradients: a dual tensor's tangent is
@@ -685,7 +691,7 @@ Tensor rows_of_cells(const Tensor& given, const Tensor& entries_given, int64_t k
   int32(entries_given, "row_entries");
   const int type = data_type(given, "in_data data type");
   const Tensor in = dense(given), entries = dense(entries_given);
-  const int64_t T = in.size(0), cell = T > 0 ? in.numel() / T : 0, P = entries.numel();
+  const int64_t T = in.size(0), cell = row_elements(in), P = entries.numel();
   const Tensor weights = entry_weights(weights_given, T * k);
   const c10::DeviceGuard guard(in.device());
   if (!out.defined()) out = empty(rows_of(in, P), in.scalar_type(), in);
@@ -763,7 +769,7 @@ Tensor cells_of_rows(const Tensor& given, const Tensor& ids_given, const Tensor&
     runtime_error("path_ids and seat_rows must both be [cells, k]");
   const Tensor in = dense(given), ids = dense(ids_given), seats = dense(seats_given);
   const int64_t T = ids.size(0), k = ids.size(1), P = in.size(0);
-  const int64_t cell = P > 0 ? in.numel() / P : residual.defined() && T > 0 ? residual.numel() / T : 0;
+  const int64_t cell = P == 0 && T > 0 && residual.defined() ? residual.numel() / T : row_elements(in);
   const Tensor weights = entry_weights(weights_given, T * k);
   const c10::DeviceGuard guard(in.device());
   Tensor out = residual;

@@ -501,6 +501,38 @@ def test_no_cells_and_no_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_results_of_no_cells_and_of_no_rows_are_zeros(dtype):
+    """Rows of a dispatch without cells, cells of a combine without rows; memory that held something else before."""
+    d, dtype = 24, TYPES[dtype]
+    none = torch.zeros(0, 2, dtype=torch.int32, device="cuda")
+
+    def used(rows, kind):
+        torch.full((rows, d), 7.0, dtype=kind, device="cuda")  # (what the allocator hands out next)
+
+    for seat_rows in (None, none):
+        x = torch.zeros(0, d, dtype=dtype, device="cuda", requires_grad=True)
+        used(3, dtype)
+        rows = c_router.dispatch_by_rows(x, torch.zeros(3, dtype=torch.int32, device="cuda"), 2, seat_rows=seat_rows)
+        assert rows.shape == (3, d) and not rows.any()
+    ids = torch.tensor([[0, 1], [1, 2], [-1, 0], [2, 1], [0, 2]], dtype=torch.int32, device="cuda")
+    bare, nothing = torch.zeros(5, 2, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda")
+    gates, w = normal(1, 5, 3).requires_grad_(), normal(2, 5, 2).requires_grad_()
+    y = torch.zeros(0, d, dtype=dtype, device="cuda", requires_grad=True)
+    for entries in (None, nothing):
+        for kind in {dtype, torch.float32}:
+            for operand in ({}, {"weights": w}, {"gates": gates}):
+                used(5, kind)
+                out = c_router.combine_by_rows(y, ids, bare, out_dtype=kind, row_entries=entries, **operand)
+                assert out.shape == (5, d) and out.dtype == kind and not out.any()
+                if entries is not None:
+                    found = torch.autograd.grad(out, [y] + list(operand.values()), torch.ones_like(out))
+                    assert found[0].shape == y.shape and not any(g.any() for g in found)
+    kept = torch.full((5, d), 7.0, dtype=dtype, device="cuda")
+    assert bool((c_router.combine_by_rows(y.detach(), ids, bare, None, kept) == 7.0).all())
+
+
+@pytest.mark.gpu
 def test_a_training_step_of_all_three_on_a_stream_and_replayed():
     """Gate, route, sort and back with identity experts: against autograd over plain torch in 64 bits, on a stream of its own,
     and captured once and replayed for other inputs."""
