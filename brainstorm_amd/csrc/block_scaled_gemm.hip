@@ -409,7 +409,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
   const int run = gridDim.x / kXcds, per = kPatchRows * a.tiles_n;
   // Where a last round has work for half of the workgroups at most, its tiles are dealt out by the halves of their rows: those have
   // one wavefront of each SIMD at work (the second halves of tiles that have none are left out; nothing follows them).
-  constexpr bool kHalves = WAVES == 8 && WM * WN / 2 == 4;
+  constexpr bool kHalves = WAVES == 8;
   const long real = static_cast<long>(blocks) * a.tiles_n, whole = kHalves && real % gridDim.x * 2 <= gridDim.x ? real / gridDim.x * gridDim.x : real;
   const long tiles = whole + 2 * (real - whole);
   long t = static_cast<long>(blockIdx.x % kXcds) * run + blockIdx.x / kXcds;
@@ -621,12 +621,11 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_tiles_kernel(Fp8Args a) {
 }
 
 // Few rows per expert: the weights are streamed once and set the time.  A workgroup takes 16 NT columns and 16 MT rows; its
-// W wavefronts take K-steps in turn (D of them in flight, weights straight into the fragments' registers) and add up their
-// sums through LDS.  Rows that are not 8-bit yet are quantized on the way in: the 32 elements that a lane holds of its row's
+// W wavefronts take K-steps in turn (weights straight into the fragments' registers) and add up their sums through LDS.  Rows that are not 8-bit yet are quantized on the way in: the 32 elements that a lane holds of its row's
 // block are exactly its fragment, so that costs two exchanges among the row's four lanes and no launch of its own.  One row of 2048 ->
 // 8192: 6.5 us (16.8 MB, 2.6 TB/s: a launch, the loads and one chain of requests); 48 rows of 8 experts 1024 -> 4096 with bias and
 // GELU 9.7 (33.9 MB, 3.5 TB/s).
-template <int XDT, int MT, int NT, int W, int D, bool EXACT>
+template <int XDT, int MT, int NT, int W, bool EXACT>
 __global__ __launch_bounds__(W * 64) void fp8_few_rows_kernel(Fp8Args a) {
   constexpr bool kQuantized = XDT < 0;
   constexpr int kBytes = kQuantized ? 1 : elem_bytes(XDT == BRT_F32 ? BRT_F32 : BRT_F16);
@@ -657,89 +656,77 @@ __global__ __launch_bounds__(W * 64) void fp8_few_rows_kernel(Fp8Args a) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  for (int kb0 = wave; kb0 < a.KB; kb0 += W * D) {
-    u32x4 wv[D][NT][2], xv[D][MT][kLoads];
-    float scale[D], given[D][MT];
+  for (int kb = wave; kb < a.KB; kb += W) {
+    u32x4 wv[NT][2], xv[MT][kLoads];
+    float given[MT];
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
-      const int kb = kb0 + d * W;
+    for (int h = 0; h < 2; ++h) {  // the lane's chunks of 16: g and g + 4
+      const bool there = kb * kB + h * 64 + g * 16 < a.K;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {  // the lane's chunks of 16: g and g + 4
-        const bool there = kb * kB + h * 64 + g * 16 < a.K;
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-          wv[d][j][h] = __builtin_amdgcn_raw_buffer_load_b128(rw, there ? (j * 16 + c16) * a.K + h * 64 + g * 16 : kNowhere, kb * kB, 0);
-      }
-      scale[d] = sw[min(kb, a.KB - 1)];
+      for (int j = 0; j < NT; ++j)
+        wv[j][h] = __builtin_amdgcn_raw_buffer_load_b128(rw, there ? (j * 16 + c16) * a.K + h * 64 + g * 16 : kNowhere, kb * kB, 0);
     }
+    const float scale = sw[kb];
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
-      const int kb = kb0 + d * W;
+    for (int i = 0; i < MT; ++i) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
+      for (int l = 0; l < kLoads; ++l) {
+        const int h = l / kBytes;
+        const bool there = kb * kB + h * 64 + g * 16 < a.K;
+        xv[i][l] = __builtin_amdgcn_raw_buffer_load_b128(
+            rx, there ? (i * 16 + c16) * pitch + (h * 64 + g * 16) * kBytes + (l % kBytes) * 16 : kNowhere, kb * kB * kBytes, 0);
+      }
+      if constexpr (kQuantized) given[i] = a.sx[static_cast<size_t>(kb) * a.P + at.row0 + min(i * 16 + c16, at.rows - 1)];
+    }
+    decltype(operand<EXACT>(i32x8{})) x[MT];
+    float s[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      i32x8 q;
+      if constexpr (kQuantized) {
+#pragma unroll
+        for (int l = 0; l < 2; ++l)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) q[4 * l + c] = static_cast<int>(xv[i][l][c]);
+        s[i] = given[i] * scale;
+      } else {
+        constexpr int NE = 16 / kBytes;
+        float v[32];
+        uint32_t top = 0;
 #pragma unroll
         for (int l = 0; l < kLoads; ++l) {
-          const int h = l / kBytes;
-          const bool there = kb * kB + h * 64 + g * 16 < a.K;
-          xv[d][i][l] = __builtin_amdgcn_raw_buffer_load_b128(
-              rx, there ? (i * 16 + c16) * pitch + (h * 64 + g * 16) * kBytes + (l % kBytes) * 16 : kNowhere, kb * kB * kBytes, 0);
+          float part[NE];
+          unpack<XDT, 16>(xv[i][l], part);
+#pragma unroll
+          for (int c = 0; c < NE; ++c) {
+            v[l * NE + c] = part[c];
+            top = max(top, magnitude(part[c]));
+          }
         }
-        if constexpr (kQuantized)
-          given[d][i] = a.sx[static_cast<size_t>(min(kb, a.KB - 1)) * a.P + at.row0 + min(i * 16 + c16, at.rows - 1)];
+        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, kWave)));
+        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, kWave)));
+        float own, inverse;
+        scale_of(top, &own, &inverse);
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          q[c] = static_cast<int>(pack4(v[4 * c] * inverse, v[4 * c + 1] * inverse, v[4 * c + 2] * inverse, v[4 * c + 3] * inverse));
+        s[i] = own * scale;
       }
+      x[i] = operand<EXACT>(q);
     }
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
-      decltype(operand<EXACT>(i32x8{})) x[MT];
-      float s[MT];
+    for (int j = 0; j < NT; ++j) {
+      i32x8 v;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[4 * h + c] = static_cast<int>(wv[j][h][c]);
+      const auto w = operand<EXACT>(v);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        i32x8 q;
-        if constexpr (kQuantized) {
+        const f32x4 part = multiply(w, x[i]);
 #pragma unroll
-          for (int l = 0; l < 2; ++l)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) q[4 * l + c] = static_cast<int>(xv[d][i][l][c]);
-          s[i] = given[d][i] * scale[d];
-        } else {
-          constexpr int NE = 16 / kBytes;
-          float v[32];
-          uint32_t top = 0;
-#pragma unroll
-          for (int l = 0; l < kLoads; ++l) {
-            float part[NE];
-            unpack<XDT, 16>(xv[d][i][l], part);
-#pragma unroll
-            for (int c = 0; c < NE; ++c) {
-              v[l * NE + c] = part[c];
-              top = max(top, magnitude(part[c]));
-            }
-          }
-          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, kWave)));
-          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, kWave)));
-          float own, inverse;
-          scale_of(top, &own, &inverse);
-#pragma unroll
-          for (int c = 0; c < 8; ++c)
-            q[c] = static_cast<int>(pack4(v[4 * c] * inverse, v[4 * c + 1] * inverse, v[4 * c + 2] * inverse, v[4 * c + 3] * inverse));
-          s[i] = own * scale[d];
-        }
-        x[i] = operand<EXACT>(q);
-      }
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        i32x8 v;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) v[4 * h + c] = static_cast<int>(wv[d][j][h][c]);
-        const auto w = operand<EXACT>(v);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const f32x4 part = multiply(w, x[i]);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) acc[i][j][q] = __builtin_fmaf(part[q], s[i], acc[i][j][q]);
-        }
+        for (int q = 0; q < 4; ++q) acc[i][j][q] = __builtin_fmaf(part[q], s[i], acc[i][j][q]);
       }
     }
   }
@@ -765,29 +752,29 @@ __global__ __launch_bounds__(W * 64) void fp8_few_rows_kernel(Fp8Args a) {
   }
 }
 
-template <int XDT, int MT, int NT, int W, int D, bool EXACT>
+template <int XDT, int MT, int NT, int W, bool EXACT>
 int launch_few_rows(Fp8Args& a, hipStream_t st) {
   constexpr int kRows = 16 * MT;
   const long blocks = static_cast<long>(a.P) / kRows + std::min(a.E, a.P);
   a.tiles_n = (a.N + 16 * NT - 1) / (16 * NT);
   if (blocks * a.tiles_n >= (1l << 31)) return fail(BRT_E_UNSUPPORTED, "too many tiles");
-  hipLaunchKernelGGL((fp8_few_rows_kernel<XDT, MT, NT, W, D, EXACT>), dim3(static_cast<unsigned>(blocks * a.tiles_n)), dim3(W * 64), 0, st, a);
+  hipLaunchKernelGGL((fp8_few_rows_kernel<XDT, MT, NT, W, EXACT>), dim3(static_cast<unsigned>(blocks * a.tiles_n)), dim3(W * 64), 0, st, a);
   return check_launch("fp8_few_rows_kernel");
 }
-// Rows and columns of a workgroup, wavefronts that share K, K-steps in flight.  `tiles` of 16 columns is what there is to deal
+// Rows and columns of a workgroup, wavefronts that share K.  `tiles` of 16 columns is what there is to deal
 // out (the loads are on the device: every expert is taken to have rows where there are as many rows).  Few of them: as many
 // wavefronts as possible on each; many: more columns to a wavefront, which quantizes the rows once for all of them.
 template <int XDT, bool EXACT>
 int launch_few_rows(Fp8Args& a, hipStream_t st) {
   const long tiles = static_cast<long>(std::min(a.E, a.P)) * ((a.N + 15) / 16);
   if (a.P > 16 && a.P > 10l * a.E) {
-    if (tiles < 1024) return launch_few_rows<XDT, 2, 2, 8, 1, EXACT>(a, st);
-    return launch_few_rows<XDT, 2, 4, 4, 1, EXACT>(a, st);
+    if (tiles < 1024) return launch_few_rows<XDT, 2, 2, 8, EXACT>(a, st);
+    return launch_few_rows<XDT, 2, 4, 4, EXACT>(a, st);
   }
-  if (tiles < 512) return launch_few_rows<XDT, 1, 1, 16, 1, EXACT>(a, st);
-  if (tiles < 1536) return launch_few_rows<XDT, 1, 2, 8, 1, EXACT>(a, st);
-  if (tiles < 4096) return launch_few_rows<XDT, 1, 4, 8, 1, EXACT>(a, st);
-  return launch_few_rows<XDT, 1, 4, 4, 1, EXACT>(a, st);
+  if (tiles < 512) return launch_few_rows<XDT, 1, 1, 16, EXACT>(a, st);
+  if (tiles < 1536) return launch_few_rows<XDT, 1, 2, 8, EXACT>(a, st);
+  if (tiles < 4096) return launch_few_rows<XDT, 1, 4, 8, EXACT>(a, st);
+  return launch_few_rows<XDT, 1, 4, 4, EXACT>(a, st);
 }
 template <int XDT>
 int launch_few_rows(Fp8Args& a, hipStream_t st) {
