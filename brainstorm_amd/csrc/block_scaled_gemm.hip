@@ -29,6 +29,7 @@ constexpr float kLeast = 0x1p-100f;  // blocks whose largest value is below this
 constexpr int kXcds = 8, kCusPerXcd = 32;
 constexpr int kPatchRows = 4;
 constexpr int kMostRows = 1 << 24;   // 65 times as many are added up in 32 bits
+constexpr int kMostColumns = 1 << 30;  // and experts: rounded up to tiles they are counted in 32 bits
 constexpr int kMostExperts = 512;  // whose row blocks a workgroup keeps in LDS
 constexpr uint32_t kNowhere = 0x7ffffff0u;  // an offset past every extent: reads as zero, costs no request
 
@@ -862,13 +863,13 @@ int launch_any_tiles(Fp8Args& a, hipStream_t st) {
 using namespace brt;
 
 extern "C" int brt_hip_quantize_rows(const void* x, int P, int K, int dtype, void* q, int pitch, float* scales, void* stream) {
-  if (P < 0 || K < 0 || pitch < (K + kB - 1) / kB * kB) return fail(BRT_E_INVALID, "bad shape P=%d K=%d pitch=%d", P, K, pitch);
+  if (P < 0 || K < 0 || pitch < (K + kB - 1l) / kB * kB) return fail(BRT_E_INVALID, "bad shape P=%d K=%d pitch=%d", P, K, pitch);
   if (dtype != BRT_F32 && dtype != BRT_F16 && dtype != BRT_BF16) return fail(BRT_E_UNSUPPORTED, "dtype %d is not supported", dtype);
   if (P == 0 || K == 0) return BRT_OK;
   if (!x || !q || !scales) return fail(BRT_E_INVALID, "null argument");
   if (K % 16 != 0 || pitch % 16 != 0 || !aligned(x, 16) || !aligned(q, 16))
     return fail(BRT_E_UNSUPPORTED, "rows must be whole, aligned units of 16 elements (K=%d)", K);
-  const int KB = (K + kB - 1) / kB;
+  const int KB = static_cast<int>((K + kB - 1l) / kB);
   const long waves = (static_cast<long>(P) + 7) / 8 * KB;
   if (waves >= (1l << 31)) return fail(BRT_E_UNSUPPORTED, "too many blocks");
   const dim3 grid(static_cast<unsigned>((waves + 3) / 4)), block(256);
@@ -906,6 +907,7 @@ extern "C" int brt_hip_grouped_gemm_fp8(const void* x, int x_dtype, int pitch, c
   if (K % 16 != 0 || pitch % 16 != 0 || !aligned(x, 16) || !aligned(w, 16))
     return fail(BRT_E_UNSUPPORTED, "rows must be whole, aligned units of 16 elements (K=%d)", K);
   if (P >= kMostRows) return fail(BRT_E_UNSUPPORTED, "more than %d rows", kMostRows - 1);
+  if (E > kMostColumns || N > kMostColumns) return fail(BRT_E_UNSUPPORTED, "more than %d columns or experts", kMostColumns);
   if (pitch > (1 << 20)) return fail(BRT_E_UNSUPPORTED, "rows of more than 1 Mi elements");  // (256 of them are addressed by 31 bits)
   if (out_scales && (!quantizes_result(E, P, N, K, out_dtype) || !aligned(out, 16)))
     return fail(BRT_E_UNSUPPORTED, "results of this shape are not quantized by the product's kernel");

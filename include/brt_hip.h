@@ -521,7 +521,7 @@ int brt_hip_combine_by_rows_grad(const void* grad, const void* rows, const float
  *   With out_scales, where brt_hip_grouped_gemm_fp8_blocks(E, P, N, K, out_dtype) is 1, the result is rounded to out_dtype and
  *   quantized as brt_hip_quantize_rows would quantize it: out is e4m3 [P,ceil(N/128)*128], out_scales [ceil(N/128),P].
  *
- * K is a multiple of 16, and x, q and w are 16-byte aligned; N is any number, P below 2^24.  Loads below zero count as none, rows
+ * K is a multiple of 16, and x, q and w are 16-byte aligned; N is any number up to 2^30, P below 2^24.  Loads below zero count as none, rows
  * of experts behind the P-th do not exist.  The first call of a shape on a device has to happen outside graph capture.
  */
 int brt_hip_quantize_rows(const void* x, int P, int K, int dtype, void* q, int pitch, float* scales, void* stream);

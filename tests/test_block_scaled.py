@@ -460,6 +460,18 @@ def test_arguments_are_checked_before_anything_runs():
     assert back(None, None, None, None, None, None, 16, None, 4, 1, 8, 4, 0, 0, None) == -1
 
 
+def test_dimensions_that_do_not_fit_in_32_bits_once_rounded_up():
+    from brainstorm_amd import _lib
+
+    lib = _lib.lib()
+    last = 2 ** 31 - 16
+    assert lib.brt_hip_quantize_rows(None, 1, last, 0, None, last, None, None) == -1 and b"pitch" in lib.brt_hip_last_error()
+    call = lambda E, N: lib.brt_hip_grouped_gemm_fp8(  # noqa: E731
+        16, 0, 128, 16, 16, 16, 16, None, 0, 16, 0, None, E, 4, N, 128, 0, 0, None)
+    assert call(2, 2 ** 31 - 1) == -4 and b"columns" in lib.brt_hip_last_error()
+    assert call(2 ** 31 - 1, 128) == -4 and b"columns" in lib.brt_hip_last_error()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("cells", [1, 17, 300, 3000])
 def test_a_served_layer_of_all_operators(cells):
