@@ -36,8 +36,8 @@ struct GateGradArgs {
 
 // A row is held by 1 << ls lanes, STEPS units of V columns each (one 16-byte unit where the rows are whole units, one column
 // otherwise): 16-bit scores of 128 paths take 16 lanes, so that a wavefront has four rows in flight and its reductions stay
-// on the DPP network.  Bound by the issue of the exponentials and the masks as much as by memory: 65536 x 128 bf16 11.6 us, 33.6 MB
-// at 2.9 TB/s.
+// on the DPP network.  Bound by the issue of the exponentials and the masks: 65536 x 128 bf16 11.6 us (33.6 MB, 2.9 TB/s), of which its 5.67 M
+// vector instructions at four clocks on 1024 SIMDs of 2.4 GHz are 9.2.
 template <int DT, int V, int STEPS>
 __global__ __launch_bounds__(kBlock) void gate_grad_kernel(GateGradArgs a) {
   using namespace std;
