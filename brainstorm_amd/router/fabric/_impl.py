@@ -626,10 +626,14 @@ class FusedCombineFabric(CombineFabric):
         if route.differentiable:
             if gates is not None and (gates.dim() != 2 or gates.size(1) < route.paths):
                 raise RuntimeError(f"the score does not have a column for each of {route.paths} paths")
+            kind = data.dtype if residual is None else residual.dtype
+            # (a floating-point type that the combine does not write for these rows is rounded to from fp32)
+            direct = kind in (data.dtype, torch.float32) or data.dtype == torch.float32 and kind in (torch.float16, torch.bfloat16)
             out = c_router.combine_by_rows(data, route.path_ids, route.seat_rows, gates=gates, row_entries=route.row_entries,
-                                           out_dtype=None if residual is None else residual.dtype)
+                                           out_dtype=kind if direct or not kind.is_floating_point else torch.float32)
             if residual is None:
                 return out
+            out = out.to(kind)
             # the residual's type and shape, as when it is written in place
             if residual.numel() != out.numel():
                 raise RuntimeError("the residual does not have the elements of the cells")

@@ -687,6 +687,35 @@ def test_a_residual_of_another_type(k, weighted, rows, kept):
         assert torch.equal(dr.view(cells, d), torch.where(bare[:, None], back.view(cells, d), 0.0)) and not dx[bare].any() and bool(dx[~bare].any())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,kept", [("bf16", torch.float16), ("f16", torch.bfloat16), ("f32", torch.float64), ("bf16", torch.float64)])
+def test_a_residual_of_a_type_that_the_combine_does_not_write(rows, kept):
+    """The sum in fp32, rounded to the residual's type once."""
+    cells, paths, d = 70, 4, 16
+    x, residual = normal(1, cells, d, dtype=TYPES[rows]).requires_grad_(), normal(3, cells, d).to(kept).requires_grad_()
+    score = torch.softmax(normal(2, cells, paths), 1)
+    wide = routed_layer(True, 2, True, 9, x, score, residual.detach().float())
+    got = routed_layer(True, 2, True, 9, x, score, residual)
+    bare = (wide == residual.detach().float()).all(1, keepdim=True)
+    assert got.dtype == kept and torch.equal(got, torch.where(bare, residual, wide.to(kept)))
+    dx, dr = torch.autograd.grad(got.double().sum(), [x, residual])
+    assert not dx[bare[:, 0]].any() and bool(dx[~bare[:, 0]].any()) and torch.equal(dr, bare.to(kept).expand(cells, d))
+    with pytest.raises(NotImplementedError):
+        routed_layer(True, 2, True, 9, x, score, torch.zeros(cells, d, dtype=torch.int64, device="cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("differentiable", [False, True])
+def test_a_residual_that_is_a_flow(differentiable):
+    from brt import Annotator, to_torch_tensor
+
+    cells, d = 70, 16
+    x, score, residual = normal(1, cells, d), torch.softmax(normal(2, cells, 4), 1), normal(3, cells, d)
+    want = routed_layer(False, 2, True, 9, x, score, residual.clone())
+    got = routed_layer(differentiable, 2, True, 9, x, score, Annotator([0])(residual.clone()))
+    assert torch.equal(to_torch_tensor(got), want)
+
+
 def test_a_differentiable_fabric_needs_the_compact_route():
     from brt.router import ScatterRouter
 
