@@ -506,8 +506,8 @@ int brt_hip_combine_by_rows_grad(const void* grad, const void* rows, const float
  *
  * brt_hip_quantize_rows: rows [P,K] (dtype) -> q [P,pitch] and scales [KB,P], KB = ceil(K / 128): of every 128 elements of a
  *   row, top = max(|x|, 2^-100), scale = top / 448 and q = e4m3(x * (1 / top * 448)), each operation rounded in fp32.  Elements of
- *   q from K to the next multiple of 128 are zeroed; pitch is at least that.  A block that holds NaN or an infinity has a scale
- *   of NaN or infinity, and products with its row are NaN, behind an activation too.
+ *   q from K to the next multiple of 128 are zeroed (NaN where the block holds NaN); pitch is at least that.  A block that holds
+ *   NaN or an infinity has a scale of NaN or infinity, and products with its row are NaN, behind an activation too.
  *
  * brt_hip_grouped_gemm_fp8: for the rows r of expert e (packed by expert, rows behind the last one's are not written)
  *     out[r,n] = act(sum_kb x_scales[kb,r] * w_scales[e,n/128,kb] * (sum over block kb of x[r,k] * w[e,n,k]) + bias[e,n]),
