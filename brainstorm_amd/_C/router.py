@@ -680,6 +680,21 @@ def gate_topk(score: torch.Tensor, top_k: int, softmax: bool = False,
     return _lib.native().gate_topk(score, top_k, softmax, hot_mask, differentiable)
 
 
+def balance_loss(score: torch.Tensor, path_ids: torch.Tensor, counted: Optional[torch.Tensor] = None
+                 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(balance, z, counts)``: the two losses that a router is trained with beside its task, and the entries per path.  With
+    ``p = softmax(score[t])`` over the ``n`` cells that count (``counted``, bool ``[cells]``; all of them without it: leave padding out),
+    ``counts[e]`` (int32, before any capacity) is how many of their entries in ``path_ids`` (``[cells, k]``, from
+    :func:`gate_topk`) name path ``e``, ``balance = paths / (n * n * k) * sum_e counts[e] * sum_t p[t, e]`` (one where all paths are
+    used evenly) and ``z = mean(logsumexp(score[t])**2)``, fp32 scalars.  Ids outside the paths name none; without cells or entries
+    that count a loss is zero.
+
+    The losses carry the gradient of ``score`` where gradients are recorded (counts have none), made in one launch; cells that do not
+    count have none, whatever they hold, and no gradients of these gradients.  A counted cell that holds NaN, or no score above -inf,
+    makes the losses NaN, as its softmax is.  At most 1024 paths."""
+    return _lib.native().balance_loss(score, path_ids, counted)
+
+
 def route_by_path(
     path_ids: torch.Tensor,
     path_num: int,

@@ -1,0 +1,391 @@
+// The losses that keep a router balanced, and their gradient (no counterpart in the reference, whose ops are not
+// differentiable).  Of scores s [T,E] and the paths chosen from them, over the n cells that count:
+//
+//   p = softmax(s[t])      lse = log(sum exp s[t])      counts[e] = entries that name path e
+//   balance = E / (n n k) * sum_e counts[e] * sum_t p[t,e]           z = 1/n * sum_t lse[t]^2
+//   ds[t,e] = p[t,e] * (c[e] - sum_i c[i] p[t,i] + q lse[t])         c = g_balance E / (n n k) counts,  q = g_z 2 / n
+//
+// A row is held by 1 << ls lanes, STEPS units of V columns each (one 16-byte unit where the rows are whole units, one column
+// otherwise), so every lane keeps its columns for all rows of its wavefront: the column sums stay in registers, go through LDS
+// once per workgroup and to memory as one vector of E per workgroup, which a second launch adds up (one launch, one workgroup, for
+// small batches).  No floating-point atomics: the order of every sum follows from the sizes.  Exponents are taken of s - max, so rows of the
+// type's lowest value have a softmax; a cell that does not count is read as zeros, whatever it holds.
+#include <algorithm>
+
+#include "gate.hpp"
+#include "rows.hpp"
+
+namespace brt {
+namespace {
+
+constexpr int kBlock = 512;
+constexpr int kWaves = kBlock / kWave;
+constexpr int kMostBlocks = 256;  // one per CU: the second launch reads 8 bytes per column of each
+constexpr int kMostPaths = 1024;
+constexpr float kLog2E = 1.44269504088896341f;
+
+struct BalanceArgs {
+  const void* scores;
+  const int* ids;
+  const uint8_t* counted;  // [T] or null
+  float* balance;
+  float* z;
+  int* counts;         // [E]
+  float* row_stats;    // [T, 2] max and sum of the exponentials, or null
+  float* coefficients; // [E + 1] c and q of unit gradients, or null
+  float* part_p;       // [blocks][E]
+  int* part_counts;    // [blocks][E]
+  float* part_z;       // [blocks]
+  int* part_n;         // [blocks]
+  int T, E, k, blocks;
+  int ls;  // log2 of the lanes that share a row
+};
+
+// exp(x) for x <= 0, within 2 + |x| steps of 2^-24: small exponents are exact to the last bits, where the large probabilities are
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2E); }
+
+// Column sums and what belongs to the batch -> the losses, the counts and the gradient's coefficients; by the whole workgroup.
+// column(e, &p, &count) gives the sums of a column.
+template <typename F>
+__device__ __forceinline__ void finish(const BalanceArgs& a, double z, long n, double* s_dot, F&& column) {
+  const double entries = static_cast<double>(n) * a.k;
+  const double scale = n > 0 && a.k > 0 ? a.E / (entries * n) : 0.0;
+  double dot = 0.0;
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+    double p;
+    int count;
+    column(e, &p, &count);
+    dot += p * count;
+    a.counts[e] = count;
+    if (a.coefficients != nullptr) a.coefficients[e] = static_cast<float>(scale * count);
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) dot += __shfl_xor(dot, d, kWave);
+  if (lane_id() == 0) s_dot[threadIdx.x >> 6] = dot;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double sum = 0.0;
+    for (int w = 0; w < static_cast<int>(blockDim.x) / kWave; ++w) sum += s_dot[w];
+    *a.balance = static_cast<float>(scale * sum);
+    *a.z = n > 0 ? static_cast<float>(z / n) : 0.0f;
+    if (a.coefficients != nullptr) a.coefficients[a.E] = n > 0 ? static_cast<float>(2.0 / n) : 0.0f;
+  }
+}
+
+template <int DT, int V, int STEPS, int ROWS>
+__global__ __launch_bounds__(kBlock) void balance_kernel(BalanceArgs a) {
+  __shared__ float s_p[kWaves][kMostPaths];
+  __shared__ int s_counts[kMostPaths];
+  __shared__ float s_z[kWaves];
+  __shared__ int s_n[kWaves];
+  __shared__ double s_dot[kWaves];
+  constexpr int kBytes = V * elem_bytes(DT);
+  using U = typename Unit<kBytes>::type;
+  const int lane = lane_id(), wave = threadIdx.x >> 6;
+  const int ls = a.ls, lpr = 1 << ls, glane = lane & (lpr - 1), per = kWave >> ls;  // rows of a wavefront side by side
+  const int units = a.E / V;
+  for (int e = threadIdx.x; e < a.E; e += kBlock) s_counts[e] = 0;
+  __syncthreads();
+  float acc[STEPS][V];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[s][v] = 0.0f;
+  float z = 0.0f;
+  int n = 0;
+  // the rows of a workgroup lie side by side; its wavefronts take them in turn, ROWS loads at a time
+  const long share = (static_cast<long>(a.T) + a.blocks - 1) / a.blocks;
+  const long first = share * blockIdx.x, last = min(first + share, static_cast<long>(a.T));
+  for (long r0 = first + wave * (per * ROWS); r0 < last; r0 += kWaves * per * ROWS) {
+    U raw[ROWS][STEPS];
+    bool use[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const long row = r0 + i * per + (lane >> ls), at = min(row, last - 1);
+      use[i] = row < last && (a.counted == nullptr || a.counted[at] != 0);
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) raw[i][s] = static_cast<const U*>(a.scores)[at * units + min(s * lpr + glane, units - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const long row = r0 + i * per + (lane >> ls);
+      float x[STEPS][V], top = -INFINITY;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        unpack<DT, kBytes>(use[i] ? raw[i][s] : zero_unit<kBytes>(), x[s]);
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (s * lpr + glane < units) top = fmaxf(top, x[s][v]);
+      }
+      top = segment_max(top, lpr);
+      float sum = 0.0f;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          x[s][v] = exp_of(x[s][v] - top);
+          if (s * lpr + glane < units) sum += x[s][v];
+        }
+      sum = segment_sum(sum, lpr);
+      const float inverse = use[i] ? 1.0f / sum : 0.0f;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[s][v] = __builtin_fmaf(x[s][v], inverse, acc[s][v]);
+      if (glane == 0 && row < last) {
+        if (use[i]) {
+          const float lse = top + logf(sum);
+          z += lse * lse;
+          ++n;
+        }
+        if (a.row_stats != nullptr) *reinterpret_cast<f32x2*>(a.row_stats + 2 * row) = f32x2{top, sum};
+      }
+    }
+  }
+  // entries of the workgroup's rows, by path (whole numbers: their order does not matter)
+  for (long i = first * a.k + threadIdx.x; i < last * a.k; i += kBlock) {
+    const int id = a.ids[i];
+    if (id >= 0 && id < a.E && (a.counted == nullptr || a.counted[static_cast<uint32_t>(i) / a.k] != 0)) atomicAdd(&s_counts[id], 1);
+  }
+  for (int d = lpr; d < kWave; d <<= 1) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[s][v] += __shfl_xor(acc[s][v], d, kWave);
+  }
+  if (lane < lpr) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (s * lpr + lane < units) s_p[wave][(s * lpr + lane) * V + v] = acc[s][v];
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) z += __shfl_xor(z, d, kWave), n += __shfl_xor(n, d, kWave);
+  if (lane == 0) s_z[wave] = z, s_n[wave] = n;
+  __syncthreads();
+  float block_z = 0.0f;
+  int block_n = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) block_z += s_z[w], block_n += s_n[w];
+  auto column = [&](int e, auto* p, int* count) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) sum += s_p[w][e];
+    *p = sum, *count = s_counts[e];
+  };
+  if (a.blocks == 1) return finish(a, block_z, block_n, s_dot, column);
+  for (int e = threadIdx.x; e < a.E; e += kBlock) {
+    const size_t at = static_cast<size_t>(blockIdx.x) * a.E + e;
+    column(e, &a.part_p[at], &a.part_counts[at]);
+  }
+  if (threadIdx.x == 0) a.part_z[blockIdx.x] = block_z, a.part_n[blockIdx.x] = block_n;
+}
+
+// The workgroups' sums added up: a thread takes a column of every `slices`-th of them.
+constexpr int kJoin = 1024;
+__global__ __launch_bounds__(kJoin) void balance_join_kernel(BalanceArgs a, int slices) {
+  __shared__ double s_p[kJoin];
+  __shared__ int s_counts[kJoin];
+  __shared__ double s_dot[kJoin / kWave], s_z[kJoin / kWave];
+  __shared__ int s_n[kJoin / kWave];
+  const int width = kJoin / slices, slice = threadIdx.x / width, e = threadIdx.x % width;
+  double p = 0.0;
+  int count = 0;
+  if (e < a.E) {
+#pragma unroll 8
+    for (int b = slice; b < a.blocks; b += slices) {
+      p += a.part_p[static_cast<size_t>(b) * a.E + e];
+      count += a.part_counts[static_cast<size_t>(b) * a.E + e];
+    }
+  }
+  s_p[threadIdx.x] = p, s_counts[threadIdx.x] = count;
+  double z = 0.0;
+  int n = 0;
+  for (int b = threadIdx.x; b < a.blocks; b += kJoin) z += a.part_z[b], n += a.part_n[b];
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) z += __shfl_xor(z, d, kWave), n += __shfl_xor(n, d, kWave);
+  if (lane_id() == 0) s_z[threadIdx.x >> 6] = z, s_n[threadIdx.x >> 6] = n;
+  __syncthreads();
+  z = 0.0, n = 0;
+  for (int w = 0; w < kJoin / kWave; ++w) z += s_z[w], n += s_n[w];
+  finish(a, z, n, s_dot, [&](int column, double* sum, int* total) {
+    *sum = 0.0, *total = 0;
+    for (int s = 0; s < slices; ++s) *sum += s_p[s * width + column], *total += s_counts[s * width + column];
+  });
+}
+
+struct BalanceGradArgs {
+  const void* scores;
+  const uint8_t* counted;
+  const float* row_stats;
+  const float* coefficients;
+  const float* grad_balance;  // one value each, or null
+  const float* grad_z;
+  void* out;
+  int T, E, ls, passes;  // passes: rows of a lane group, side by side with its neighbours'
+};
+
+template <int DT, int V, int STEPS, int ROWS>
+__global__ __launch_bounds__(256) void balance_grad_kernel(BalanceGradArgs a) {
+  constexpr int kBytes = V * elem_bytes(DT);
+  using U = typename Unit<kBytes>::type;
+  const int lane = lane_id(), ls = a.ls, lpr = 1 << ls, glane = lane & (lpr - 1), per = kWave >> ls, units = a.E / V;
+  const float by = a.grad_balance != nullptr ? *a.grad_balance : 0.0f;
+  const float q = a.grad_z != nullptr ? *a.grad_z * a.coefficients[a.E] : 0.0f;
+  float c[STEPS][V];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int e = (s * lpr + glane) * V + v;
+      c[s][v] = a.grad_balance != nullptr && e < a.E ? by * a.coefficients[e] : 0.0f;
+    }
+  const long wave = static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  for (int pass = 0; pass < a.passes; pass += ROWS) {
+    const long r0 = (wave * a.passes + pass) * per + (lane >> ls);
+    U raw[ROWS][STEPS];
+    f32x2 stats[ROWS];
+    bool use[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const long at = min(r0 + i * per, static_cast<long>(a.T) - 1);
+      use[i] = a.counted == nullptr || a.counted[at] != 0;
+      stats[i] = reinterpret_cast<const f32x2*>(a.row_stats)[at];
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) raw[i][s] = static_cast<const U*>(a.scores)[at * units + min(s * lpr + glane, units - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const long row = r0 + i * per;
+      const float top = stats[i][0], inverse = 1.0f / stats[i][1];
+      float p[STEPS][V], dot = 0.0f;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        unpack<DT, kBytes>(raw[i][s], p[s]);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          p[s][v] = exp_of(p[s][v] - top) * inverse;
+          if (s * lpr + glane < units) dot = __builtin_fmaf(c[s][v], p[s][v], dot);
+        }
+      }
+      dot = segment_sum(dot, lpr);
+      if (a.grad_z != nullptr) dot -= q * (top + logf(stats[i][1]));
+      if (row >= a.T || pass + i >= a.passes) continue;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        float o[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] = use[i] ? p[s][v] * (c[s][v] - dot) : 0.0f;
+        const int u = s * lpr + glane;
+        if (u < units) pack_store<DT, V>(static_cast<char*>(a.out) + (static_cast<size_t>(row) * units + u) * kBytes, o);
+      }
+    }
+  }
+}
+
+int check_scores(int T, int E, int dtype) {
+  if (T < 0 || E <= 0) return fail(BRT_E_INVALID, "bad shape T=%d E=%d", T, E);
+  if (dtype != BRT_F32 && dtype != BRT_F16 && dtype != BRT_BF16) return fail(BRT_E_UNSUPPORTED, "dtype %d is not supported", dtype);
+  if (E > kMostPaths) return fail(BRT_E_UNSUPPORTED, "more than %d paths", kMostPaths);
+  if (static_cast<long>(T) * E >= (1l << 31)) return fail(BRT_E_UNSUPPORTED, "T*E >= 2^31");
+  return BRT_OK;
+}
+
+// Lanes that share a row of n units.
+int lanes_of(int n) {
+  int ls = 0;
+  while ((1 << ls) < std::min(n, kWave)) ++ls;
+  return ls;
+}
+
+int blocks_of(int T, int E) {
+  if (static_cast<long>(T) * E <= (1 << 14)) return 1;
+  return static_cast<int>(std::min<long>(kMostBlocks, (static_cast<long>(T) * E + (1 << 13) - 1) >> 13));
+}
+
+// The kernel of a row shape: launch(type, V, STEPS, ROWS)
+template <typename F>
+void with_scores(int dtype, int E, bool units, F&& launch) {
+  using std::integral_constant;
+  auto shape = [&](auto dt, auto v) {
+    constexpr int V = decltype(v)::value;
+    const int n = E / V;
+    if (n <= kWave) launch(dt, v, integral_constant<int, 1>{}, integral_constant<int, 4>{});
+    else if (n <= 4 * kWave) launch(dt, v, integral_constant<int, V == 8 ? 2 : 4>{}, integral_constant<int, 1>{});
+    else if constexpr (V == 1) launch(dt, v, integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  };
+  auto type = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (units) shape(dt, integral_constant<int, 16 / elem_bytes(DT)>{});
+    else shape(dt, integral_constant<int, 1>{});
+  };
+  if (dtype == BRT_F32) type(integral_constant<int, BRT_F32>{});
+  else if (dtype == BRT_F16) type(integral_constant<int, BRT_F16>{});
+  else type(integral_constant<int, BRT_BF16>{});
+}
+
+}  // namespace
+}  // namespace brt
+
+using namespace brt;
+
+extern "C" size_t brt_hip_balance_loss_workspace_bytes(int T, int E) {
+  if (T < 0 || E <= 0 || E > kMostPaths || static_cast<long>(T) * E >= (1l << 31)) return 0;
+  const int blocks = blocks_of(T, E);
+  return blocks == 1 ? 0 : static_cast<size_t>(blocks) * (E + 1) * 8;
+}
+
+extern "C" int brt_hip_balance_loss(const void* scores, const int32_t* path_ids, const uint8_t* counted, float* balance, float* z,
+                                    int32_t* counts, float* row_stats, float* coefficients, int T, int E, int k, int dtype,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int rc = check_scores(T, E, dtype); rc != BRT_OK) return rc;
+  if (k < 0) return fail(BRT_E_INVALID, "bad shape k=%d", k);
+  if (static_cast<long>(T) * k >= (1l << 31)) return fail(BRT_E_UNSUPPORTED, "T*k >= 2^31");
+  if ((T > 0 && (!scores || (k > 0 && !path_ids))) || !balance || !z || !counts) return fail(BRT_E_INVALID, "null argument");
+  if (row_stats && !aligned(row_stats, 8)) return fail(BRT_E_UNSUPPORTED, "row_stats is not aligned to 8 bytes");
+  BalanceArgs a{scores, path_ids, counted, balance, z, counts, row_stats, coefficients, nullptr, nullptr, nullptr, nullptr, T, E, k, blocks_of(T, E), 0};
+  if (a.blocks > 1) {
+    if (!workspace || !aligned(workspace, 4) || workspace_bytes < brt_hip_balance_loss_workspace_bytes(T, E))
+      return fail(BRT_E_WORKSPACE, "workspace of %zu bytes needed, got %zu", brt_hip_balance_loss_workspace_bytes(T, E), workspace_bytes);
+    a.part_p = static_cast<float*>(workspace);
+    a.part_counts = static_cast<int*>(workspace) + static_cast<size_t>(a.blocks) * E;
+    a.part_z = a.part_p + static_cast<size_t>(a.blocks) * E * 2;
+    a.part_n = static_cast<int*>(workspace) + static_cast<size_t>(a.blocks) * (2 * E + 1);
+  }
+  const int per = 16 / elem_bytes(dtype);
+  const bool units = E % per == 0 && aligned(scores, 16);
+  a.ls = lanes_of(units ? E / per : E);
+  hipStream_t st = as_stream(stream);
+  with_scores(dtype, E, units, [&](auto dt, auto v, auto steps, auto rows) {
+    hipLaunchKernelGGL((balance_kernel<decltype(dt)::value, decltype(v)::value, decltype(steps)::value, decltype(rows)::value>),
+                       dim3(a.blocks), dim3(kBlock), 0, st, a);
+  });
+  if (const int rc = check_launch("balance_kernel"); rc != BRT_OK || a.blocks == 1) return rc;
+  int slices = 1;
+  while (slices < 64 && kJoin / (2 * slices) >= E) slices *= 2;
+  hipLaunchKernelGGL(balance_join_kernel, dim3(1), dim3(kJoin), 0, st, a, slices);
+  return check_launch("balance_join_kernel");
+}
+
+extern "C" int brt_hip_balance_loss_grad(const void* scores, const uint8_t* counted, const float* row_stats, const float* coefficients,
+                                         const float* grad_balance, const float* grad_z, void* grad_scores, int T, int E, int dtype,
+                                         void* stream) {
+  if (const int rc = check_scores(T, E, dtype); rc != BRT_OK) return rc;
+  if (T == 0) return BRT_OK;
+  if (!scores || !row_stats || !coefficients || !grad_scores) return fail(BRT_E_INVALID, "null argument");
+  if (!aligned(row_stats, 8)) return fail(BRT_E_UNSUPPORTED, "row_stats is not aligned to 8 bytes");
+  BalanceGradArgs a{scores, counted, row_stats, coefficients, grad_balance, grad_z, grad_scores, T, E, 0, 1};
+  const int per = 16 / elem_bytes(dtype);
+  const bool units = E % per == 0 && aligned(scores, 16) && aligned(grad_scores, 16);
+  a.ls = lanes_of(units ? E / per : E);
+  hipStream_t st = as_stream(stream);
+  with_scores(dtype, E, units, [&](auto dt, auto v, auto steps, auto rows) {
+    constexpr int R = decltype(rows)::value;
+    a.passes = R;
+    const long rows_pb = static_cast<long>(4 * R) << (6 - a.ls);
+    hipLaunchKernelGGL((balance_grad_kernel<decltype(dt)::value, decltype(v)::value, decltype(steps)::value, R>),
+                       dim3(static_cast<unsigned>((T + rows_pb - 1) / rows_pb)), dim3(256), 0, st, a);
+  });
+  return check_launch("balance_grad_kernel");
+}

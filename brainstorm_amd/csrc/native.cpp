@@ -847,6 +847,69 @@ PyObject* combine_by_rows(const Args& a) {  // in_data, path_ids, seat_rows, wei
   return wrap(CombineByRows::apply(in, optional(weights), ids, seats, entries, o.typed ? o.out_type : in.scalar_type()));
 }
 
+// ---- losses of the router ------------------------------------------------------------------------------
+struct Losses {
+  Tensor balance, z, counts, row_stats, coefficients;
+};
+Losses losses(const Tensor& given, const Tensor& ids_given, const Tensor& counted_given, bool gradient) {
+  const Tensor score = dense(given), ids = dense(ids_given), counted = counted_given.defined() ? dense(counted_given) : counted_given;
+  const c10::DeviceGuard guard(score.device());
+  const int64_t T = score.size(0), E = score.size(1);
+  Losses made{empty({}, at::kFloat, score), empty({}, at::kFloat, score), empty({E}, at::kInt, score), Tensor(), Tensor()};
+  if (gradient) made.row_stats = empty({T, 2}, at::kFloat, score), made.coefficients = empty({E + 1}, at::kFloat, score);
+  const size_t bytes = brt_hip_balance_loss_workspace_bytes(T, E);
+  const Tensor ws = bytes > 0 ? scratch(bytes, score) : Tensor();
+  check(brt_hip_balance_loss(ptr(score), iptr(ids), static_cast<const uint8_t*>(ptr(counted)), fptr(made.balance), fptr(made.z), iptr(made.counts),
+                             fptr(made.row_stats), fptr(made.coefficients), T, E, ids.size(1), code_of(score.scalar_type()), ptr(ws), bytes,
+                             stream_of(score)));
+  return made;
+}
+
+struct BalanceLoss : Function<BalanceLoss> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& score, const Tensor& ids, const std::optional<Tensor>& counted) {
+    ctx->set_materialize_grads(false);
+    const Losses made = losses(score, ids, counted.value_or(Tensor()), true);
+    ctx->mark_non_differentiable({made.counts});
+    ctx->save_for_backward({score, counted.value_or(Tensor()), made.row_stats, made.coefficients});
+    return {made.balance, made.z, made.counts};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    return differentiable_once(3, grads, saved, [&](variable_list& made) {
+      if (!grads[0].defined() && !grads[1].defined()) return;
+      const Tensor score = dense(saved[0]), counted = saved[1].defined() ? dense(saved[1]) : Tensor();
+      const Tensor by_balance = grads[0].defined() ? dense(grads[0]) : Tensor(), by_z = grads[1].defined() ? dense(grads[1]) : Tensor();
+      const c10::DeviceGuard guard(score.device());
+      made[0] = empty(score.sizes(), score.scalar_type(), score);
+      check(brt_hip_balance_loss_grad(ptr(score), static_cast<const uint8_t*>(ptr(counted)), fptr(saved[2]), fptr(saved[3]), fptr(by_balance),
+                                      fptr(by_z), ptr(made[0]), score.size(0), score.size(1), code_of(score.scalar_type()), stream_of(score)));
+    });
+  }
+};
+
+PyObject* balance_loss(const Args& a) {  // score, path_ids, counted
+  const Tensor score = a.tensor(0), ids = a.tensor(1), counted = a.tensor_or_none(2);
+  on_device(score, "score"), on_device(ids, "path_ids");
+  if (score.dim() != 2) runtime_error("score must be [cells, paths]");
+  data_type(score, "score data type");
+  int32(ids, "path_ids");
+  if (ids.dim() != 2 || ids.size(0) != score.size(0)) runtime_error("path_ids must be [cells, k]");
+  if (ids.device() != score.device()) runtime_error("path_ids is on another device than score");
+  if (counted.defined()) {
+    if (counted.scalar_type() != at::kBool || counted.dim() != 1 || counted.size(0) != score.size(0)) runtime_error("counted must be a bool tensor [cells]");
+    if (counted.device() != score.device()) runtime_error("counted is on another device than score");
+  }
+  // (the library counts in 32 bits and checks there; what it is handed has to fit)
+  for (const int64_t n : {score.size(0), score.size(1), ids.size(1)})
+    if (n >= int64_t{1} << 31) not_implemented("a dimension of 2^31 and more");
+  if (tracked(score)) {
+    const variable_list made = BalanceLoss::apply(score, ids, optional(counted));
+    return tuple(wrap(made[0]), wrap(made[1]), wrap(made[2]));
+  }
+  const Losses made = losses(score, ids, counted, false);
+  return tuple(wrap(made.balance), wrap(made.z), wrap(made.counts));
+}
+
 // ---- grouped GEMM ------------------------------------------------------------------------------------
 Tensor rounded_to_bf16(const Tensor& given) {
   const Tensor in = dense(given);
@@ -1332,7 +1395,7 @@ PyObject* entry(PyObject*, PyObject* const* v, Py_ssize_t n) {
 #define BRT_ENTRY(name, n) \
   { #name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&entry<name, n>)), METH_FASTCALL, nullptr }
 PyMethodDef methods[] = {
-    BRT_ENTRY(topk_hot_mask, 2),    BRT_ENTRY(gate_topk, 5),           BRT_ENTRY(throttle_hotmask, 3),
+    BRT_ENTRY(topk_hot_mask, 2),    BRT_ENTRY(gate_topk, 5),           BRT_ENTRY(balance_loss, 3),        BRT_ENTRY(throttle_hotmask, 3),
     BRT_ENTRY(generate, 5),         BRT_ENTRY(route_and_dispatch, 7),  BRT_ENTRY(route_by_path, 7),
     BRT_ENTRY(dispatch, 12),  BRT_ENTRY(dispatch_and_read, 8),        BRT_ENTRY(combine, 8),             BRT_ENTRY(combine_by_row_tags, 5),
     BRT_ENTRY(top1_to_capacity, 2), BRT_ENTRY(top1_route_to_capacity, 4), BRT_ENTRY(dispatch_by_rows, 6), BRT_ENTRY(combine_by_rows, 8),     BRT_ENTRY(grouped_linear, 16),

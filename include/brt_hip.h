@@ -502,6 +502,26 @@ int brt_hip_combine_by_rows_grad(const void* grad, const void* rows, const float
                                  void* stream);
 
 /*
+ * Losses that keep a router balanced (no counterpart in the reference), over the n cells t with counted[t] != 0 (counted [T] bytes, NULL: all
+ * of them): p = softmax(scores[t]), counts[e] the entries of path_ids [T,k] that name path e (ids outside 0 .. E-1 name none),
+ *     balance = E / (n * n * k) * sum_e counts[e] * sum_t p[t,e]        z = 1 / n * sum_t log(sum_e exp(scores[t,e]))^2,
+ *   both zero where nothing counts.  Sums are fp32 within a workgroup and fp64 over them, in an order that the sizes fix.
+ *   row_stats [T,2] (8-byte aligned) and coefficients [E+1] are what the gradient reads; NULL where none is wanted.  E <= 1024.
+ *   Workspace of brt_hip_balance_loss_workspace_bytes(T, E) bytes (may be 0), 4-byte aligned, uninitialised, one per call in flight.
+ *
+ * brt_hip_balance_loss_grad: grad_scores [T,E] (of dtype) from the gradients of the two losses (one fp32 value each on the device;
+ *   NULL: zero): p * (c[e] - sum_i c[i] p[t,i] + q * log(sum exp)), c = grad_balance * E / (n * n * k) * counts, q = grad_z * 2 / n; zeros
+ *   for cells that do not count.  scores and counted as they were given.
+ */
+size_t brt_hip_balance_loss_workspace_bytes(int T, int E);
+int brt_hip_balance_loss(const void* scores, const int32_t* path_ids, const uint8_t* counted, float* balance, float* z,
+                         int32_t* counts, float* row_stats, float* coefficients, int T, int E, int k, int dtype,
+                         void* workspace, size_t workspace_bytes, void* stream);
+int brt_hip_balance_loss_grad(const void* scores, const uint8_t* counted, const float* row_stats,
+                              const float* coefficients, const float* grad_balance, const float* grad_z,
+                              void* grad_scores, int T, int E, int dtype, void* stream);
+
+/*
  * Expert products in 8-bit floating point (OCP e4m3, round to nearest even) with one fp32 scale per block of 128.
  *
  * brt_hip_quantize_rows: rows [P,K] (dtype) -> q [P,pitch] and scales [KB,P], KB = ceil(K / 128): of every 128 elements of a
