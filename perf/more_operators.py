@@ -317,10 +317,11 @@ def _own_weight(w):
 
 def _own(state):
     from brainstorm_amd._C import router as c_router
-    from brainstorm_amd.jit import grouped_linear_int4
 
     case = state["case"]
     kind = case["kind"]
+    if kind in ("int4", "serve"):
+        from brainstorm_amd.jit import grouped_linear_int4
     if kind == "int4":
         return {"out": grouped_linear_int4(state["x"], _own_weight(state["w"]), state["loads"], bias=state["bias"],
                                            activation=case["activation"])}
