@@ -160,6 +160,11 @@ SIGNATURES = {
         [_c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_int, _c_int,
          _c_int, _c_int, _c_int, _c_int, _c_ptr],
     ),
+    "brt_hip_grouped_gemm_int4": (
+        _c_int,
+        [_c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int,
+         _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr],
+    ),
     "brt_hip_grouped_gemm_fp8_blocks": (_c_int, [_c_int] * 5),
     "brt_hip_gate_topk_grad": (
         _c_int,
@@ -274,7 +279,8 @@ def call_count() -> int:
     """Calls into the library that queued device work since the process started, read-backs of a few words
     among them.  Every such call is one kernel launch, except the compact route, the tag-index gather and the throttled
     top-1 route, which are two, and index generation and throttling, which are one or two by the size of the mask.
-    The router's losses are one launch, or two for larger batches, their gradient is one.  A product in 8 bits is one launch, or two where its rows are quantized first; a gradient of the route is one.
+    The router's losses are one launch, or two for larger batches, their gradient is one.
+    A product in 8 bits is one launch, or two where its rows are quantized first; one with 4-bit weights is one; a gradient of the route is one.
     Tests use the difference around a layer to pin how many launches a route costs."""
     return _calls + (_native.calls() if _native is not None else 0)
 

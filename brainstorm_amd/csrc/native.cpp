@@ -1165,6 +1165,63 @@ PyObject* grouped_linear_fp8(const Args& a) {
   return !out_blocks ? wrap(out) : as_rows(made.q.defined() ? made : quantized(out, "out"), N);
 }
 
+// ---- products with weights of 4 bits -------------------------------------------------------------------
+// x, values, scales, zeros, in_features, out_features, group, loads, bias, activation, out, out_dtype, row_entries, entries_per_cell
+PyObject* grouped_linear_int4(const Args& a) {
+  const Tensor x = a.tensor(0), w = a.tensor(1), w_scales = a.tensor(2), w_zeros = a.tensor_or_none(3), loads_given = a.tensor(7);
+  const Tensor bias_given = a.tensor_or_none(8), entries_given = a.tensor_or_none(12);
+  const int64_t K = a.integer(4), N = a.integer(5), group = a.integer(6), per_cell = a.integer(13);
+  Tensor out = a.tensor_or_none(10);
+  on_device(x, "x"), on_device(w, "weight"), on_device(w_scales, "weight scales"), on_device(loads_given, "loads");
+  int32(loads_given, "loads");
+  if (group != 32 && group != 64 && group != 128) not_implemented("groups of other than 32, 64 or 128 elements");
+  if (x.dim() != 2 || x.size(1) != K) runtime_error("x must be [rows, in_features]");
+  if (K < 0 || N < 0 || w.scalar_type() != at::kByte || w.dim() != 4 || w.size(3) != 1024 || w.size(1) != (N + 15) / 16 || w.size(2) != blocks_of(K))
+    runtime_error("weight values must be uint8 [experts, tiles of 16 rows, blocks of 128 columns, 1024]");
+  const int64_t E = w.size(0), G = (K + group - 1) / group;
+  data_type(w_scales, "weight scale data type");
+  if (w_scales.sizes() != at::IntArrayRef({E, w.size(1), G, 16})) runtime_error("weight scales must be [experts, tiles of 16 rows, groups, 16]");
+  if (w_zeros.defined() && (w_zeros.scalar_type() != at::kByte || w_zeros.sizes() != w_scales.sizes()))
+    runtime_error("weight zeros must be uint8 of the scales' shape");
+  if (loads_given.numel() != E) runtime_error("one load per expert is needed");
+  if (bias_given.defined()) {
+    data_type(bias_given, "bias data type");
+    if (bias_given.sizes() != at::IntArrayRef({E, N})) runtime_error("bias must be [experts, out_features]");
+  }
+  if (entries_given.defined()) {
+    on_device(entries_given, "row_entries"), int32(entries_given, "row_entries");
+    if (entries_given.dim() != 1) runtime_error("row_entries must be a vector");
+    if (per_cell < 1) runtime_error("entries_per_cell must be at least one");
+  }
+  for (const Tensor* t : std::initializer_list<const Tensor*>{&w, &w_scales, &w_zeros, &loads_given, &bias_given, &entries_given, &out})
+    if (t->defined()) same_device(*t, x, "an operand");
+  const int64_t P = entries_given.defined() ? entries_given.numel() : x.size(0);
+  for (const int64_t n : {x.size(0), P, K, E, N, per_cell})
+    if (n >= int64_t{1} << 31) not_implemented("a dimension of 2^31 and more");
+  const int x_type = data_type(x, "x data type");
+  at::ScalarType type = x.scalar_type();
+  const bool typed = a.dtype(11, &type);
+  if (code_of(type) < 0) not_implemented("output data type is not supported");
+  const c10::DeviceGuard guard(x.device());
+  if (out.defined()) {
+    if (typed && type != out.scalar_type()) runtime_error("out is given: it says its type");
+    data_type(out, "output data type");
+    if (out.sizes() != at::IntArrayRef({P, N}) || !out.is_contiguous()) runtime_error("out must be a contiguous [rows, out_features] tensor");
+    for (const Tensor* t : std::initializer_list<const Tensor*>{&x, &w, &w_scales, &w_zeros, &loads_given, &bias_given, &entries_given})
+      if (t->defined() && shares_memory(out, *t)) runtime_error("out shares memory with an operand");
+  } else {
+    out = empty({P, N}, type, x);
+  }
+  const Tensor rows = dense_units(x), values = dense_units(w), scales = dense_units(w_scales), loads = dense(loads_given);
+  const Tensor zero_points = w_zeros.defined() ? dense_units(w_zeros) : w_zeros, bias = bias_given.defined() ? dense(bias_given) : bias_given;
+  const Tensor entries = entries_given.defined() ? dense(entries_given) : entries_given;
+  check(brt_hip_grouped_gemm_int4(ptr(rows), x_type, iptr(entries), per_cell, x.size(0), ptr(values), ptr(scales), code_of(scales.scalar_type()),
+                                  static_cast<const uint8_t*>(ptr(zero_points)), group, iptr(loads), ptr(bias),
+                                  bias.defined() ? code_of(bias.scalar_type()) : BRT_F32, ptr(out), code_of(out.scalar_type()), E, P, N, K,
+                                  a.integer(9), stream_of(x)));
+  return wrap(out);
+}
+
 // ---- values on the host ------------------------------------------------------------------------------
 // The values of an int32 vector as a list.
 PyObject* int_list(const Args& a) {
@@ -1402,7 +1459,7 @@ PyMethodDef methods[] = {
     BRT_ENTRY(grouped_linear_f32, 16), BRT_ENTRY(cast_f32_to_bf16, 1), BRT_ENTRY(branch_key, 5),        BRT_ENTRY(int_list, 1),
     BRT_ENTRY(ordinary, 3),         BRT_ENTRY(plain, 1),            BRT_ENTRY(of_class, 2),            BRT_ENTRY(matrix, 4),
     BRT_ENTRY(grid, 5),                BRT_ENTRY(split_rows, 4),
-    BRT_ENTRY(quantize_rows, 1), BRT_ENTRY(grouped_linear_fp8, 11),
+    BRT_ENTRY(quantize_rows, 1), BRT_ENTRY(grouped_linear_fp8, 11), BRT_ENTRY(grouped_linear_int4, 14),
     BRT_ENTRY(sum_rows_by_index, 3), BRT_ENTRY(combine_flows, 2), BRT_ENTRY(one_value, 2),         BRT_ENTRY(unique_tags, 1),      BRT_ENTRY(calls, 0),            {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "brt_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

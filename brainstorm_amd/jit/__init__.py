@@ -21,9 +21,11 @@ import torch.nn as nn
 
 from brainstorm_amd import _lib
 from brainstorm_amd._C import router as c_router
+from brainstorm_amd.jit.int4 import Int4Weight, pack_int4, quantize_int4
 from brainstorm_amd.runtime import deferred
 
-__all__ = ["make_jit_kernel", "grouped_linear", "grouped_linear_fp8", "quantize_rows", "GroupedLinearKernel"]
+__all__ = ["make_jit_kernel", "grouped_linear", "grouped_linear_fp8", "quantize_rows", "grouped_linear_int4", "Int4Weight", "pack_int4",
+           "quantize_int4", "GroupedLinearKernel"]
 
 _ACT = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "gelu": _lib.ACT_GELU, "relu": _lib.ACT_RELU}
 
@@ -97,6 +99,24 @@ def grouped_linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scales: tor
     twice the rate."""
     return _lib.native().grouped_linear_fp8(x, weight, weight_scales, loads, bias, _ACT[activation], x_scales, out, out_dtype,
                                             bool(out_blocks), exact)
+
+
+def grouped_linear_int4(x: torch.Tensor, weight: Int4Weight, loads: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
+                        activation: Optional[str] = None, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                        row_entries: Optional[torch.Tensor] = None, entries_per_cell: int = 1) -> torch.Tensor:
+    """:func:`grouped_linear` on 4-bit weights: ``out[s_e : s_e + loads[e]] = act(x[s_e : s_e + loads[e]] @ W_e^T + b_e)`` with an
+    :class:`Int4Weight` (:func:`quantize_int4`, :func:`pack_int4`).  ``x`` (``[rows, in_features]``, fp32 / fp16 / bf16, in_features a
+    multiple of 8) is not rounded; a group's products are summed with fp32 accumulation, scaled in fp32 and summed in an order that the
+    shape fixes; bias (``[experts, out_features]``), activation and one rounding follow.
+
+    With ``row_entries`` (what ``route_by_path`` writes: 1-based entry ``t * k + j + 1`` of every row, ``k = entries_per_cell``) ``x`` is
+    cell-major and row r is its cell ``(row_entries[r] - 1) // k``: no dispatch is needed.  A row without an entry is a row of zeros.
+
+    The result has ``x``'s type (or ``out_dtype``); a given ``out`` is filled in place (contiguous ``[rows, out_features]``, memory of its
+    own: it is written while the operands are read).  Rows behind the last expert's are not written.  A row that holds NaN or an infinity
+    gives NaN.  Results are cut off from autograd, as those of :func:`grouped_linear`."""
+    return _lib.native().grouped_linear_int4(x, weight.values, weight.scales, weight.zeros, weight.in_features, weight.out_features,
+                                             weight.group, loads, bias, _ACT[activation], out, out_dtype, row_entries, int(entries_per_cell))
 
 
 def _linear(x, out, weight_table, bias_table, loads, in_features, out_features, activation, *, tags=None, gather=False,

@@ -553,6 +553,24 @@ int brt_hip_grouped_gemm_fp8_quantizes(int E, int P, int N);
 int brt_hip_grouped_gemm_fp8_blocks(int E, int P, int N, int K, int out_dtype);
 
 /*
+ * Expert products with weights of 4 bits: for the rows r of expert e (packed by expert, rows behind the last one's are not written)
+ *     out[r,n] = act(sum over groups of k of scales[e,n,group] * sum_k (q[e,n,k] - zeros[e,n,group]) * x[r,k] + bias[e,n]),
+ *   group 32, 64 or 128 elements, zeros NULL: all 8.  x [P,K] of x_dtype; or, with row_entries [P] (1-based entries t * entries_per_cell + j
+ *   + 1, as brt_hip_route_by_path writes them), the cells [T,K], and row r is cell (row_entries[r] - 1) / entries_per_cell, zeros where
+ *   there is none.  bias [E,N] of bias_dtype or NULL, out [P,N] of out_dtype, apart from all that is read.
+ *   w [E, ceil(N/16), ceil(K/128), 1024] bytes: byte 16 * (16 * g + r) + 4 * j + m of a block is row r of the tile, column 32 * j + 8 * g + m in its
+ *   low and column + 4 in its high four bits.  scales (of scale_dtype) and zeros (bytes) [E, ceil(N/16), ceil(K/group), 16].  What stands behind
+ *   the N-th row or K-th column does not count (scales there are finite).
+ * Products are exact, sums fp32 in an order that the shape fixes, the result is rounded once.  K is a multiple of 8, x, w and scales are 16-byte
+ * aligned, zeros 4-byte; P below 2^24, N, K and E up to 2^28.  Loads below zero count as none, rows of experts behind the P-th do not exist.
+ * The first call of a shape on a device has to happen outside graph capture.
+ */
+int brt_hip_grouped_gemm_int4(const void* x, int x_dtype, const int32_t* row_entries, int entries_per_cell, int T,
+                              const void* w, const void* scales, int scale_dtype, const uint8_t* zeros, int group,
+                              const int32_t* loads, const void* bias, int bias_dtype, void* out, int out_dtype, int E,
+                              int P, int N, int K, int activation, void* stream);
+
+/*
  * brt_hip_grouped_gemm / _f32out / _routed / _routed_f32out / _by_rows on fp32 rows of x (16-byte aligned), which the
  * kernel rounds to bf16 itself: the bits of brt_hip_cast_f32_to_bf16 followed by the bf16 form, without that pass.
  * gather_in as in the routed forms, from the tag matrix (entries_per_cell = 0; row_tags_out as there) or the row
