@@ -22,18 +22,15 @@
 namespace brt {
 namespace {
 
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kB = 128;            // elements of a scale block, bytes of a K-step
 constexpr float kMax = 448.0f;     // the largest e4m3 value
 constexpr float kLeast = 0x1p-100f;  // blocks whose largest value is below this are scaled as if it were this
-constexpr int kXcds = 8, kCusPerXcd = 32;
 constexpr int kPatchRows = 4;
 constexpr int kMostRows = 1 << 24;   // 65 times as many are added up in 32 bits
 constexpr int kMostColumns = 1 << 30;  // and experts: rounded up to tiles they are counted in 32 bits
 constexpr int kMostExperts = 512;  // whose row blocks a workgroup keeps in LDS
-constexpr uint32_t kNowhere = 0x7ffffff0u;  // an offset past every extent: reads as zero, costs no request
 
 // ------------------------------------------------------------------------------------- quantization
 // A block's largest magnitude as the bits of its magnitude (integers order them, NaN on top) -> its scale and the inverse.
@@ -100,38 +97,6 @@ struct Fp8Args {
   int E, P, N, K, KB, NB, tiles_n;
 };
 
-__device__ __forceinline__ i32x4 make_rsrc(const void* p, size_t bytes) {
-  const uint64_t a = reinterpret_cast<uint64_t>(p);
-  i32x4 r;
-  r[0] = __builtin_amdgcn_readfirstlane(static_cast<int>(a));
-  r[1] = __builtin_amdgcn_readfirstlane(static_cast<int>((a >> 32) & 0xffff));
-  r[2] = __builtin_amdgcn_readfirstlane(static_cast<int>(bytes));
-  r[3] = 0x00020000;
-  return r;
-}
-// 16 bytes per lane from the buffer into LDS at lds_base + 16 * lane (M0; one wait state between its write and the load).  The
-// compiler does not know that it touches LDS, nor counts it: every wait for such a load is written out.
-__device__ __forceinline__ void load_to_lds(const i32x4& rsrc, uint32_t voffset, uint32_t soffset, uint32_t lds_base) {
-  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :
-               : "{m0}"(lds_base), "v"(voffset), "s"(rsrc), "s"(soffset)
-               : "memory");
-}
-// ... 4 bytes per lane, at lds_base + 4 * lane
-__device__ __forceinline__ void load_word_to_lds(const i32x4& rsrc, uint32_t voffset, uint32_t lds_base) {
-  asm volatile("s_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-               :
-               : "{m0}"(lds_base), "v"(voffset), "s"(rsrc)
-               : "memory");
-}
-// all but the last N loads of this wavefront have landed
-template <int N>
-__device__ __forceinline__ void wait_loads_but() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
-__device__ __forceinline__ void block_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
 __device__ __forceinline__ f32x4 multiply(const i32x8& w, const i32x8& x) {
   const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, 0, 0, 0);

@@ -35,7 +35,7 @@ struct Int4Args {
   const void* bias;      // [E, N] of bias_dtype or null
   void* out;             // [P, N] of out_dtype
   int s_dtype, bias_dtype, out_dtype, act;
-  int E, P, N, K, KB, G, T, per_cell, tiles, tiles_n;
+  int E, P, N, K, KB, G, T, per_cell, tiles, tiles_n, blocks;
 };
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -126,6 +126,11 @@ __device__ __forceinline__ f32x4 values_of(const Four& f, int dtype) {
 __device__ __forceinline__ float gelu_f32(float v) {
   const float b = __builtin_elementwise_maximum(v, -1e30f);  // (0 * inf; NaN stays)
   return 0.5f * b * (1.0f + erff(b * 0.70710678118654752f));
+}
+template <int ACT, int OUT>
+__device__ __forceinline__ float activated_for(float v) {
+  if constexpr (ACT == BRT_ACT_GELU && OUT == BRT_F32) return gelu_f32(v);
+  else return activated<ACT>(v);
 }
 __device__ __forceinline__ float activated_for(float v, int act, int out_dtype) {
   return act == BRT_ACT_GELU && out_dtype == BRT_F32 ? gelu_f32(v) : activated(v, act);
@@ -283,11 +288,278 @@ int launch_few_rows(Int4Args& a, hipStream_t st) {
   if (tiles < 512) return launch_few_rows<XDT, GJ, 1, 1, 8>(a, st);
   return launch_few_rows<XDT, GJ, 1, 2, 8>(a, st);
 }
+// Row blocks of all experts (blocks of 1 << bits rows; at most `most`, which the host has made the grid for).
+__device__ __forceinline__ int count_blocks(const Int4Args& a, int bits, int most) {
+  const int lane = lane_id();
+  int blocks = 0;
+  for (int base = 0; base < a.E; base += kWave) {
+    const int given = a.loads[min(base + lane, a.E - 1)];
+    const int m = base + lane < a.E ? min(max(given, 0), a.P) : 0;
+    blocks = min(blocks + read_lane(wave_inclusive_scan((m + (1 << bits) - 1) >> bits), kWave - 1), most);
+  }
+  return blocks;
+}
+
+// Many rows per expert: 64 x 256 tiles, four wavefronts, 64 columns and all rows each: a weight is unpacked once a workgroup, and not held in
+// LDS.  Rows go straight into LDS, two blocks of 128 columns ahead, weights and scales into registers one block ahead.  The groups'
+// sums of x are made for the block ahead by a quarter of its rows a wavefront, and pass through LDS; -scale * zero times them, for four
+// groups at a time, is a product of its own in fp32 (v_mfma_f32_16x16x4_f32): the vector units, which unpack and scale beside the matrix
+// units, have no part in it.
+template <int XDT, int GJ>
+__global__ __launch_bounds__(256, XDT == BRT_F32 ? 1 : 2) void int4_tiles_kernel(Int4Args a) {
+  using Part = RowPart<XDT>;
+  using W = decltype(weights_of<XDT>(0));
+  constexpr int MT = 4, BM = 16 * MT, NT = 4, kGroups = 4 / GJ, kStages = 3;
+  constexpr int kBits = 6;
+  constexpr int kRow = kB * elem_bytes(XDT), kChunks = kRow / 16, kRowsOfLoad = 64 / kChunks;  // of a row in LDS; rows of a load
+  constexpr int XL = BM / kRowsOfLoad / 4;  // loads of a wavefront and block
+  constexpr int kStage = BM * kRow;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  // of the last eight groups: the rows' sums, and a wavefront's scales and their products with the zero points
+  float* const s_sums = reinterpret_cast<float*>(smem + kStages * kStage);  // [8][BM]
+  float* const s_scales = s_sums + 8 * BM + (threadIdx.x >> 6) * (2 * 8 * 16 * NT);  // [8][16 NT]
+  float* const s_zeros = s_scales + 8 * 16 * NT;                                      // [8][16 NT]
+  const int lane = lane_id(), g = lane >> 4, c16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Tiles are dealt out in runs, one per XCD: neighbours in the list, four row blocks wide, share rows and weights in its L2.
+  const int blocks = count_blocks(a, kBits, a.blocks);
+  const int tiles = blocks * a.tiles_n, run = (tiles + kXcds - 1) / kXcds;
+  const int turn = blockIdx.x / kXcds, t = blockIdx.x % kXcds * run + turn;
+  if (turn >= run || t >= tiles) return;
+  constexpr int kPatch = 4;
+  const int patch = t / (kPatch * a.tiles_n), in = t - patch * kPatch * a.tiles_n, wide = min(kPatch, blocks - patch * kPatch);
+  const Block found = find_block(a, patch * kPatch + in % wide, kBits);
+  if (found.rows == 0) return;
+  const int e = __builtin_amdgcn_readfirstlane(found.e), row0 = __builtin_amdgcn_readfirstlane(found.row0), rows = __builtin_amdgcn_readfirstlane(found.rows);
+  const int tile0 = in / wide * 16 + wave * NT;
+
+  // Slot s of LDS row r holds chunk s ^ (r & 15) of that row: the 16 rows that are read together at one chunk cover all banks.
+  const uint32_t row_bytes = static_cast<uint32_t>(a.K) * elem_bytes(XDT);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem)));
+  i32x4 rx;
+  if (a.entries != nullptr) rx = make_rsrc(a.x, static_cast<size_t>(a.T) * row_bytes);
+  else rx = make_rsrc(static_cast<const char*>(a.x) + static_cast<size_t>(row0) * row_bytes, static_cast<size_t>(rows) * row_bytes);
+  uint32_t from[XL], chunk_at[XL];
+#pragma unroll
+  for (int i = 0; i < XL; ++i) {
+    const int r = (wave * XL + i) * kRowsOfLoad + lane / kChunks;
+    chunk_at[i] = ((lane % kChunks) ^ (r & 15)) * 16;
+    from[i] = kNowhere;
+    if (r < rows) {
+      if (a.entries == nullptr) {
+        from[i] = r * row_bytes + chunk_at[i];
+      } else {
+        const int word = a.entries[row0 + r], cell = a.per_cell > 1 ? (word - 1) / a.per_cell : word - 1;
+        if (word >= 1 && cell < a.T) from[i] = cell * row_bytes + chunk_at[i];
+      }
+    }
+  }
+  auto request = [&](int kb) {
+    const uint32_t to = lds0 + kb % kStages * kStage, start = kb * kRow;
+    if (start + kRow <= row_bytes) {
+#pragma unroll
+      for (int i = 0; i < XL; ++i) load_to_lds(rx, from[i], start, to + (wave * XL + i) * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < XL; ++i) load_to_lds(rx, start + chunk_at[i] >= row_bytes ? kNowhere : from[i], start, to + (wave * XL + i) * 1024);
+    }
+  };
+  struct Loaded {
+    u32x4 w[NT];
+    uint32_t s[kGroups], z[kGroups];  // of the wavefront's column `lane`
+  };
+  auto load = [&](int kb, Loaded& to) {
+    const size_t first = static_cast<size_t>(e) * a.tiles;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+      to.w[j] = *reinterpret_cast<const u32x4*>(a.w + ((first + min(tile0 + j, a.tiles - 1)) * a.KB + kb) * 1024 + lane * 16);
+    size_t one[kGroups];
+#pragma unroll
+    for (int h = 0; h < kGroups; ++h)
+      one[h] = ((first + min(tile0 + g, a.tiles - 1)) * a.G + min(kb * kGroups + h, a.G - 1)) * 16 + c16;
+    if (a.s_dtype == BRT_F32) {
+#pragma unroll
+      for (int h = 0; h < kGroups; ++h) to.s[h] = static_cast<const uint32_t*>(a.scales)[one[h]];
+    } else {
+#pragma unroll
+      for (int h = 0; h < kGroups; ++h) to.s[h] = static_cast<const uint16_t*>(a.scales)[one[h]];
+    }
+#pragma unroll
+    for (int h = 0; h < kGroups; ++h) to.z[h] = 8;
+    if (a.zeros != nullptr) {
+#pragma unroll
+      for (int h = 0; h < kGroups; ++h) to.z[h] = a.zeros[one[h]];
+    }
+  };
+  auto keep_scales = [&](int kb, const Loaded& of) {
+#pragma unroll
+    for (int h = 0; h < kGroups; ++h) {
+      const int at = (kb * kGroups + h & 7) * 16 * NT + lane;
+      const float s = a.s_dtype == BRT_F32 ? __uint_as_float(of.s[h]) : a.s_dtype == BRT_F16 ? f16_to_float(of.s[h]) : bf16_to_float(of.s[h]);
+      s_scales[at] = s, s_zeros[at] = -static_cast<float>(of.z[h]) * s;
+    }
+  };
+  // fragment p of a block, of 16 rows from row r0
+  auto part_of = [&](int kb, int r0, int p) {
+    const char* const row = smem + kb % kStages * kStage + (r0 + c16) * kRow;
+    u32x4 raw[Part::kUnits];
+#pragma unroll
+    for (int u = 0; u < Part::kUnits; ++u) raw[u] = *reinterpret_cast<const u32x4*>(row + ((((p * 4 + g) * Part::kUnits + u) ^ c16) * 16));
+    return Part(raw);
+  };
+  W one;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) one[i] = 1.0f;
+  auto sum_up = [&](int kb) {
+    const int r0 = wave * (BM / 4);
+#pragma unroll
+    for (int h = 0; h < kGroups; ++h) {
+      f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int p = 0; p < GJ; ++p) sum = multiply(one, part_of(kb, r0, h * GJ + p), sum);
+      if (g == 0) s_sums[((kb * kGroups + h) & 7) * BM + r0 + c16] = sum[0];
+    }
+  };
+
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  Loaded now;
+  request(0);
+  if (a.KB > 1) request(1);
+  load(0, now);
+  keep_scales(0, now);
+  wait_loads_but<0>();
+  __syncthreads();
+  sum_up(0);
+#pragma unroll 1
+  for (int kb = 0; kb < a.KB; ++kb) {
+    wait_loads_but<0>();
+    __syncthreads();  // the block after this one has landed, its sums' place and the stage of the one before are free
+    // groups four by four: their zero points come off when the last of them is at hand
+    const int group = (kb * kGroups & ~3) + g;
+    const bool correct = ((kb + 1) * kGroups & 3) == 0 || kb + 1 == a.KB;
+    if (kb + 2 < a.KB) request(kb + 2);
+    Loaded next;
+    if (kb + 1 < a.KB) {
+      load(kb + 1, next);
+      sum_up(kb + 1);
+    }
+#pragma unroll
+    for (int h = 0; h < kGroups; ++h) {
+      W w[NT][GJ];
+      f32x4 s[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        s[j] = *reinterpret_cast<const f32x4*>(s_scales + (kb * kGroups + h & 7) * 16 * NT + j * 16 + g * 4);
+#pragma unroll
+        for (int p = 0; p < GJ; ++p) w[j][p] = weights_of<XDT>(now.w[j][h * GJ + p]);
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        f32x4 part[NT];
+#pragma unroll
+        for (int p = 0; p < GJ; ++p) {
+          const Part x = part_of(kb, i * 16, h * GJ + p);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) part[j] = multiply(w[j][p], x, p == 0 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : part[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) acc[i][j][q] = __builtin_fmaf(part[j][q], s[j][q], acc[i][j][q]);
+      }
+      // (the sums are complete here: left alone, the compiler puts off the additions of all groups, whose parts do not fit)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(acc[i][j]));
+    }
+    if (correct) {
+      float off[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) off[j] = group < a.G ? s_zeros[(group & 7) * 16 * NT + j * 16 + c16] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const float sum = group < (kb + 1) * kGroups ? s_sums[(group & 7) * BM + i * 16 + c16] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(off[j], sum, acc[i][j], 0, 0, 0);
+      }
+    }
+    now = next;
+    if (kb + 1 < a.KB) keep_scales(kb + 1, now);
+  }
+
+  const bool whole = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+  auto store = [&](auto act, auto out) {
+    constexpr int ACT = decltype(act)::value, OUT = decltype(out)::value;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int n = (tile0 + j) * 16 + g * 4;
+      float bias[4];
+      biases<4>(a, e, min(n, a.N - 1), bias);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        float v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = activated_for<ACT, OUT>(acc[i][j][q] + bias[q]);
+        char* const to = static_cast<char*>(a.out) + ((static_cast<size_t>(row0) + i * 16 + c16) * a.N + n) * elem_bytes(OUT);
+        if (i * 16 + c16 >= rows || n >= a.N) continue;
+        if (whole) {
+          pack_store<OUT, 4>(to, v);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float one[1] = {v[q]};
+            if (n + q < a.N) pack_store<OUT, 1>(to + q * elem_bytes(OUT), one);
+          }
+        }
+      }
+    }
+  };
+  auto with_act = [&](auto out) {
+    if (a.act == BRT_ACT_GELU) store(std::integral_constant<int, BRT_ACT_GELU>{}, out);
+    else if (a.act == BRT_ACT_RELU) store(std::integral_constant<int, BRT_ACT_RELU>{}, out);
+    else store(std::integral_constant<int, BRT_ACT_NONE>{}, out);
+  };
+  if (a.out_dtype == BRT_F32) with_act(std::integral_constant<int, BRT_F32>{});
+  else if (a.out_dtype == BRT_F16) with_act(std::integral_constant<int, BRT_F16>{});
+  else with_act(std::integral_constant<int, BRT_BF16>{});
+}
+
+template <int XDT, int GJ>
+int launch_tiles(Int4Args& a, hipStream_t st) {
+  constexpr int BM = 64, kBytes = 3 * BM * kB * elem_bytes(XDT) + 8 * BM * 4 + 4 * 2 * 8 * 64 * 4;
+  const auto fn = int4_tiles_kernel<XDT, GJ>;
+  if (const int rc = allow_dynamic_lds(reinterpret_cast<const void*>(fn), kBytes); rc != BRT_OK) return rc;
+  a.tiles_n = (a.tiles + 15) / 16;
+  // an expert adds at most one row block that it does not fill
+  const long blocks = static_cast<long>(a.P) / BM + std::min(a.E, a.P);
+  if (blocks * a.tiles_n >= (1l << 31) - kXcds) return fail(BRT_E_UNSUPPORTED, "too many tiles");
+  a.blocks = static_cast<int>(blocks);
+  const long grid = (blocks * a.tiles_n + kXcds - 1) / kXcds * kXcds;
+  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(256), kBytes, st, a);
+  return check_launch("int4_tiles_kernel");
+}
+
+bool few_rows(const Int4Args& a, int x_dtype) {
+  // (the tiles address 64 rows, or all cells, in 31 bits)
+  const long row = static_cast<long>(a.K) * elem_bytes(x_dtype), reach = a.entries != nullptr ? a.T * row : 64 * row;
+  if (reach >= (1l << 31) - (1 << 16) || (a.entries != nullptr && a.T == 0)) return true;
+  return a.P <= 16 || a.P <= 16l * a.E;
+}
+template <int XDT, int GJ>
+int launch(Int4Args& a, hipStream_t st) {
+  if (few_rows(a, XDT)) return launch_few_rows<XDT, GJ>(a, st);
+  return launch_tiles<XDT, GJ>(a, st);
+}
 template <int XDT>
 int launch(Int4Args& a, int group, hipStream_t st) {
-  if (group == 32) return launch_few_rows<XDT, 1>(a, st);
-  if (group == 64) return launch_few_rows<XDT, 2>(a, st);
-  return launch_few_rows<XDT, 4>(a, st);
+  if (group == 32) return launch<XDT, 1>(a, st);
+  if (group == 64) return launch<XDT, 2>(a, st);
+  return launch<XDT, 4>(a, st);
 }
 
 bool is_type(int dtype) { return dtype == BRT_F32 || dtype == BRT_F16 || dtype == BRT_BF16; }

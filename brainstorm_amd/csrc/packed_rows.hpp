@@ -1,5 +1,5 @@
-// Shared by the products of rows that are packed by expert with weights of few bits: where an expert's rows are, and the
-// epilogue.  `A` is a kernel's argument block: loads [E], P rows, N columns; bias [E, N] of bias_dtype or null; out [P, N] of
+// Shared by the products of rows that are packed by expert with weights of few bits: loads straight into LDS, where an expert's
+// rows are, and the epilogue.  `A` is a kernel's argument block: loads [E], P rows, N columns; bias [E, N] of bias_dtype or null; out [P, N] of
 // out_dtype; act.
 #pragma once
 
@@ -7,6 +7,44 @@
 #include "rows.hpp"
 
 namespace brt {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kXcds = 8, kCusPerXcd = 32;
+constexpr uint32_t kNowhere = 0x7ffffff0u;  // an offset past every extent: reads as zero, costs no request
+
+__device__ __forceinline__ i32x4 make_rsrc(const void* p, size_t bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  i32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane(static_cast<int>(a));
+  r[1] = __builtin_amdgcn_readfirstlane(static_cast<int>((a >> 32) & 0xffff));
+  r[2] = __builtin_amdgcn_readfirstlane(static_cast<int>(bytes));
+  r[3] = 0x00020000;
+  return r;
+}
+// 16 bytes per lane from the buffer into LDS at lds_base + 16 * lane (M0; one wait state between its write and the load).  The
+// compiler does not know that it touches LDS, nor counts it: every wait for such a load is written out.
+__device__ __forceinline__ void load_to_lds(const i32x4& rsrc, uint32_t voffset, uint32_t soffset, uint32_t lds_base) {
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "{m0}"(lds_base), "v"(voffset), "s"(rsrc), "s"(soffset)
+               : "memory");
+}
+// ... 4 bytes per lane, at lds_base + 4 * lane
+__device__ __forceinline__ void load_word_to_lds(const i32x4& rsrc, uint32_t voffset, uint32_t lds_base) {
+  asm volatile("s_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "{m0}"(lds_base), "v"(voffset), "s"(rsrc)
+               : "memory");
+}
+// all but the last N loads of this wavefront have landed
+template <int N>
+__device__ __forceinline__ void wait_loads_but() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
+__device__ __forceinline__ void block_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 struct Block {
   int e, row0, rows;
