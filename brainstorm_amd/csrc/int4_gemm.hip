@@ -92,34 +92,30 @@ __device__ __forceinline__ f32x4 multiply(const W& w, const RowPart<XDT>& x, f32
   for (int p = RowPart<XDT>::kParts - 1; p >= 0; --p) c = multiply(w, x.part[p], c);  // (the small parts first)
   return c;
 }
-
-// Four values of the layout's 16 columns of a group.
-struct Four {
-  u32x4 raw;
-};
-__device__ __forceinline__ Four load_four(const void* base, int dtype, size_t at) {
-  Four f{};
-  if (dtype == BRT_F32) {
-    f.raw = *reinterpret_cast<const u32x4*>(static_cast<const float*>(base) + at);
-  } else {
-    const u32x2 half = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(base) + at);
-    f.raw[0] = half[0], f.raw[1] = half[1];
-  }
-  return f;
+template <int XDT, typename W>
+__device__ __forceinline__ f32x4 multiply(const RowPart<XDT>& x, const W& w, f32x4 c) {
+#pragma unroll
+  for (int p = RowPart<XDT>::kParts - 1; p >= 0; --p) c = multiply(x.part[p], w, c);
+  return c;
 }
-__device__ __forceinline__ f32x4 values_of(const Four& f, int dtype) {
-  f32x4 v;
+
+// The scale that was loaded as `bits`.
+__device__ __forceinline__ float scale_of(uint32_t bits, int dtype) {
+  return dtype == BRT_F32 ? __uint_as_float(bits) : dtype == BRT_F16 ? f16_to_float(bits) : bf16_to_float(bits);
+}
+
+template <int COUNT>
+__device__ __forceinline__ void scales_of(const uint32_t (&bits)[COUNT], int dtype, float (&s)[COUNT]) {
   if (dtype == BRT_F32) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = __uint_as_float(f.raw[q]);
+    for (int i = 0; i < COUNT; ++i) s[i] = __uint_as_float(bits[i]);
+  } else if (dtype == BRT_F16) {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) s[i] = f16_to_float(bits[i]);
   } else {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const uint32_t h = q % 2 ? f.raw[q / 2] >> 16 : f.raw[q / 2] & 0xffffu;
-      v[q] = dtype == BRT_F16 ? f16_to_float(h) : bf16_to_float(h);
-    }
+    for (int i = 0; i < COUNT; ++i) s[i] = bf16_to_float(bits[i]);
   }
-  return v;
 }
 
 // GELU of an fp32 result: the fit that the other products share is off by up to 4.3e-6, which 16 bits hide and fp32 shows.
@@ -148,146 +144,133 @@ __device__ __forceinline__ const char* row_of(const Int4Args& a, int row) {
   return static_cast<const char*>(a.x) + at * a.K * elem_bytes(XDT);
 }
 
-// Few rows per expert: the weights are streamed once and set the time.  A workgroup takes 16 NT columns and 16 MT rows; its W
-// wavefronts take blocks of 128 columns in turn, weights and rows straight into the fragments' registers, the next block's requested
-// while this one is multiplied, and add up their sums through LDS.
-template <int XDT, int GJ, int MT, int NT, int W>
+// Few rows per expert: the weights are streamed once and set the time.  A workgroup takes 16 NT columns and 16 rows; its W
+// wavefronts take blocks of 128 columns in turn, weights and rows straight into the fragments' registers, and add up their sums through
+// LDS.  The rows are the first operand here: a lane holds results of one column, whose scale and zero point are one register each.
+template <int XDT, int GJ, int NT, int W>
 __global__ __launch_bounds__(W * 64) void int4_few_rows_kernel(Int4Args a) {
   using Part = RowPart<XDT>;
+  using Weights = decltype(weights_of<XDT>(0));
   constexpr int kGroups = 4 / GJ;  // of a block; GJ fragments share a group
-  constexpr int kBits = MT == 1 ? 4 : MT == 2 ? 5 : 6;
-  __shared__ f32x4 s_part[W][NT * MT][64];
+  __shared__ float s_part[W][NT][16][17];  // [row][column], a column of padding
   const int lane = lane_id(), g = lane >> 4, c16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int block = blockIdx.x / a.tiles_n, tile0 = (blockIdx.x - block * a.tiles_n) * NT, n0 = tile0 * 16;
-  const Block at = find_block(a, block, kBits);
+  const Block at = find_block(a, block, 4);
   if (at.rows == 0) return;
-  const char* row[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) row[i] = row_of<XDT>(a, at.row0 + min(i * 16 + c16, at.rows - 1));
-  // the biases of the tiles that this wavefront finishes: fetched ahead of the weights, not behind the last barrier
-  constexpr int kFinished = (MT * NT + W - 1) / W;
-  float bias[kFinished][4];
-#pragma unroll
-  for (int f = 0; f < kFinished; ++f) biases<4>(a, at.e, n0 + (wave + f * W) % NT * 16 + g * 4, bias[f]);
+  const char* const row = row_of<XDT>(a, at.row0 + min(c16, at.rows - 1));
+  const bool whole_rows = __ballot(row == nullptr) == 0;
 
-  struct Loaded {
-    u32x4 w[NT], x[MT][4 * Part::kUnits];
-    Four s[NT][kGroups];
-    uint32_t z[NT][kGroups];
-  };
-  auto load = [&](int kb, Loaded& to) {
+  f32x4 acc[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  Weights minus_one;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) minus_one[i] = -1.0f;
+  for (int kb = wave; kb < a.KB; kb += W) {
+    u32x4 raw_w[NT], raw_x[4 * Part::kUnits];
+    uint32_t raw_s[NT][kGroups], raw_z[NT][kGroups];
+    size_t one[NT][kGroups];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const size_t tile = static_cast<size_t>(at.e) * a.tiles + min(tile0 + j, a.tiles - 1);
-      to.w[j] = *reinterpret_cast<const u32x4*>(a.w + (tile * a.KB + kb) * 1024 + lane * 16);
+      raw_w[j] = *reinterpret_cast<const u32x4*>(a.w + (tile * a.KB + kb) * 1024 + lane * 16);
 #pragma unroll
-      for (int h = 0; h < kGroups; ++h) {
-        const size_t four = (tile * a.G + min(kb * kGroups + h, a.G - 1)) * 16 + g * 4;
-        to.s[j][h] = load_four(a.scales, a.s_dtype, four);
-        to.z[j][h] = a.zeros != nullptr ? *reinterpret_cast<const uint32_t*>(a.zeros + four) : 0x08080808u;
-      }
+      for (int h = 0; h < kGroups; ++h) one[j][h] = (tile * a.G + min(kb * kGroups + h, a.G - 1)) * 16 + c16, raw_z[j][h] = 8;
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int l = 0; l < 4 * Part::kUnits; ++l) {
-        const int k = kb * kB + l / Part::kUnits * 32 + g * 8;
-        const bool there = k < a.K && row[i] != nullptr;  // (K is a multiple of 8)
-        to.x[i][l] = zero_unit<16>();
-        if (there) to.x[i][l] = *reinterpret_cast<const u32x4*>(row[i] + static_cast<size_t>(k) * elem_bytes(XDT) + l % Part::kUnits * 16);
+    for (int l = 0; l < 4 * Part::kUnits; ++l) {
+      const int k = kb * kB + l / Part::kUnits * 32 + g * 8;
+      const char* const from = row + static_cast<size_t>(k) * elem_bytes(XDT) + l % Part::kUnits * 16;
+      if (whole_rows && kb * kB + kB <= a.K) {
+        raw_x[l] = *reinterpret_cast<const u32x4*>(from);
+      } else {
+        raw_x[l] = zero_unit<16>();
+        if (k < a.K && row != nullptr) raw_x[l] = *reinterpret_cast<const u32x4*>(from);  // (K is a multiple of 8)
       }
-  };
-
-  f32x4 acc[MT][NT];
+    }
+    if (a.s_dtype == BRT_F32) {
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  decltype(weights_of<XDT>(0)) minus_one;
+        for (int h = 0; h < kGroups; ++h) raw_s[j][h] = static_cast<const uint32_t*>(a.scales)[one[j][h]];
+    } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) minus_one[i] = -1.0f;
-
-  Loaded now;
-  if (wave < a.KB) load(wave, now);
-  for (int kb = wave; kb < a.KB; kb += W) {
-    Loaded next;
-    if (kb + W < a.KB) load(kb + W, next);
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int h = 0; h < kGroups; ++h) raw_s[j][h] = static_cast<const uint16_t*>(a.scales)[one[j][h]];
+    }
+    if (a.zeros != nullptr) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int h = 0; h < kGroups; ++h) raw_z[j][h] = a.zeros[one[j][h]];
+    }
 #pragma unroll
     for (int h = 0; h < kGroups; ++h) {
-      decltype(weights_of<XDT>(0)) w[NT][GJ];
-      f32x4 s[NT];
-      float z[NT][4];
+      f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f}, part[NT];  // sum: minus the rows' sums over the group, in every column
+#pragma unroll
+      for (int p = 0; p < GJ; ++p) sum = multiply(Part(&raw_x[(h * GJ + p) * Part::kUnits]), minus_one, sum);
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) part[j][q] = static_cast<float>(raw_z[j][h]) * sum[q];
+#pragma unroll
+      for (int p = 0; p < GJ; ++p) {
+        const Part x(&raw_x[(h * GJ + p) * Part::kUnits]);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) part[j] = multiply(x, weights_of<XDT>(raw_w[j][h * GJ + p]), part[j]);
+      }
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        s[j] = values_of(now.s[j][h], a.s_dtype);
+        const float s = scale_of(raw_s[j][h], a.s_dtype);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) z[j][q] = static_cast<float>((now.z[j][h] >> (8 * q)) & 0xffu);
-#pragma unroll
-        for (int p = 0; p < GJ; ++p) w[j][p] = weights_of<XDT>(now.w[j][h * GJ + p]);
-      }
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f}, part[NT];  // sum: minus the row's sum over the group, in all four
-#pragma unroll
-        for (int p = 0; p < GJ; ++p) sum = multiply(minus_one, Part(&now.x[i][(h * GJ + p) * Part::kUnits]), sum);
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) part[j][q] = z[j][q] * sum[q];
-#pragma unroll
-        for (int p = 0; p < GJ; ++p) {
-          const Part x(&now.x[i][(h * GJ + p) * Part::kUnits]);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) part[j] = multiply(w[j][p], x, part[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) acc[i][j][q] = __builtin_fmaf(part[j][q], s[j][q], acc[i][j][q]);
+        for (int q = 0; q < 4; ++q) acc[j][q] = __builtin_fmaf(part[j][q], s, acc[j][q]);
       }
     }
-    now = next;
   }
 
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+  for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int j = 0; j < NT; ++j) s_part[wave][i * NT + j][lane] = acc[i][j];
+    for (int q = 0; q < 4; ++q) s_part[wave][j][g * 4 + q][c16] = acc[j][q];
   __syncthreads();
+  // four lanes a row of a tile, four columns each
   const bool whole = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+  const int r = lane >> 2, c4 = (lane & 3) * 4;
+  for (int j = wave; j < NT; j += W) {
+    const int n = n0 + j * 16 + c4;
+    if (r >= at.rows || n >= a.N) continue;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, bias[4];
+    biases<4>(a, at.e, n, bias);
 #pragma unroll
-  for (int f = 0; f < kFinished; ++f) {
-    const int p = wave + f * W;
-    if (p >= MT * NT) break;
-    f32x4 sum = s_part[0][p][lane];
+    for (int w = 0; w < W; ++w)
 #pragma unroll
-    for (int w = 1; w < W; ++w) sum += s_part[w][p][lane];
-    const int r = p / NT * 16 + c16, n = n0 + p % NT * 16 + g * 4;
-    float v[4];
+      for (int q = 0; q < 4; ++q) v[q] += s_part[w][j][r][c4 + q];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = activated_for(sum[q] + bias[f][q], a.act, a.out_dtype);
-    if (r < at.rows && n < a.N) store_part<4>(a, static_cast<size_t>(at.row0) + r, n, whole, v);
+    for (int q = 0; q < 4; ++q) v[q] = activated_for(v[q] + bias[q], a.act, a.out_dtype);
+    store_part<4>(a, static_cast<size_t>(at.row0) + r, n, whole, v);
   }
 }
 
-template <int XDT, int GJ, int MT, int NT, int W>
+template <int XDT, int GJ, int NT, int W>
 int launch_few_rows(Int4Args& a, hipStream_t st) {
-  constexpr int kRows = 16 * MT;
-  const long blocks = static_cast<long>(a.P) / kRows + std::min(a.E, a.P);
+  const long blocks = static_cast<long>(a.P) / 16 + std::min(a.E, a.P);
   a.tiles_n = (a.tiles + NT - 1) / NT;
   if (blocks * a.tiles_n >= (1l << 31)) return fail(BRT_E_UNSUPPORTED, "too many tiles");
-  hipLaunchKernelGGL((int4_few_rows_kernel<XDT, GJ, MT, NT, W>), dim3(static_cast<unsigned>(blocks * a.tiles_n)), dim3(W * 64), 0, st, a);
+  hipLaunchKernelGGL((int4_few_rows_kernel<XDT, GJ, NT, W>), dim3(static_cast<unsigned>(blocks * a.tiles_n)), dim3(W * 64), 0, st, a);
   return check_launch("int4_few_rows_kernel");
 }
 template <int XDT, int GJ>
 int launch_few_rows(Int4Args& a, hipStream_t st) {
-  const long tiles = static_cast<long>(std::min(a.E, a.P)) * a.tiles;
-  if constexpr (XDT != BRT_F32)
-    if (a.P > 16 && a.P > 10l * a.E) return launch_few_rows<XDT, GJ, 2, 2, 8>(a, st);
-  if (tiles < 512) return launch_few_rows<XDT, GJ, 1, 1, 8>(a, st);
-  return launch_few_rows<XDT, GJ, 1, 2, 8>(a, st);
+  const long tiles = (static_cast<long>(a.P) / 16 + std::min(a.E, a.P)) * a.tiles;
+  if (tiles < 384) return launch_few_rows<XDT, GJ, 1, 16>(a, st);
+  if (tiles < 1536) return launch_few_rows<XDT, GJ, 2, 8>(a, st);
+  if (a.KB >= 24) return launch_few_rows<XDT, GJ, 4, 8>(a, st);
+  if (tiles < 4096) return launch_few_rows<XDT, GJ, 2, 4>(a, st);
+  return launch_few_rows<XDT, GJ, 4, 4>(a, st);
 }
+
 // Row blocks of all experts (blocks of 1 << bits rows; at most `most`, which the host has made the grid for).
 __device__ __forceinline__ int count_blocks(const Int4Args& a, int bits, int most) {
   const int lane = lane_id();
@@ -305,11 +288,11 @@ __device__ __forceinline__ int count_blocks(const Int4Args& a, int bits, int mos
 // sums of x are made for the block ahead by a quarter of its rows a wavefront, and pass through LDS; -scale * zero times them, for four
 // groups at a time, is a product of its own in fp32 (v_mfma_f32_16x16x4_f32): the vector units, which unpack and scale beside the matrix
 // units, have no part in it.
-template <int XDT, int GJ>
+template <int XDT, int GJ, int NT>
 __global__ __launch_bounds__(256, XDT == BRT_F32 ? 1 : 2) void int4_tiles_kernel(Int4Args a) {
   using Part = RowPart<XDT>;
   using W = decltype(weights_of<XDT>(0));
-  constexpr int MT = 4, BM = 16 * MT, NT = 4, kGroups = 4 / GJ, kStages = 3;
+  constexpr int MT = 4, BM = 16 * MT, kGroups = 4 / GJ, kStages = 3;
   constexpr int kBits = 6;
   constexpr int kRow = kB * elem_bytes(XDT), kChunks = kRow / 16, kRowsOfLoad = 64 / kChunks;  // of a row in LDS; rows of a load
   constexpr int XL = BM / kRowsOfLoad / 4;  // loads of a wavefront and block
@@ -331,7 +314,7 @@ __global__ __launch_bounds__(256, XDT == BRT_F32 ? 1 : 2) void int4_tiles_kernel
   const Block found = find_block(a, patch * kPatch + in % wide, kBits);
   if (found.rows == 0) return;
   const int e = __builtin_amdgcn_readfirstlane(found.e), row0 = __builtin_amdgcn_readfirstlane(found.row0), rows = __builtin_amdgcn_readfirstlane(found.rows);
-  const int tile0 = in / wide * 16 + wave * NT;
+  const int tile0 = in / wide * (4 * NT) + wave * NT;
 
   // Slot s of LDS row r holds chunk s ^ (r & 15) of that row: the 16 rows that are read together at one chunk cover all banks.
   const uint32_t row_bytes = static_cast<uint32_t>(a.K) * elem_bytes(XDT);
@@ -354,8 +337,8 @@ __global__ __launch_bounds__(256, XDT == BRT_F32 ? 1 : 2) void int4_tiles_kernel
       }
     }
   }
-  auto request = [&](int kb) {
-    const uint32_t to = lds0 + kb % kStages * kStage, start = kb * kRow;
+  auto request = [&](int kb, int stage) {
+    const uint32_t to = lds0 + stage, start = kb * kRow;
     if (start + kRow <= row_bytes) {
 #pragma unroll
       for (int i = 0; i < XL; ++i) load_to_lds(rx, from[i], start, to + (wave * XL + i) * 1024);
@@ -366,58 +349,69 @@ __global__ __launch_bounds__(256, XDT == BRT_F32 ? 1 : 2) void int4_tiles_kernel
   };
   struct Loaded {
     u32x4 w[NT];
-    uint32_t s[kGroups], z[kGroups];  // of the wavefront's column `lane`
+    uint32_t s[kGroups];  // of the wavefront's column `lane`
+    uint8_t z[kGroups];
   };
+  // (tiles behind the last hold what that one does; groups behind the last, whose rows are zeros, a scale of zero)
+  const size_t first = static_cast<size_t>(e) * a.tiles + min(tile0, a.tiles - 1);
+  const int left = a.tiles - 1 - min(tile0, a.tiles - 1);
+  const uint8_t* const w0 = a.w + first * a.KB * 1024;
+  const int s_bytes = a.s_dtype == BRT_F32 ? 4 : 2;
+  const uint32_t s_place = min(g, left) * a.G * 16 + c16;
+  const int s_extent = (min(NT - 1, left) + 1) * a.G * 16;
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<char*>(static_cast<const char*>(a.scales)) + first * a.G * 16 * s_bytes, 0, s_extent * s_bytes, 0x00020000);
+  // (without zero points: nothing is in reach, which reads as zeros)
+  const __amdgpu_buffer_rsrc_t rz = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.zeros) + first * a.G * 16, 0, a.zeros != nullptr ? s_extent : 0, 0x00020000);
+  const float z_least = a.zeros != nullptr ? 0.0f : 8.0f;
   auto load = [&](int kb, Loaded& to) {
-    const size_t first = static_cast<size_t>(e) * a.tiles;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
-      to.w[j] = *reinterpret_cast<const u32x4*>(a.w + ((first + min(tile0 + j, a.tiles - 1)) * a.KB + kb) * 1024 + lane * 16);
-    size_t one[kGroups];
+      to.w[j] = *reinterpret_cast<const u32x4*>(w0 + (static_cast<size_t>(min(j, left)) * a.KB + kb) * 1024 + static_cast<uint32_t>(lane * 16));
+    uint32_t place[kGroups];
 #pragma unroll
-    for (int h = 0; h < kGroups; ++h)
-      one[h] = ((first + min(tile0 + g, a.tiles - 1)) * a.G + min(kb * kGroups + h, a.G - 1)) * 16 + c16;
+    for (int h = 0; h < kGroups; ++h) place[h] = kb * kGroups + h < a.G ? s_place : kNowhere / 4;
     if (a.s_dtype == BRT_F32) {
 #pragma unroll
-      for (int h = 0; h < kGroups; ++h) to.s[h] = static_cast<const uint32_t*>(a.scales)[one[h]];
+      for (int h = 0; h < kGroups; ++h) to.s[h] = __builtin_amdgcn_raw_buffer_load_b32(rs, place[h] * 4, (kb * kGroups + h) * 64, 0);
     } else {
 #pragma unroll
-      for (int h = 0; h < kGroups; ++h) to.s[h] = static_cast<const uint16_t*>(a.scales)[one[h]];
+      for (int h = 0; h < kGroups; ++h) to.s[h] = __builtin_amdgcn_raw_buffer_load_b16(rs, place[h] * 2, (kb * kGroups + h) * 32, 0);
     }
 #pragma unroll
-    for (int h = 0; h < kGroups; ++h) to.z[h] = 8;
-    if (a.zeros != nullptr) {
-#pragma unroll
-      for (int h = 0; h < kGroups; ++h) to.z[h] = a.zeros[one[h]];
-    }
+    for (int h = 0; h < kGroups; ++h) to.z[h] = __builtin_amdgcn_raw_buffer_load_b8(rz, a.zeros != nullptr ? place[h] : kNowhere, (kb * kGroups + h) * 16, 0);
   };
   auto keep_scales = [&](int kb, const Loaded& of) {
+    float s[kGroups];
+    scales_of(of.s, a.s_dtype, s);
 #pragma unroll
     for (int h = 0; h < kGroups; ++h) {
-      const int at = (kb * kGroups + h & 7) * 16 * NT + lane;
-      const float s = a.s_dtype == BRT_F32 ? __uint_as_float(of.s[h]) : a.s_dtype == BRT_F16 ? f16_to_float(of.s[h]) : bf16_to_float(of.s[h]);
-      s_scales[at] = s, s_zeros[at] = -static_cast<float>(of.z[h]) * s;
+      const int at = (kb * kGroups + h & 7) * 16 * NT + lane % (16 * NT);  // (lanes beyond hold what another one does)
+      s_scales[at] = s[h], s_zeros[at] = -(static_cast<float>(of.z[h]) + z_least) * s[h];
     }
   };
-  // fragment p of a block, of 16 rows from row r0
-  auto part_of = [&](int kb, int r0, int p) {
-    const char* const row = smem + kb % kStages * kStage + (r0 + c16) * kRow;
+  // fragment p of 16 rows from row r0 of a stage
+  uint32_t part_at[4][Part::kUnits];
+#pragma unroll
+  for (int p = 0; p < 4; ++p)
+#pragma unroll
+    for (int u = 0; u < Part::kUnits; ++u) part_at[p][u] = c16 * kRow + (((p * 4 + g) * Part::kUnits + u) ^ c16) * 16;
+  auto part_of = [&](int stage, int r0, int p) {
     u32x4 raw[Part::kUnits];
 #pragma unroll
-    for (int u = 0; u < Part::kUnits; ++u) raw[u] = *reinterpret_cast<const u32x4*>(row + ((((p * 4 + g) * Part::kUnits + u) ^ c16) * 16));
+    for (int u = 0; u < Part::kUnits; ++u) raw[u] = *reinterpret_cast<const u32x4*>(smem + (part_at[p][u] + stage) + r0 * kRow);
     return Part(raw);
   };
   W one;
 #pragma unroll
   for (int i = 0; i < 8; ++i) one[i] = 1.0f;
-  auto sum_up = [&](int kb) {
-    const int r0 = wave * (BM / 4);
+  auto sum_up = [&](int kb, int stage) {
 #pragma unroll
     for (int h = 0; h < kGroups; ++h) {
       f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int p = 0; p < GJ; ++p) sum = multiply(one, part_of(kb, r0, h * GJ + p), sum);
-      if (g == 0) s_sums[((kb * kGroups + h) & 7) * BM + r0 + c16] = sum[0];
+      for (int p = 0; p < GJ; ++p) sum = multiply(one, part_of(stage + wave * (BM / 4) * kRow, 0, h * GJ + p), sum);
+      s_sums[((kb * kGroups + h) & 7) * BM + wave * (BM / 4) + c16] = sum[0];  // (four lanes hold and write the same)
     }
   };
 
@@ -427,13 +421,14 @@ __global__ __launch_bounds__(256, XDT == BRT_F32 ? 1 : 2) void int4_tiles_kernel
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   Loaded now;
-  request(0);
-  if (a.KB > 1) request(1);
+  request(0, 0);
+  if (a.KB > 1) request(1, kStage);
   load(0, now);
   keep_scales(0, now);
   wait_loads_but<0>();
   __syncthreads();
-  sum_up(0);
+  sum_up(0, 0);
+  int stage = 0, stage1 = kStage, stage2 = 2 * kStage;  // of this block and the two after it
 #pragma unroll 1
   for (int kb = 0; kb < a.KB; ++kb) {
     wait_loads_but<0>();
@@ -441,42 +436,51 @@ __global__ __launch_bounds__(256, XDT == BRT_F32 ? 1 : 2) void int4_tiles_kernel
     // groups four by four: their zero points come off when the last of them is at hand
     const int group = (kb * kGroups & ~3) + g;
     const bool correct = ((kb + 1) * kGroups & 3) == 0 || kb + 1 == a.KB;
-    if (kb + 2 < a.KB) request(kb + 2);
+    if (kb + 2 < a.KB) request(kb + 2, stage2);
     Loaded next;
-    if (kb + 1 < a.KB) {
-      load(kb + 1, next);
-      sum_up(kb + 1);
-    }
+    load(min(kb + 1, a.KB - 1), next);
+    sum_up(kb + 1, stage1);  // (behind the last block: of what the stage holds, for a place that is not read)
+    // fragment by fragment: the next one's weights are unpacked and its rows fetched beside this one's products
+    W w[2][NT];
+    Part x[2][MT] = {{part_of(stage, 0, 0), part_of(stage, 16, 0), part_of(stage, 32, 0), part_of(stage, 48, 0)}, {part_of(stage, 0, 1), part_of(stage, 16, 1), part_of(stage, 32, 1), part_of(stage, 48, 1)}};
+    f32x4 part[MT][NT];
 #pragma unroll
-    for (int h = 0; h < kGroups; ++h) {
-      W w[NT][GJ];
-      f32x4 s[NT];
+    for (int j = 0; j < NT; ++j) w[0][j] = weights_of<XDT>(now.w[j][0]);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        s[j] = *reinterpret_cast<const f32x4*>(s_scales + (kb * kGroups + h & 7) * 16 * NT + j * 16 + g * 4);
+    for (int p = 0; p < 4; ++p) {
+      if (p > 0 && p < 3) {
 #pragma unroll
-        for (int p = 0; p < GJ; ++p) w[j][p] = weights_of<XDT>(now.w[j][h * GJ + p]);
+        for (int i = 0; i < MT; ++i) x[(p + 1) & 1][i] = part_of(stage, i * 16, p + 1);
       }
+      if (p < 3) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        f32x4 part[NT];
-#pragma unroll
-        for (int p = 0; p < GJ; ++p) {
-          const Part x = part_of(kb, i * 16, h * GJ + p);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) part[j] = multiply(w[j][p], x, p == 0 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : part[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) acc[i][j][q] = __builtin_fmaf(part[j][q], s[j][q], acc[i][j][q]);
+        for (int j = 0; j < NT; ++j) w[(p + 1) & 1][j] = weights_of<XDT>(now.w[j][p + 1]);
       }
-      // (the sums are complete here: left alone, the compiler puts off the additions of all groups, whose parts do not fit)
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(acc[i][j]));
+        for (int j = 0; j < NT; ++j) part[i][j] = multiply(w[p & 1][j], x[p & 1][i], p % GJ == 0 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : part[i][j]);
+      if (p % GJ == GJ - 1) {
+        f32x4 s[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) s[j] = *reinterpret_cast<const f32x4*>(s_scales + (kb * kGroups + p / GJ & 7) * 16 * NT + j * 16 + g * 4);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[i][j][q] = __builtin_fmaf(part[i][j][q], s[j][q], acc[i][j][q]);
+            asm volatile("" : "+v"(acc[i][j]));  // (left alone, the compiler puts the additions off, and the parts do not fit)
+          }
+      }
     }
+#ifdef SGB
+#pragma unroll
+    for (int m = 0; m < MT * NT * 4 * Part::kParts; ++m) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, SGB, 0);
+    }
+#endif
     if (correct) {
       float off[NT];
 #pragma unroll
@@ -489,7 +493,9 @@ __global__ __launch_bounds__(256, XDT == BRT_F32 ? 1 : 2) void int4_tiles_kernel
       }
     }
     now = next;
-    if (kb + 1 < a.KB) keep_scales(kb + 1, now);
+    keep_scales(kb + 1, now);
+    const int free = stage;
+    stage = stage1, stage1 = stage2, stage2 = free;
   }
 
   const bool whole = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
@@ -529,12 +535,12 @@ __global__ __launch_bounds__(256, XDT == BRT_F32 ? 1 : 2) void int4_tiles_kernel
   else with_act(std::integral_constant<int, BRT_BF16>{});
 }
 
-template <int XDT, int GJ>
+template <int XDT, int GJ, int NT>
 int launch_tiles(Int4Args& a, hipStream_t st) {
-  constexpr int BM = 64, kBytes = 3 * BM * kB * elem_bytes(XDT) + 8 * BM * 4 + 4 * 2 * 8 * 64 * 4;
-  const auto fn = int4_tiles_kernel<XDT, GJ>;
+  constexpr int BM = 64, kBytes = 3 * BM * kB * elem_bytes(XDT) + 8 * BM * 4 + 4 * 2 * 8 * 16 * NT * 4;
+  const auto fn = int4_tiles_kernel<XDT, GJ, NT>;
   if (const int rc = allow_dynamic_lds(reinterpret_cast<const void*>(fn), kBytes); rc != BRT_OK) return rc;
-  a.tiles_n = (a.tiles + 15) / 16;
+  a.tiles_n = (a.tiles + 4 * NT - 1) / (4 * NT);
   // an expert adds at most one row block that it does not fill
   const long blocks = static_cast<long>(a.P) / BM + std::min(a.E, a.P);
   if (blocks * a.tiles_n >= (1l << 31) - kXcds) return fail(BRT_E_UNSUPPORTED, "too many tiles");
@@ -553,7 +559,7 @@ bool few_rows(const Int4Args& a, int x_dtype) {
 template <int XDT, int GJ>
 int launch(Int4Args& a, hipStream_t st) {
   if (few_rows(a, XDT)) return launch_few_rows<XDT, GJ>(a, st);
-  return launch_tiles<XDT, GJ>(a, st);
+  return launch_tiles<XDT, GJ, 4>(a, st);
 }
 template <int XDT>
 int launch(Int4Args& a, int group, hipStream_t st) {
