@@ -160,6 +160,13 @@ __global__ __launch_bounds__(W * 64) void int4_few_rows_kernel(Int4Args a) {
   if (at.rows == 0) return;
   const char* const row = row_of<XDT>(a, at.row0 + min(c16, at.rows - 1));
   const bool whole_rows = __ballot(row == nullptr) == 0;
+  // the biases of the tiles that this wavefront finishes, four lanes a row of a tile and four columns each: fetched ahead of the weights,
+  // not behind the last barrier
+  constexpr int kFinished = (NT + W - 1) / W;
+  const int r = lane >> 2, c4 = (lane & 3) * 4;
+  float bias[kFinished][4];
+#pragma unroll
+  for (int f = 0; f < kFinished; ++f) biases<4>(a, at.e, n0 + (wave + f * W) % NT * 16 + c4, bias[f]);
 
   f32x4 acc[NT];
 #pragma unroll
@@ -235,20 +242,18 @@ __global__ __launch_bounds__(W * 64) void int4_few_rows_kernel(Int4Args a) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) s_part[wave][j][g * 4 + q][c16] = acc[j][q];
   __syncthreads();
-  // four lanes a row of a tile, four columns each
   const bool whole = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
-  const int r = lane >> 2, c4 = (lane & 3) * 4;
-  for (int j = wave; j < NT; j += W) {
-    const int n = n0 + j * 16 + c4;
-    if (r >= at.rows || n >= a.N) continue;
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, bias[4];
-    biases<4>(a, at.e, n, bias);
+#pragma unroll
+  for (int f = 0; f < kFinished; ++f) {
+    const int j = wave + f * W, n = n0 + j * 16 + c4;
+    if (j >= NT || r >= at.rows || n >= a.N) continue;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < W; ++w)
 #pragma unroll
       for (int q = 0; q < 4; ++q) v[q] += s_part[w][j][r][c4 + q];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = activated_for(v[q] + bias[q], a.act, a.out_dtype);
+    for (int q = 0; q < 4; ++q) v[q] = activated_for(v[q] + bias[f][q], a.act, a.out_dtype);
     store_part<4>(a, static_cast<size_t>(at.row0) + r, n, whole, v);
   }
 }
@@ -261,14 +266,31 @@ int launch_few_rows(Int4Args& a, hipStream_t st) {
   hipLaunchKernelGGL((int4_few_rows_kernel<XDT, GJ, NT, W>), dim3(static_cast<unsigned>(blocks * a.tiles_n)), dim3(W * 64), 0, st, a);
   return check_launch("int4_few_rows_kernel");
 }
+// Tiles of 16 x 16 results: experts' last row blocks are taken as half full, and every expert to have rows where there are as many rows.
+long small_tiles(const Int4Args& a) {
+  const long used = std::min(a.E, a.P);
+  return (a.P > 8l * a.E ? std::max(used, a.P / 16 + used / 2) : used) * a.tiles;
+}
+// Columns of a workgroup and wavefronts that share its K, by the tiles that there are to deal out and the blocks of K.  Few tiles: as many
+// wavefronts as possible on each; many: more columns to a wavefront, which fetches the rows once for all of them (us, bf16 rows; 16
+// NT columns, W wavefronts).  1 row 2048 -> 8192: 2, 8 4.7, 1, 16 6.3, 4, 4 6.9; 1 row 8192 -> 1024: 1, 16 6.4, 2, 8 8.9; 128 rows of
+// 32 experts 1024 -> 4096: 4, 2 16.0, 2, 4 18.7, 4, 8 19.9, 1, 8 27; 128 of 32 4096 -> 1024: 4, 8 16.5, 4, 4 18.2, 4, 2 25.
 template <int XDT, int GJ>
 int launch_few_rows(Int4Args& a, hipStream_t st) {
-  const long tiles = (static_cast<long>(a.P) / 16 + std::min(a.E, a.P)) * a.tiles;
-  if (tiles < 384) return launch_few_rows<XDT, GJ, 1, 16>(a, st);
-  if (tiles < 1536) return launch_few_rows<XDT, GJ, 2, 8>(a, st);
-  if (a.KB >= 24) return launch_few_rows<XDT, GJ, 4, 8>(a, st);
-  if (tiles < 4096) return launch_few_rows<XDT, GJ, 2, 4>(a, st);
-  return launch_few_rows<XDT, GJ, 4, 4>(a, st);
+  const long tiles = small_tiles(a);
+  if (tiles < 384) {
+    if (a.KB >= 32 && tiles <= 256) return launch_few_rows<XDT, GJ, 1, 16>(a, st);
+    if (a.KB >= 8 || tiles < 128) return launch_few_rows<XDT, GJ, 1, 8>(a, st);
+    return launch_few_rows<XDT, GJ, 1, 4>(a, st);
+  }
+  if (tiles < 1280 || a.KB < 4) {
+    if (a.KB >= 8) return launch_few_rows<XDT, GJ, 2, 8>(a, st);
+    if (a.KB >= 4) return launch_few_rows<XDT, GJ, 2, 4>(a, st);
+    return launch_few_rows<XDT, GJ, 2, 2>(a, st);
+  }
+  if (a.KB >= 32 && tiles <= 2560) return launch_few_rows<XDT, GJ, 4, 8>(a, st);
+  if (a.KB >= 16 || a.KB <= 4 || tiles <= 4096) return launch_few_rows<XDT, GJ, 4, 4>(a, st);
+  return launch_few_rows<XDT, GJ, 4, 2>(a, st);
 }
 
 // Row blocks of all experts (blocks of 1 << bits rows; at most `most`, which the host has made the grid for).
@@ -289,7 +311,7 @@ __device__ __forceinline__ int count_blocks(const Int4Args& a, int bits, int mos
 // groups at a time, is a product of its own in fp32 (v_mfma_f32_16x16x4_f32): the vector units, which unpack and scale beside the matrix
 // units, have no part in it.
 template <int XDT, int GJ, int NT>
-__global__ __launch_bounds__(256, XDT == BRT_F32 ? 1 : 2) void int4_tiles_kernel(Int4Args a) {
+__global__ __launch_bounds__(256, 2) void int4_tiles_kernel(Int4Args a) {
   using Part = RowPart<XDT>;
   using W = decltype(weights_of<XDT>(0));
   constexpr int MT = 4, BM = 16 * MT, kGroups = 4 / GJ, kStages = 3;
@@ -357,7 +379,7 @@ __global__ __launch_bounds__(256, XDT == BRT_F32 ? 1 : 2) void int4_tiles_kernel
   const int left = a.tiles - 1 - min(tile0, a.tiles - 1);
   const uint8_t* const w0 = a.w + first * a.KB * 1024;
   const int s_bytes = a.s_dtype == BRT_F32 ? 4 : 2;
-  const uint32_t s_place = min(g, left) * a.G * 16 + c16;
+  const uint32_t s_place = min(min(g, NT - 1), left) * a.G * 16 + c16;
   const int s_extent = (min(NT - 1, left) + 1) * a.G * 16;
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<char*>(static_cast<const char*>(a.scales)) + first * a.G * 16 * s_bytes, 0, s_extent * s_bytes, 0x00020000);
@@ -550,16 +572,43 @@ int launch_tiles(Int4Args& a, hipStream_t st) {
   return check_launch("int4_tiles_kernel");
 }
 
-bool few_rows(const Int4Args& a, int x_dtype) {
+// Which kernel takes 16-bit rows, by what each is estimated to take (us): few rows, or 64 x 64, 64 x 128 and 64 x 256 tiles.  The
+// first fetches the weights again for every 16 rows, 5300 tiles of 16 x 16 x 128 a microsecond with the chip full; the others take a time per
+// block of 128 columns, waiting for loads while there is a workgroup to a CU at most, multiplying beyond: 64 rows 4096 -> 4096 9.6 and 27 / 35
+// / 46 us; 600 rows of 2 experts 4096 -> 4096 50 and 58 / 46 / 48; 1024 rows of 16 1024 -> 4096 32 and 33 / 26 / 24; 8192 of 64 2048 -> 2048
+// 187 and 185 / 125 / 100.  (The estimates of 202 shapes choose 5 % worse in the mean than the best of the kernels would be.)
+enum RowsKind { kFewRows, kTiles64, kTiles128, kTiles256 };
+RowsKind rows_kind(const Int4Args& a, int group, int x_dtype) {
   // (the tiles address 64 rows, or all cells, in 31 bits)
   const long row = static_cast<long>(a.K) * elem_bytes(x_dtype), reach = a.entries != nullptr ? a.T * row : 64 * row;
-  if (reach >= (1l << 31) - (1 << 16) || (a.entries != nullptr && a.T == 0)) return true;
-  return a.P <= 16 || a.P <= 16l * a.E;
+  if (reach >= (1l << 31) - (1 << 16) || (a.entries != nullptr && a.T == 0)) return kFewRows;
+  const double used = std::min(a.E, a.P), blocks = std::max(used, a.P / 64.0 + used / 2);
+  const double by_group = group == 32 ? 1.25 : group == 64 ? 1.1 : 1.0;
+  double least = 3.5 + static_cast<double>(small_tiles(a)) * a.KB / 5300;
+  RowsKind kind = kFewRows;
+  auto consider = [&](RowsKind of, int columns, double alone, double full) {
+    const double rounds = blocks * ((a.N + columns - 1) / columns) / (kXcds * kCusPerXcd);
+    const double time = 2.0 + a.KB * by_group * std::max(alone, full * rounds);
+    if (time < least) least = time, kind = of;
+  };
+  consider(kTiles64, 64, 0.84, 0.5);
+  consider(kTiles128, 128, 1.07, 0.69);
+  consider(kTiles256, 256, 1.43, 1.15);
+  return kind;
 }
+
+// (fp32 rows: the tiles would split them again in every wavefront; 4096 rows of 64 experts 2048 -> 2048 197 us, 64 x 256 tiles 283)
 template <int XDT, int GJ>
 int launch(Int4Args& a, hipStream_t st) {
-  if (few_rows(a, XDT)) return launch_few_rows<XDT, GJ>(a, st);
-  return launch_tiles<XDT, GJ, 4>(a, st);
+  if constexpr (XDT != BRT_F32) {
+    switch (rows_kind(a, 32 * GJ, XDT)) {
+      case kTiles64: return launch_tiles<XDT, GJ, 1>(a, st);
+      case kTiles128: return launch_tiles<XDT, GJ, 2>(a, st);
+      case kTiles256: return launch_tiles<XDT, GJ, 4>(a, st);
+      default: break;
+    }
+  }
+  return launch_few_rows<XDT, GJ>(a, st);
 }
 template <int XDT>
 int launch(Int4Args& a, int group, hipStream_t st) {
