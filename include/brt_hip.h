@@ -507,7 +507,7 @@ int brt_hip_combine_by_rows_grad(const void* grad, const void* rows, const float
  *     balance = E / (n * n * k) * sum_e counts[e] * sum_t p[t,e]        z = 1 / n * sum_t log(sum_e exp(scores[t,e]))^2,
  *   both zero where nothing counts.  Sums are fp32 within a workgroup and fp64 over them, in an order that the sizes fix.
  *   row_stats [T,2] (8-byte aligned) and coefficients [E+1] are what the gradient reads; NULL where none is wanted.  E <= 1024.
- *   Workspace of brt_hip_balance_loss_workspace_bytes(T, E) bytes (may be 0), 4-byte aligned, uninitialised, one per call in flight.
+ *   Workspace of brt_hip_balance_loss_workspace_bytes(T, E) bytes (may be 0), 16-byte aligned, uninitialised, one per call in flight.
  *
  * brt_hip_balance_loss_grad: grad_scores [T,E] (of dtype) from the gradients of the two losses (one fp32 value each on the device;
  *   NULL: zero): p * (c[e] - sum_i c[i] p[t,i] + q * log(sum exp)), c = grad_balance * E / (n * n * k) * counts, q = grad_z * 2 / n; zeros
