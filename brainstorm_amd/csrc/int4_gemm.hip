@@ -379,7 +379,7 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(Int4Args a) {
   const int left = a.tiles - 1 - min(tile0, a.tiles - 1);
   const uint8_t* const w0 = a.w + first * a.KB * 1024;
   const int s_bytes = a.s_dtype == BRT_F32 ? 4 : 2;
-  const uint32_t s_place = min(min(g, NT - 1), left) * a.G * 16 + c16;
+  const uint32_t s_place = min(g % NT, left) * a.G * 16 + c16;  // (lane l has column l % (16 NT))
   const int s_extent = (min(NT - 1, left) + 1) * a.G * 16;
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<char*>(static_cast<const char*>(a.scales)) + first * a.G * 16 * s_bytes, 0, s_extent * s_bytes, 0x00020000);
@@ -408,7 +408,7 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(Int4Args a) {
     scales_of(of.s, a.s_dtype, s);
 #pragma unroll
     for (int h = 0; h < kGroups; ++h) {
-      const int at = (kb * kGroups + h & 7) * 16 * NT + lane % (16 * NT);  // (lanes beyond hold what another one does)
+      const int at = (kb * kGroups + h & 7) * 16 * NT + lane % (16 * NT);
       s_scales[at] = s[h], s_zeros[at] = -(static_cast<float>(of.z[h]) + z_least) * s[h];
     }
   };
@@ -577,8 +577,9 @@ int launch_tiles(Int4Args& a, hipStream_t st) {
 // block of 128 columns, waiting for loads while there is a workgroup to a CU at most, multiplying beyond: 64 rows 4096 -> 4096 9.6 and 27 / 35
 // / 46 us; 600 rows of 2 experts 4096 -> 4096 50 and 58 / 46 / 48; 1024 rows of 16 1024 -> 4096 32 and 33 / 26 / 24; 8192 of 64 2048 -> 2048
 // 187 and 185 / 125 / 100.  (The estimates of 202 shapes choose 5 % worse in the mean than the best of the kernels would be.)
-enum RowsKind { kFewRows, kTiles64, kTiles128, kTiles256 };
+enum RowsKind { kFewRows = 16, kTiles64 = 64, kTiles128 = 128, kTiles256 = 256 };
 RowsKind rows_kind(const Int4Args& a, int group, int x_dtype) {
+  if (x_dtype == BRT_F32) return kFewRows;  // (the tiles would split them again in every wavefront: 4096 rows of 64 experts 2048 -> 2048 197 us, 283)
   // (the tiles address 64 rows, or all cells, in 31 bits)
   const long row = static_cast<long>(a.K) * elem_bytes(x_dtype), reach = a.entries != nullptr ? a.T * row : 64 * row;
   if (reach >= (1l << 31) - (1 << 16) || (a.entries != nullptr && a.T == 0)) return kFewRows;
@@ -597,7 +598,6 @@ RowsKind rows_kind(const Int4Args& a, int group, int x_dtype) {
   return kind;
 }
 
-// (fp32 rows: the tiles would split them again in every wavefront; 4096 rows of 64 experts 2048 -> 2048 197 us, 64 x 256 tiles 283)
 template <int XDT, int GJ>
 int launch(Int4Args& a, hipStream_t st) {
   if constexpr (XDT != BRT_F32) {
@@ -623,6 +623,15 @@ bool is_type(int dtype) { return dtype == BRT_F32 || dtype == BRT_F16 || dtype =
 }  // namespace brt
 
 using namespace brt;
+
+extern "C" int brt_hip_grouped_gemm_int4_kernel(int x_dtype, int T, int group, int E, int P, int N, int K) {
+  if (!is_type(x_dtype) || (group != 32 && group != 64 && group != 128) || E <= 0 || P <= 0 || N <= 0 || K <= 0) return BRT_E_INVALID;
+  Int4Args a{};
+  static const int kRoutes = 0;
+  a.entries = T >= 0 ? &kRoutes : nullptr;  // (whether there are any is all that is asked)
+  a.T = T; a.E = E; a.P = P; a.N = N; a.K = K; a.KB = (K + kB - 1) / kB; a.tiles = (N + 15) / 16;
+  return rows_kind(a, group, x_dtype);
+}
 
 extern "C" int brt_hip_grouped_gemm_int4(const void* x, int x_dtype, const int32_t* row_entries, int entries_per_cell, int T,
                                          const void* w, const void* scales, int scale_dtype, const uint8_t* zeros, int group,

@@ -58,7 +58,7 @@ def assert_losses(made, scores, ids, counted=None):
     want = in_64_bits(scores.detach().double(), ids, counted)
     assert counts.dtype == torch.int32 and torch.equal(counts, want[2])
     assert balance.dtype == z.dtype == torch.float32 and balance.shape == z.shape == ()
-    rows = cells if cells * paths <= 1 << 14 else -(-cells // min(256, -(-cells * paths >> 13)))
+    rows = cells if cells * paths <= 1 << 15 else -(-cells // min(256, -(-cells * paths >> 11)))
     steps = 3 * spread(scores) + 2.2 * paths + 8 + rows + 16
     assert abs(float(balance) - float(want[0])) <= (steps * U + U) * float(want[0])
     part = scores.detach().double() if counted is None else scores.detach().double()[counted]

@@ -191,6 +191,45 @@ def test_products(rows, k, n, experts, group, zeros, dtype):
     assert_near(got, want, size, group, k)
 
 
+KERNELS = [  # columns of the tiles that take these sizes; rows, in, out, experts, group
+    (16, 200, 264, 48, 4, 64), (16, 400, 328, 1100, 4, 64),
+    (64, 156, 136, 2100, 9, 64), (64, 200, 64, 100, 2, 128), (64, 586, 328, 1001, 5, 128), (64, 3615, 136, 100, 40, 32),
+    (128, 1420, 328, 1300, 9, 32), (128, 2043, 488, 1001, 20, 64), (128, 3485, 136, 600, 5, 128), (128, 4392, 488, 384, 128, 64),
+    (256, 642, 136, 2100, 40, 128), (256, 3144, 72, 1001, 40, 32), (256, 3347, 264, 1300, 2, 64), (256, 3585, 328, 1300, 3, 32),
+]
+
+
+def test_which_kernel_takes_the_shapes_below():
+    kernel = _lib.lib().brt_hip_grouped_gemm_int4_kernel
+    for columns, rows, k, n, experts, group in KERNELS:
+        assert kernel(2, -1, group, experts, rows, n, k) == kernel(1, rows, group, experts, rows, n, k) == columns, (columns, rows, k, n, experts, group)
+        assert kernel(0, -1, group, experts, rows, n, k) == 16
+    assert kernel(2, 0, 128, 8, 4096, 4096, 4096) == 16 and kernel(2, 1 << 20, 128, 8, 4096, 4096, 4096) == 16  # no cells; cells beyond 31 bits
+    assert kernel(2, -1, 48, 8, 4096, 4096, 4096) == kernel(3, -1, 64, 8, 4096, 4096, 4096) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("zeros,scales", [(False, "bf16"), (True, "f16"), (True, "f32")])
+@pytest.mark.parametrize("columns,rows,k,n,experts,group", KERNELS)
+def test_products_of_every_kernel(columns, rows, k, n, experts, group, zeros, scales, dtype):
+    """Ragged loads with empty experts, tails of K and N in every kernel, with and without row entries, 16-bit and fp32 results."""
+    dtype = TYPES[dtype]
+    w = Weights(rows + k, experts, n, k, group, zeros, scale_dtype=TYPES[scales])
+    x, loads, bias = normal(1, rows, k, dtype=dtype), loads_of(rows, rows, experts, empty=(1,) if experts > 2 else ()), normal(2, experts, n)
+    for out, activation in ((dtype, "gelu"), (torch.float32, "none")):
+        got = grouped_linear_int4(x.cuda(), w.cuda(), loads.cuda(), bias=bias.cuda(), activation=activation, out_dtype=out)
+        want, size = product_in_64(x, w, loads, bias, activation)
+        assert_near(got, want, size, group, k, gelu=activation == "gelu")
+    cells = rows // 2 + 1
+    entries = torch.randint(-1, 2 * cells + 2, (rows,), generator=torch.Generator().manual_seed(3)).int()
+    there = (entries >= 1) & (entries <= 2 * cells)
+    packed = torch.where(there[:, None], x[((entries.long() - 1) // 2).clamp(0, cells - 1)], 0)
+    want = grouped_linear_int4(packed.cuda(), w.cuda(), loads.cuda(), bias=bias.cuda())
+    got = grouped_linear_int4(x[:cells].cuda(), w.cuda(), loads.cuda(), bias=bias.cuda(), row_entries=entries.cuda(), entries_per_cell=2)
+    assert torch.equal(got, want)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("activation", ["none", "relu", "gelu"])
 @pytest.mark.parametrize("dtype,out,scales", [("bf16", "bf16", "f32"), ("bf16", "f32", "bf16"), ("f16", "bf16", "f16"), ("f32", "f16", "f32"), ("f32", "f32", "bf16")])
