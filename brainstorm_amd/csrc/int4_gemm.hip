@@ -132,6 +132,29 @@ __device__ __forceinline__ float activated_for(float v, int act, int out_dtype) 
   return act == BRT_ACT_GELU && out_dtype == BRT_F32 ? gelu_f32(v) : activated(v, act);
 }
 
+// Four results of a row, columns n .. n + 3 (n < N), rounded and stored.  Rows of any N begin at any element: the four leave in one store
+// all the same, which need not be aligned to more than an element.
+typedef u32x4 u32x4_at_4 __attribute__((aligned(4)));
+typedef u32x2 u32x2_at_2 __attribute__((aligned(2)));
+template <int OUT>
+__device__ __forceinline__ void store_four(const Int4Args& a, size_t row, int n, const float (&v)[4]) {
+  char* const to = static_cast<char*>(a.out) + (row * a.N + n) * elem_bytes(OUT);
+  if (n + 4 <= a.N) {
+    if constexpr (OUT == BRT_F32) {
+      *reinterpret_cast<u32x4_at_4*>(to) = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+    } else {
+      *reinterpret_cast<u32x2_at_2*>(to) = u32x2{float_to_half_bits<OUT>(v[0]) | float_to_half_bits<OUT>(v[1]) << 16,
+                                                 float_to_half_bits<OUT>(v[2]) | float_to_half_bits<OUT>(v[3]) << 16};
+    }
+    return;
+  }
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    const float one[1] = {v[q]};
+    if (n + q < a.N) pack_store<OUT, 1>(to + q * elem_bytes(OUT), one);
+  }
+}
+
 // Row `row` of the packed layout: its elements, or null where it stands for none (padding of a path: a row of zeros).
 template <int XDT>
 __device__ __forceinline__ const char* row_of(const Int4Args& a, int row) {
@@ -242,7 +265,6 @@ __global__ __launch_bounds__(W * 64) void int4_few_rows_kernel(Int4Args a) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) s_part[wave][j][g * 4 + q][c16] = acc[j][q];
   __syncthreads();
-  const bool whole = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
 #pragma unroll
   for (int f = 0; f < kFinished; ++f) {
     const int j = wave + f * W, n = n0 + j * 16 + c4;
@@ -254,7 +276,10 @@ __global__ __launch_bounds__(W * 64) void int4_few_rows_kernel(Int4Args a) {
       for (int q = 0; q < 4; ++q) v[q] += s_part[w][j][r][c4 + q];
 #pragma unroll
     for (int q = 0; q < 4; ++q) v[q] = activated_for(v[q] + bias[f][q], a.act, a.out_dtype);
-    store_part<4>(a, static_cast<size_t>(at.row0) + r, n, whole, v);
+    const size_t to = static_cast<size_t>(at.row0) + r;
+    if (a.out_dtype == BRT_F32) store_four<BRT_F32>(a, to, n, v);
+    else if (a.out_dtype == BRT_F16) store_four<BRT_F16>(a, to, n, v);
+    else store_four<BRT_BF16>(a, to, n, v);
   }
 }
 
@@ -520,7 +545,6 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(Int4Args a) {
     stage = stage1, stage1 = stage2, stage2 = free;
   }
 
-  const bool whole = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
   auto store = [&](auto act, auto out) {
     constexpr int ACT = decltype(act)::value, OUT = decltype(out)::value;
 #pragma unroll
@@ -533,17 +557,7 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(Int4Args a) {
         float v[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) v[q] = activated_for<ACT, OUT>(acc[i][j][q] + bias[q]);
-        char* const to = static_cast<char*>(a.out) + ((static_cast<size_t>(row0) + i * 16 + c16) * a.N + n) * elem_bytes(OUT);
-        if (i * 16 + c16 >= rows || n >= a.N) continue;
-        if (whole) {
-          pack_store<OUT, 4>(to, v);
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float one[1] = {v[q]};
-            if (n + q < a.N) pack_store<OUT, 1>(to + q * elem_bytes(OUT), one);
-          }
-        }
+        if (i * 16 + c16 < rows && n < a.N) store_four<OUT>(a, static_cast<size_t>(row0) + i * 16 + c16, n, v);
       }
     }
   };

@@ -90,10 +90,13 @@ __device__ __forceinline__ void biases(const A& a, int e, int n, float (&b)[COUN
     b[q] = a.bias != nullptr ? load_gate(a.bias, a.bias_dtype, static_cast<size_t>(e) * a.N + min(n + q, a.N - 1)) : 0.0f;
 }
 
-// COUNT results of one row, columns n .. n + COUNT - 1 (n < N), rounded and stored; `whole`: the row's pieces are aligned and N is a
-// multiple of COUNT.
+// COUNT results of one row, columns n .. n + COUNT - 1, biased, activated, rounded and stored; `whole`: the row's pieces are
+// aligned and N is a multiple of COUNT.
 template <int COUNT, typename A>
-__device__ __forceinline__ void store_part(const A& a, size_t row, int n, bool whole, const float (&v)[COUNT]) {
+__device__ __forceinline__ void finish(const A& a, size_t row, int n, bool whole, const float (&bias)[COUNT], float (&v)[COUNT]) {
+  if (n >= a.N) return;
+#pragma unroll
+  for (int q = 0; q < COUNT; ++q) v[q] = activated(v[q] + bias[q], a.act);
   const size_t at = row * a.N + n;
   if (whole) {
     if (a.out_dtype == BRT_F32) pack_store<BRT_F32, COUNT>(static_cast<float*>(a.out) + at, v);
@@ -108,13 +111,4 @@ __device__ __forceinline__ void store_part(const A& a, size_t row, int n, bool w
     else static_cast<uint16_t*>(a.out)[at + q] = static_cast<uint16_t>(a.out_dtype == BRT_F16 ? float_to_f16(v[q]) : float_to_bf16(v[q]));
   }
 }
-// ... biased and activated first
-template <int COUNT, typename A>
-__device__ __forceinline__ void finish(const A& a, size_t row, int n, bool whole, const float (&bias)[COUNT], float (&v)[COUNT]) {
-  if (n >= a.N) return;
-#pragma unroll
-  for (int q = 0; q < COUNT; ++q) v[q] = activated(v[q] + bias[q], a.act);
-  store_part<COUNT>(a, row, n, whole, v);
-}
-
 }  // namespace brt
