@@ -294,26 +294,25 @@ int launch_few_rows(Int4Args& a, hipStream_t st) {
 // Tiles of 16 x 16 results: experts' last row blocks are taken as half full, and every expert to have rows where there are as many rows.
 long small_tiles(const Int4Args& a) {
   const long used = std::min(a.E, a.P);
-  return (a.P > 8l * a.E ? std::max(used, a.P / 16 + used / 2) : used) * a.tiles;
+  return (a.P > 8l * a.E ? std::max(used, (a.P + 15l) / 16 + (a.E > 1 ? used / 2 : 0)) : used) * a.tiles;
 }
-// Columns of a workgroup and wavefronts that share its K, by the tiles that there are to deal out and the blocks of K.  Few tiles: as many
-// wavefronts as possible on each; many: more columns to a wavefront, which fetches the rows once for all of them (us, bf16 rows; 16
-// NT columns, W wavefronts).  1 row 2048 -> 8192: 2, 8 4.7, 1, 16 6.3, 4, 4 6.9; 1 row 8192 -> 1024: 1, 16 6.4, 2, 8 8.9; 128 rows of
-// 32 experts 1024 -> 4096: 4, 2 16.0, 2, 4 18.7, 4, 8 19.9, 1, 8 27; 128 of 32 4096 -> 1024: 4, 8 16.5, 4, 4 18.2, 4, 2 25.
+// Columns of a workgroup (16 NT) and wavefronts that share its K (W), by the tiles that there are to deal out and the blocks of K.  Few
+// tiles: as many wavefronts as possible on each; many: more columns to a wavefront, which fetches the rows once for all of them.  (us, bf16
+// rows; NT, W) 1 row 2048 -> 8192: 2, 8 4.7, 1, 16 6.3, 4, 4 6.9; 1 row 8192 -> 1024: 1, 16 6.4, 2, 8 8.9; 64 rows 4096 -> 4096: 4, 8 9.7, 2, 8
+// 12.4; 128 rows of 32 experts 1024 -> 4096: 4, 2 16.0, 2, 4 18.7, 4, 8 19.9, 1, 8 27; 128 of 32 4096 -> 1024: 4, 8 16.5, 4, 4 18.2, 4, 2 25.
 template <int XDT, int GJ>
 int launch_few_rows(Int4Args& a, hipStream_t st) {
   const long tiles = small_tiles(a);
   if (tiles < 384) {
     if (a.KB >= 32 && tiles <= 256) return launch_few_rows<XDT, GJ, 1, 16>(a, st);
-    if (a.KB >= 8 || tiles < 128) return launch_few_rows<XDT, GJ, 1, 8>(a, st);
-    return launch_few_rows<XDT, GJ, 1, 4>(a, st);
+    return launch_few_rows<XDT, GJ, 1, 8>(a, st);
   }
-  if (tiles < 1280 || a.KB < 4) {
+  if (tiles < 640 || a.KB < 4) {
     if (a.KB >= 8) return launch_few_rows<XDT, GJ, 2, 8>(a, st);
     if (a.KB >= 4) return launch_few_rows<XDT, GJ, 2, 4>(a, st);
     return launch_few_rows<XDT, GJ, 2, 2>(a, st);
   }
-  if (a.KB >= 32 && tiles <= 2560) return launch_few_rows<XDT, GJ, 4, 8>(a, st);
+  if (a.KB >= 8 && tiles <= 2048) return launch_few_rows<XDT, GJ, 4, 8>(a, st);
   if (a.KB >= 16 || a.KB <= 4 || tiles <= 4096) return launch_few_rows<XDT, GJ, 4, 4>(a, st);
   return launch_few_rows<XDT, GJ, 4, 2>(a, st);
 }
@@ -330,19 +329,25 @@ __device__ __forceinline__ int count_blocks(const Int4Args& a, int bits, int mos
   return blocks;
 }
 
-// Many rows per expert: 64 x 256 tiles, four wavefronts, 64 columns and all rows each: a weight is unpacked once a workgroup, and not held in
-// LDS.  Rows go straight into LDS, two blocks of 128 columns ahead, weights and scales into registers one block ahead.  The groups'
-// sums of x are made for the block ahead by a quarter of its rows a wavefront, and pass through LDS; -scale * zero times them, for four
-// groups at a time, is a product of its own in fp32 (v_mfma_f32_16x16x4_f32): the vector units, which unpack and scale beside the matrix
-// units, have no part in it.
+// Many rows per expert: tiles of 64 rows and 128 NT columns, eight wavefronts, 16 NT columns and all rows each: a weight is unpacked once a
+// workgroup, and not held in LDS.  Rows go straight into LDS, two blocks of 128 columns ahead, weights and scales into registers one block
+// ahead.  The groups' sums of x are made for the block ahead by half of the wavefronts, 16 rows each, and pass through LDS;
+// -scale * zero times them, for four groups at a time, is a product of its own in fp32 (v_mfma_f32_16x16x4_f32): the vector units, which
+// unpack and scale beside the matrix units, have no part in it.
+//   Two workgroups of 8 wavefronts fit a CU (125 registers, 66 KB), which hides the loads and the barrier: 64 x 256 tiles took four
+// wavefronts of twice the columns 76 us where these take 65 (4096 rows of 32 experts 1024 -> 4096), and as long as them where the matrix
+// units' power sets the time (16384 rows of 8 experts 4096 -> 4096, groups of 128: 575 us, 956 TFLOP/s).  There the products alone take
+// 357 us; without the unpacking and scaling the kernel takes as long as with them, without the loads 140 us less, without the sums and
+// their product 46 less (groups of 64, of which there are twice as many: 667 us in all).
+constexpr int kTileWaves = 8;
 template <int XDT, int GJ, int NT>
-__global__ __launch_bounds__(256, 2) void int4_tiles_kernel(Int4Args a) {
+__global__ __launch_bounds__(kTileWaves * 64, 2) void int4_tiles_kernel(Int4Args a) {
   using Part = RowPart<XDT>;
   using W = decltype(weights_of<XDT>(0));
   constexpr int MT = 4, BM = 16 * MT, kGroups = 4 / GJ, kStages = 3;
-  constexpr int kBits = 6;
+  constexpr int kBits = 6;  // log2 of BM
   constexpr int kRow = kB * elem_bytes(XDT), kChunks = kRow / 16, kRowsOfLoad = 64 / kChunks;  // of a row in LDS; rows of a load
-  constexpr int XL = BM / kRowsOfLoad / 4;  // loads of a wavefront and block
+  constexpr int XL = BM / kRowsOfLoad / kTileWaves;  // loads of a wavefront and block
   constexpr int kStage = BM * kRow;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   // of the last eight groups: the rows' sums, and a wavefront's scales and their products with the zero points
@@ -361,7 +366,7 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(Int4Args a) {
   const Block found = find_block(a, patch * kPatch + in % wide, kBits);
   if (found.rows == 0) return;
   const int e = __builtin_amdgcn_readfirstlane(found.e), row0 = __builtin_amdgcn_readfirstlane(found.row0), rows = __builtin_amdgcn_readfirstlane(found.rows);
-  const int tile0 = in / wide * (4 * NT) + wave * NT;
+  const int tile0 = in / wide * (kTileWaves * NT) + wave * NT;
 
   // Slot s of LDS row r holds chunk s ^ (r & 15) of that row: the 16 rows that are read together at one chunk cover all banks.
   const uint32_t row_bytes = static_cast<uint32_t>(a.K) * elem_bytes(XDT);
@@ -433,32 +438,26 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(Int4Args a) {
     scales_of(of.s, a.s_dtype, s);
 #pragma unroll
     for (int h = 0; h < kGroups; ++h) {
-      const int at = (kb * kGroups + h & 7) * 16 * NT + lane % (16 * NT);
+      const int at = ((kb * kGroups + h) & 7) * 16 * NT + lane % (16 * NT);
       s_scales[at] = s[h], s_zeros[at] = -(static_cast<float>(of.z[h]) + z_least) * s[h];
     }
   };
   // fragment p of 16 rows from row r0 of a stage
-  uint32_t part_at[4][Part::kUnits];
+  uint32_t part_at[4];
 #pragma unroll
-  for (int p = 0; p < 4; ++p)
-#pragma unroll
-    for (int u = 0; u < Part::kUnits; ++u) part_at[p][u] = c16 * kRow + (((p * 4 + g) * Part::kUnits + u) ^ c16) * 16;
-  auto part_of = [&](int stage, int r0, int p) {
-    u32x4 raw[Part::kUnits];
-#pragma unroll
-    for (int u = 0; u < Part::kUnits; ++u) raw[u] = *reinterpret_cast<const u32x4*>(smem + (part_at[p][u] + stage) + r0 * kRow);
-    return Part(raw);
-  };
+  for (int p = 0; p < 4; ++p) part_at[p] = c16 * kRow + ((p * 4 + g) ^ c16) * 16;
+  auto part_of = [&](int stage, int r0, int p) { return Part(reinterpret_cast<const u32x4*>(smem + (part_at[p] + stage) + r0 * kRow)); };
   W one;
 #pragma unroll
   for (int i = 0; i < 8; ++i) one[i] = 1.0f;
   auto sum_up = [&](int kb, int stage) {
+    if (wave >= MT) return;
 #pragma unroll
     for (int h = 0; h < kGroups; ++h) {
       f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int p = 0; p < GJ; ++p) sum = multiply(one, part_of(stage + wave * (BM / 4) * kRow, 0, h * GJ + p), sum);
-      s_sums[((kb * kGroups + h) & 7) * BM + wave * (BM / 4) + c16] = sum[0];  // (four lanes hold and write the same)
+      for (int p = 0; p < GJ; ++p) sum = multiply(one, part_of(stage, wave * 16, h * GJ + p), sum);
+      s_sums[((kb * kGroups + h) & 7) * BM + wave * 16 + c16] = sum[0];  // (four lanes hold and write the same)
     }
   };
 
@@ -481,7 +480,7 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(Int4Args a) {
     wait_loads_but<0>();
     __syncthreads();  // the block after this one has landed, its sums' place and the stage of the one before are free
     // groups four by four: their zero points come off when the last of them is at hand
-    const int group = (kb * kGroups & ~3) + g;
+    const int group = ((kb * kGroups) & ~3) + g;
     const bool correct = ((kb + 1) * kGroups & 3) == 0 || kb + 1 == a.KB;
     if (kb + 2 < a.KB) request(kb + 2, stage2);
     Loaded next;
@@ -510,7 +509,7 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(Int4Args a) {
       if (p % GJ == GJ - 1) {
         f32x4 s[NT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) s[j] = *reinterpret_cast<const f32x4*>(s_scales + (kb * kGroups + p / GJ & 7) * 16 * NT + j * 16 + g * 4);
+        for (int j = 0; j < NT; ++j) s[j] = *reinterpret_cast<const f32x4*>(s_scales + ((kb * kGroups + p / GJ) & 7) * 16 * NT + j * 16 + g * 4);
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -521,13 +520,6 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(Int4Args a) {
           }
       }
     }
-#ifdef SGB
-#pragma unroll
-    for (int m = 0; m < MT * NT * 4 * Part::kParts; ++m) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, SGB, 0);
-    }
-#endif
     if (correct) {
       float off[NT];
 #pragma unroll
@@ -573,42 +565,41 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(Int4Args a) {
 
 template <int XDT, int GJ, int NT>
 int launch_tiles(Int4Args& a, hipStream_t st) {
-  constexpr int BM = 64, kBytes = 3 * BM * kB * elem_bytes(XDT) + 8 * BM * 4 + 4 * 2 * 8 * 16 * NT * 4;
+  constexpr int BM = 64, kBytes = 3 * BM * kB * elem_bytes(XDT) + 8 * BM * 4 + kTileWaves * 2 * 8 * 16 * NT * 4;
   const auto fn = int4_tiles_kernel<XDT, GJ, NT>;
   if (const int rc = allow_dynamic_lds(reinterpret_cast<const void*>(fn), kBytes); rc != BRT_OK) return rc;
-  a.tiles_n = (a.tiles + 4 * NT - 1) / (4 * NT);
+  a.tiles_n = (a.tiles + kTileWaves * NT - 1) / (kTileWaves * NT);
   // an expert adds at most one row block that it does not fill
   const long blocks = static_cast<long>(a.P) / BM + std::min(a.E, a.P);
   if (blocks * a.tiles_n >= (1l << 31) - kXcds) return fail(BRT_E_UNSUPPORTED, "too many tiles");
   a.blocks = static_cast<int>(blocks);
   const long grid = (blocks * a.tiles_n + kXcds - 1) / kXcds * kXcds;
-  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(256), kBytes, st, a);
+  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(kTileWaves * 64), kBytes, st, a);
   return check_launch("int4_tiles_kernel");
 }
 
-// Which kernel takes 16-bit rows, by what each is estimated to take (us): few rows, or 64 x 64, 64 x 128 and 64 x 256 tiles.  The
-// first fetches the weights again for every 16 rows, 5300 tiles of 16 x 16 x 128 a microsecond with the chip full; the others take a time per
-// block of 128 columns, waiting for loads while there is a workgroup to a CU at most, multiplying beyond: 64 rows 4096 -> 4096 9.6 and 27 / 35
-// / 46 us; 600 rows of 2 experts 4096 -> 4096 50 and 58 / 46 / 48; 1024 rows of 16 1024 -> 4096 32 and 33 / 26 / 24; 8192 of 64 2048 -> 2048
-// 187 and 185 / 125 / 100.  (The estimates of 202 shapes choose 5 % worse in the mean than the best of the kernels would be.)
-enum RowsKind { kFewRows = 16, kTiles64 = 64, kTiles128 = 128, kTiles256 = 256 };
+// Which kernel takes 16-bit rows, by what each is estimated to take (us): few rows, or 64 x 128 and 64 x 256 tiles.  The first fetches the
+// weights again for every 16 rows, 5300 tiles of 16 x 16 x 128 a microsecond with the chip full; the others take a time per block of 128
+// columns, waiting for loads while there is a workgroup to a CU at most, multiplying beyond (us, groups of 128): 64 rows 4096 -> 4096
+// 9.7 and 33 / 43; 600 rows of 2 experts 4096 -> 4096 50 and 44 / 44; 1024 rows of 16 1024 -> 4096 32 and 24 / 23; 8192 of 64 2048 -> 2048 187
+// and 127 / 100.  (The estimates of 202 shapes choose 2 % worse in the mean than the best of the kernels would be.)
+enum RowsKind { kFewRows = 16, kTiles128 = 128, kTiles256 = 256 };
 RowsKind rows_kind(const Int4Args& a, int group, int x_dtype) {
   if (x_dtype == BRT_F32) return kFewRows;  // (the tiles would split them again in every wavefront: 4096 rows of 64 experts 2048 -> 2048 197 us, 283)
   // (the tiles address 64 rows, or all cells, in 31 bits)
-  const long row = static_cast<long>(a.K) * elem_bytes(x_dtype), reach = a.entries != nullptr ? a.T * row : 64 * row;
+  const long row = static_cast<long>(a.K) * elem_bytes(x_dtype), reach = std::max(64l, a.entries != nullptr ? a.T : 0l) * row;
   if (reach >= (1l << 31) - (1 << 16) || (a.entries != nullptr && a.T == 0)) return kFewRows;
   const double used = std::min(a.E, a.P), blocks = std::max(used, a.P / 64.0 + used / 2);
   const double by_group = group == 32 ? 1.25 : group == 64 ? 1.1 : 1.0;
-  double least = 3.5 + static_cast<double>(small_tiles(a)) * a.KB / 5300;
+  double least = 2.5 + static_cast<double>(small_tiles(a)) * a.KB / 5300;
   RowsKind kind = kFewRows;
   auto consider = [&](RowsKind of, int columns, double alone, double full) {
     const double rounds = blocks * ((a.N + columns - 1) / columns) / (kXcds * kCusPerXcd);
     const double time = 2.0 + a.KB * by_group * std::max(alone, full * rounds);
     if (time < least) least = time, kind = of;
   };
-  consider(kTiles64, 64, 0.84, 0.5);
-  consider(kTiles128, 128, 1.07, 0.69);
-  consider(kTiles256, 256, 1.43, 1.15);
+  consider(kTiles128, 128, 0.87, 0.69);
+  consider(kTiles256, 256, 1.36, 1.15);
   return kind;
 }
 
@@ -616,9 +607,8 @@ template <int XDT, int GJ>
 int launch(Int4Args& a, hipStream_t st) {
   if constexpr (XDT != BRT_F32) {
     switch (rows_kind(a, 32 * GJ, XDT)) {
-      case kTiles64: return launch_tiles<XDT, GJ, 1>(a, st);
-      case kTiles128: return launch_tiles<XDT, GJ, 2>(a, st);
-      case kTiles256: return launch_tiles<XDT, GJ, 4>(a, st);
+      case kTiles128: return launch_tiles<XDT, GJ, 1>(a, st);
+      case kTiles256: return launch_tiles<XDT, GJ, 2>(a, st);
       default: break;
     }
   }
