@@ -23,6 +23,7 @@ namespace {
 
 constexpr int kB = 128;              // columns of a block of the weights' layout
 constexpr int kMostRows = 1 << 24;   // 65 times as many are added up in 32 bits
+constexpr long kMostThreads = 1l << 32;  // of a launch
 constexpr int kMostColumns = 1 << 28;  // and experts and elements of a row: rounded up to tiles they are counted in 32 bits
 
 struct Int4Args {
@@ -287,7 +288,7 @@ template <int XDT, int GJ, int NT, int W>
 int launch_few_rows(Int4Args& a, hipStream_t st) {
   const long blocks = static_cast<long>(a.P) / 16 + std::min(a.E, a.P);
   a.tiles_n = (a.tiles + NT - 1) / NT;
-  if (blocks * a.tiles_n >= (1l << 31)) return fail(BRT_E_UNSUPPORTED, "too many tiles");
+  if (blocks * a.tiles_n * (W * 64) >= kMostThreads) return fail(BRT_E_UNSUPPORTED, "too many tiles");
   hipLaunchKernelGGL((int4_few_rows_kernel<XDT, GJ, NT, W>), dim3(static_cast<unsigned>(blocks * a.tiles_n)), dim3(W * 64), 0, st, a);
   return check_launch("int4_few_rows_kernel");
 }
@@ -567,13 +568,12 @@ template <int XDT, int GJ, int NT>
 int launch_tiles(Int4Args& a, hipStream_t st) {
   constexpr int BM = 64, kBytes = 3 * BM * kB * elem_bytes(XDT) + 8 * BM * 4 + kTileWaves * 2 * 8 * 16 * NT * 4;
   const auto fn = int4_tiles_kernel<XDT, GJ, NT>;
-  if (const int rc = allow_dynamic_lds(reinterpret_cast<const void*>(fn), kBytes); rc != BRT_OK) return rc;
   a.tiles_n = (a.tiles + kTileWaves * NT - 1) / (kTileWaves * NT);
   // an expert adds at most one row block that it does not fill
-  const long blocks = static_cast<long>(a.P) / BM + std::min(a.E, a.P);
-  if (blocks * a.tiles_n >= (1l << 31) - kXcds) return fail(BRT_E_UNSUPPORTED, "too many tiles");
+  const long blocks = static_cast<long>(a.P) / BM + std::min(a.E, a.P), grid = (blocks * a.tiles_n + kXcds - 1) / kXcds * kXcds;
+  if (grid * (kTileWaves * 64) >= kMostThreads) return fail(BRT_E_UNSUPPORTED, "too many tiles");
   a.blocks = static_cast<int>(blocks);
-  const long grid = (blocks * a.tiles_n + kXcds - 1) / kXcds * kXcds;
+  if (const int rc = allow_dynamic_lds(reinterpret_cast<const void*>(fn), kBytes); rc != BRT_OK) return rc;
   hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(kTileWaves * 64), kBytes, st, a);
   return check_launch("int4_tiles_kernel");
 }

@@ -100,11 +100,11 @@ def quantize_int4(weight: torch.Tensor, group: int = 128, *, zeros: bool = False
         high = parts.amax(2).clamp(min=0.0) if columns else low
         scales[e] = ((high - low) / 15.0 if zeros else torch.maximum(high, -low) / 7.0).to(scale_dtype)
         scale = scales[e].float()
-        inverse = torch.where(scale == 0.0, 0.0, 1.0 / scale)
-        zero = (-low * inverse).round().clamp(0, 15) if zeros else torch.full_like(scale, 8.0)
+        by = torch.where(scale == 0.0, 1.0, scale)
+        zero = torch.where(scale == 0.0, 0.0, (-low / by).round().clamp(0, 15)) if zeros else torch.full_like(scale, 8.0)
         if zeros:
             points[e] = zero.to(torch.uint8)
-        q = ((parts * inverse[:, :, None]).round() + zero[:, :, None]).clamp(0, 15).to(torch.uint8)
+        q = ((parts / by[:, :, None]).round() + zero[:, :, None]).clamp(0, 15).to(torch.uint8)
         _packed_values(q.view(rows, -1)[:, :columns], packed[e])
     tiles = packed.shape[1]
     return Int4Weight(packed, _packed_groups(scales, tiles), None if points is None else _packed_groups(points, tiles), columns, rows, group)

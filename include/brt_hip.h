@@ -570,7 +570,7 @@ int brt_hip_grouped_gemm_int4(const void* x, int x_dtype, const int32_t* row_ent
                               const int32_t* loads, const void* bias, int bias_dtype, void* out, int out_dtype, int E,
                               int P, int N, int K, int activation, void* stream);
 /* The rows or columns of the tiles of the kernel that takes these sizes (T: cells that the rows are gathered from, -1: none; for tests and
- * measurements): 16 the one for few rows, 64, 128 or 256 the columns of the others' tiles; or BRT_E_INVALID. */
+ * measurements): 16 the one for few rows, 128 or 256 the columns of the others' tiles; or BRT_E_INVALID. */
 int brt_hip_grouped_gemm_int4_kernel(int x_dtype, int T, int group, int E, int P, int N, int K);
 
 /*

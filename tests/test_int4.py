@@ -151,6 +151,17 @@ def test_quantized_weights(experts, n, k, group, zeros, dtype):
         assert abs(float(unpacked(again)[0, 2, 0]) - 1.0) <= 1e-6
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantized_weights_whose_reciprocal_scale_overflows(zeros):
+    """A scale below 2^-128 has no reciprocal in fp32; weights and scale are steps of 2^-149 there."""
+    weight = torch.tensor([[[0.0, 1e-39, -3e-39, 7e-40, 0.0, 2e-39, -1e-39, 3e-39]]])
+    packed = quantize_int4(weight, 32, zeros=zeros)
+    step = float(packed.scales.max())
+    assert 0 < step < 2.0 ** -128
+    assert bool(((unpacked(packed) - weight.double()).abs() <= 1.01 * step).all())
+    assert not unpacked(packed)[0, 0, [0, 4]].any()
+
+
 def test_refusals_of_the_layout():
     q, s = torch.zeros(2, 16, 64, dtype=torch.uint8), torch.ones(2, 16, 1)
     for call, error, words in (
@@ -437,6 +448,54 @@ def test_a_served_layer_on_a_stream_and_replayed(tokens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,paths", [(40, 4), (3000, 16)])
+def test_a_layer_is_trained_and_then_served_in_four_bits(tokens, paths):
+    """A step with the losses (gradients of cells, scores and experts against torch in 64 bits), its experts in 4 bits then, for the same route."""
+    d, d_ff, k = 64, 96, 2
+    x, scores = normal(1, tokens, d, scale=0.5).cuda().requires_grad_(), normal(2, tokens, paths).cuda().requires_grad_()
+    w1, w2 = normal(3, paths, d_ff, d, scale=d ** -0.5).cuda().requires_grad_(), normal(4, paths, d, d_ff, scale=d_ff ** -0.5).cuda().requires_grad_()
+    grad, leaves = normal(5, tokens, d).cuda(), [x, scores, w1, w2]
+    ids, weights = c_router.gate_topk(scores, k, softmax=True, differentiable=True)
+    balance, z, counts = c_router.balance_loss(scores, ids)
+    loads, _, seat_rows, entries = c_router.route_by_path(ids, paths)
+    assert torch.equal(loads, counts)
+    rows = c_router.dispatch_by_rows(x, entries, k, seat_rows=seat_rows)
+    parts = [torch.nn.functional.gelu(part @ w1[e].t()) @ w2[e].t() for e, part in enumerate(rows.split(loads.tolist()))]
+    out = c_router.combine_by_rows(torch.cat(parts), ids, seat_rows, weights, row_entries=entries)
+    made = torch.autograd.grad([out, balance, z], leaves, [grad, torch.tensor(0.5, device="cuda"), torch.tensor(0.1, device="cuda")])
+
+    x64, s64, w164, w264 = (t.detach().cpu().double().requires_grad_() for t in leaves)
+    chosen, p = ids.cpu().long(), torch.softmax(s64, 1)
+    want = torch.zeros(tokens, d, dtype=torch.float64)
+    for e in range(paths):
+        share = (p * torch.nn.functional.one_hot(chosen, paths).sum(1))[:, e:e + 1]
+        want = want + share * (torch.nn.functional.gelu(x64 @ w164[e].t()) @ w264[e].t())
+    balance64 = paths / (tokens * tokens * k) * (counts.cpu() * p.sum(0)).sum()
+    z64 = torch.logsumexp(s64, 1).square().mean()
+    wants = torch.autograd.grad((want * grad.cpu()).sum() + 0.5 * balance64 + 0.1 * z64, [x64, s64, w164, w264])
+    # fp32 throughout: products of at most 3000 terms, each sum off by less than 1e-5 of its magnitudes
+    for got, exact in zip([out.detach(), balance.detach(), z.detach(), *made], [want.detach(), balance64.detach(), z64.detach(), *wants]):
+        assert float((got.cpu().double() - exact).norm()) <= 1e-5 * float(exact.norm())
+
+    served1, served2 = quantize_int4(w1, 32, zeros=True), quantize_int4(w2, 32)
+    with torch.no_grad():
+        ids4, weights4 = c_router.gate_topk(scores, k, softmax=True)
+        balance4, z4, counts4 = c_router.balance_loss(scores, ids4)
+        loads4, _, seat_rows4, entries4 = c_router.route_by_path(ids4, paths)
+        hidden = grouped_linear_int4(x, served1, loads4, activation="gelu", row_entries=entries4, entries_per_cell=k)
+        got = c_router.combine_by_rows(grouped_linear_int4(hidden, served2, loads4), ids4, seat_rows4, weights4)
+    assert torch.equal(ids4, ids) and torch.equal(counts4, counts) and torch.equal(balance4, balance) and torch.equal(z4, z)
+    v1, v2 = unpacked(Int4Weight(*(t.cpu() if torch.is_tensor(t) else t for t in served1))), unpacked(Int4Weight(*(t.cpu() if torch.is_tensor(t) else t for t in served2)))
+    want4 = torch.zeros(tokens, d, dtype=torch.float64)
+    for e in range(paths):
+        share = (p.detach() * torch.nn.functional.one_hot(chosen, paths).sum(1))[:, e:e + 1]
+        want4 += share * (torch.nn.functional.gelu(x64.detach() @ v1[e].t()) @ v2[e].t())
+    assert float((got.cpu().double() - want4).norm()) <= 1e-5 * float(want4.norm())
+    # what 4 bits are worth: a step of 2/15 to 2/7 of a group's range, half of it off at most
+    assert float((want4 - want.detach()).norm()) <= 0.25 * float(want.detach().norm())
+
+
+@pytest.mark.gpu
 def test_refusals():
     w, loads = Weights(1, 2, 20, 64, 32, zeros=True).cuda(), torch.tensor([2, 3], dtype=torch.int32, device="cuda")
     x, bias = normal(2, 5, 64, dtype=torch.bfloat16).cuda(), normal(3, 2, 20).cuda()
@@ -486,5 +545,5 @@ def test_argument_errors_of_the_library_need_no_gpu():
         assert code(**change) == -1, change
     for change in ({"group": 16}, {"x_dtype": 3}, {"out_dtype": 5}, {"s_dtype": -1}, {"bias": some, "bias_dtype": 9}, {"act": 4}, {"K": 0}, {"K": 60}, {"x": 24},
                    {"w": 24}, {"scales": 24}, {"zeros": 18}, {"P": 1 << 24}, {"N": (1 << 28) + 1}, {"K": (1 << 28) + 8}, {"E": (1 << 28) + 1},
-                   {"P": (1 << 24) - 1, "N": 1 << 28, "E": 1 << 28}):
+                   {"P": (1 << 24) - 1, "N": 1 << 28, "E": 1 << 28}, {"P": (1 << 24) - 1, "N": 1 << 20}, {"x_dtype": 0, "P": (1 << 24) - 1, "N": 2048}):
         assert code(**change) == -4, change
