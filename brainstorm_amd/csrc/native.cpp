@@ -1209,6 +1209,8 @@ PyObject* grouped_linear_int4(const Args& a) {
     if (out.sizes() != at::IntArrayRef({P, N}) || !out.is_contiguous()) runtime_error("out must be a contiguous [rows, out_features] tensor");
     for (const Tensor* t : std::initializer_list<const Tensor*>{&x, &w, &w_scales, &w_zeros, &loads_given, &bias_given, &entries_given})
       if (t->defined() && shares_memory(out, *t)) runtime_error("out shares memory with an operand");
+    if (tracked(out)) runtime_error("out carries gradients");
+    if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();  // (a graph that has kept it must not use it)
   } else {
     out = empty({P, N}, type, x);
   }

@@ -525,9 +525,18 @@ def test_refusals():
             (lambda: grouped_linear_int4(x, w, loads, row_entries=entries, entries_per_cell=0), RuntimeError, "at least one"),
             (lambda: grouped_linear_int4(x, w, loads, out=room[:4]), RuntimeError, "contiguous"),
             (lambda: grouped_linear_int4(x, w, loads, out=room, out_dtype=torch.float32), RuntimeError, "says its type"),
-            (lambda: grouped_linear_int4(x, w, loads, out=x.view(-1)[:100].view(5, 20)), RuntimeError, "shares memory")):
+            (lambda: grouped_linear_int4(x, w, loads, out=x.view(-1)[:100].view(5, 20)), RuntimeError, "shares memory"),
+            (lambda: grouped_linear_int4(x, w, loads, out=room.clone().requires_grad_()), RuntimeError, "carries gradients")):
         with pytest.raises(error, match=words):
             call()
+    leaf = torch.ones_like(room, requires_grad=True)
+    product = leaf * room
+    grouped_linear_int4(x, w, loads, out=room)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+    with torch.inference_mode():
+        made = torch.zeros_like(room)
+        assert torch.equal(grouped_linear_int4(x, w, loads, out=made), room)
 
 
 def test_argument_errors_of_the_library_need_no_gpu():
