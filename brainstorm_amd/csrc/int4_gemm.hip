@@ -172,7 +172,7 @@ __device__ __forceinline__ const char* row_of(const Int4Args& a, int row) {
 // wavefronts take blocks of 128 columns in turn, weights and rows straight into the fragments' registers, and add up their sums through
 // LDS.  The rows are the first operand here: a lane holds results of one column, whose scale and zero point are one register each.
 //   256 rows of 64 experts 4096 -> 1024 30.1 us, 139 MB at 4.6 TB/s (a large copy's rate is 5.2): memory.  1 row 2048 -> 8192 4.5 us and 48
-// rows of 8 experts 1024 -> 4096 8.1 us, of which the bytes take 1.7 and 3.6: a launch, the loads and two dependent rounds of requests.
+// rows of 8 experts 1024 -> 4096 7.4 us, of which the bytes take 1.7 and 3.6: a launch, the loads and two dependent rounds of requests.
 // Two blocks of a wavefront in flight instead of one, or two and four row blocks a workgroup, which share the weights, gained nothing.
 //   fp32 rows: 333 rows of 12 experts 776 -> 1001, groups of 32, 12.1 us: two rounds of requests as well, the rows' splitting
 // (over again for every 16 NT columns) and three products in place of one between them; vector units 0.22 of the time, matrix units 0.06.
@@ -305,7 +305,8 @@ long small_tiles(const Int4Args& a) {
 // Columns of a workgroup (16 NT) and wavefronts that share its K (W), by the tiles that there are to deal out and the blocks of K.  Few
 // tiles: as many wavefronts as possible on each; many: more columns to a wavefront, which fetches the rows once for all of them.  (us, bf16
 // rows; NT, W) 1 row 2048 -> 8192: 2, 8 4.7, 1, 16 6.3, 4, 4 6.9; 1 row 8192 -> 1024: 1, 16 6.4, 2, 8 8.9; 64 rows 4096 -> 4096: 4, 8 9.7, 2, 8
-// 12.4; 128 rows of 32 experts 1024 -> 4096: 4, 2 16.0, 2, 4 18.7, 4, 8 19.9, 1, 8 27; 128 of 32 4096 -> 1024: 4, 8 16.5, 4, 4 18.2, 4, 2 25.
+// 12.4; 4 rows of 4 experts 4096 -> 4096: 2, 8 8.9, 4, 8 9.7; 48 rows of 8 1024 -> 4096: 2, 4 7.4, 4, 8 8.1, 2, 8 8.3; 128 rows of 32
+// 1024 -> 4096: 4, 2 16.0, 2, 4 18.7, 4, 8 19.9, 1, 8 27; 128 of 32 4096 -> 1024: 4, 8 16.5, 4, 4 18.2, 4, 2 25.
 template <int XDT, int GJ>
 int launch_few_rows(Int4Args& a, hipStream_t st) {
   const long tiles = small_tiles(a);
@@ -313,8 +314,10 @@ int launch_few_rows(Int4Args& a, hipStream_t st) {
     if (a.KB >= 32 && tiles <= 256) return launch_few_rows<XDT, GJ, 1, 16>(a, st);
     return launch_few_rows<XDT, GJ, 1, 8>(a, st);
   }
-  if (tiles < 640 || a.KB < 4) {
-    if (a.KB >= 8) return launch_few_rows<XDT, GJ, 2, 8>(a, st);
+  // (about one row block to an expert: no other workgroup reads its weights)
+  const bool alone = a.P <= 8l * a.E && (tiles <= 1024 || (tiles <= 2048 && a.KB < 32));
+  if (tiles < 640 || a.KB < 4 || alone) {
+    if (a.KB >= 8 && tiles <= 1024) return launch_few_rows<XDT, GJ, 2, 8>(a, st);
     if (a.KB >= 4) return launch_few_rows<XDT, GJ, 2, 4>(a, st);
     return launch_few_rows<XDT, GJ, 2, 2>(a, st);
   }

@@ -205,7 +205,7 @@ def test_products(rows, k, n, experts, group, zeros, dtype):
 KERNELS = [  # columns of the tiles that take these sizes; rows, in, out, experts, group
     (16, 200, 264, 48, 4, 64), (16, 400, 328, 1100, 4, 64), (16, 156, 136, 2100, 9, 64), (16, 200, 64, 100, 2, 128), (16, 586, 328, 1001, 5, 128),
     (16, 3615, 136, 100, 40, 32), (16, 5, 4104, 100, 2, 128), (16, 8, 1032, 1001, 8, 64), (16, 8, 520, 1001, 8, 32), (16, 40, 1096, 1300, 16, 128),
-    (16, 40, 600, 1300, 16, 64), (16, 60, 904, 2100, 40, 32),
+    (16, 40, 600, 1300, 16, 64), (16, 60, 904, 2100, 40, 32), (16, 100, 1096, 1300, 4, 128), (16, 100, 600, 1300, 4, 64),
     (128, 1420, 328, 1300, 9, 32), (128, 2043, 488, 1001, 20, 64), (128, 3485, 136, 600, 5, 128), (128, 4392, 488, 384, 128, 64),
     (256, 642, 136, 2100, 40, 128), (256, 3144, 72, 1001, 40, 32), (256, 3347, 264, 1300, 2, 64), (256, 3585, 328, 1300, 3, 32),
 ]
