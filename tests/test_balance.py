@@ -340,6 +340,51 @@ def test_a_step_on_a_stream_and_two_graphs_replayed_in_turn():
 
 
 @pytest.mark.gpu
+def test_scores_beyond_four_gib():
+    """2^31 - 64 fp32 scores: the last rows and their gradient lie past 2^33 bytes."""
+    paths = 64
+    cells = (1 << 31) // paths - 1
+    scores = torch.zeros(cells, paths, device="cuda")
+    scores[-40:] = normal(1, 40, paths)
+    ids = torch.zeros(cells, 1, dtype=torch.int32, device="cuda")
+    ids[-40:] = some_ids(2, 40, paths, 1)
+    scores.requires_grad_()
+    balance, z, counts = c_router.balance_loss(scores, ids)
+    (got,) = torch.autograd.grad([balance, z], scores, [torch.tensor(1e9, device="cuda"), torch.tensor(1e9, device="cuda")])
+    assert torch.equal(counts, torch.bincount(ids.view(-1), minlength=paths).int())
+    s = torch.cat([scores.detach()[:1], scores.detach()[-40:]]).double()
+    p, lse, c = torch.softmax(s, 1), torch.logsumexp(s, 1, keepdim=True), paths / cells ** 2 * counts.double()
+    share = (cells - 40) * p[:1].sum(0) + p[1:].sum(0)
+    squares = (cells - 40) * float(lse[0] ** 2) + float((lse[1:] ** 2).sum())
+    # a workgroup's 131072 rows are added up in fp32, 2048 of them one behind the other in a lane; the other terms as above
+    off = (2048 + 3 * spread(s) + 2 * 2.2 * paths + 40) * U
+    assert abs(float(balance.detach()) - float((c * share).sum())) <= off * float((c * share).sum())
+    assert abs(float(z.detach()) - squares / cells) <= off * squares / cells
+    for at, row in ((0, 0), (cells // 2, 0), (cells - 41, 0), *((cells - 40 + i, 1 + i) for i in range(40))):
+        want = 1e9 * p[row] * (c - (c * p[row]).sum() + 2 / cells * lse[row])
+        size = 1e9 * p[row] * (c + (c * p[row]).sum() + 2 / cells * lse[row])
+        assert bool(((got[at].double() - want).abs() <= (3 * spread(s) + 2.2 * paths + 20) * 4 * U * size).all()), at
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once():
+    def step(scores, ids):
+        balance, z, counts = c_router.balance_loss(scores, ids)
+        return [balance.detach(), z.detach(), counts, *torch.autograd.grad(balance + z, scores)]
+
+    inputs = [(normal(i, 20000, 64).requires_grad_(), some_ids(10 + i, 20000, 64, 2)) for i in range(2)]
+    want = [step(*these) for these in inputs]
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(step(*inputs[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i in range(2) for made in got[i] for a, b in zip(made, want[i]))
+
+
+@pytest.mark.gpu
 def test_refusals():
     scores, ids = normal(1, 20, 8), some_ids(2, 20, 8, 2)
     mask = torch.ones(20, dtype=torch.bool, device="cuda")

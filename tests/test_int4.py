@@ -448,6 +448,23 @@ def test_a_served_layer_on_a_stream_and_replayed(tokens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [20, 2000])
+def test_two_calls_at_once(rows):
+    w = [Weights(i, 4, 512, 512, 64, zeros=True).cuda() for i in range(2)]
+    x = [normal(i, rows, 512, dtype=torch.bfloat16).cuda() for i in range(2)]
+    loads = [loads_of(i, rows, 4).cuda() for i in range(2)]
+    want = [grouped_linear_int4(x[i], w[i], loads[i]) for i in range(2)]
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(grouped_linear_int4(x[i], w[i], loads[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(made, want[i]) for i in range(2) for made in got[i])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("tokens,paths", [(40, 4), (3000, 16)])
 def test_a_layer_is_trained_and_then_served_in_four_bits(tokens, paths):
     """A step with the losses (gradients of cells, scores and experts against torch in 64 bits), its experts in 4 bits then, for the same route."""
