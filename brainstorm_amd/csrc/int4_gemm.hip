@@ -353,6 +353,7 @@ template <int XDT, int GJ, int NT>
 __global__ __launch_bounds__(kTileWaves * 64, 2) void int4_tiles_kernel(Int4Args a) {
   using Part = RowPart<XDT>;
   using W = decltype(weights_of<XDT>(0));
+  static_assert(elem_bytes(XDT) == 2, "a chunk of 16 bytes is a lane's part of a fragment");
   constexpr int MT = 4, BM = 16 * MT, kGroups = 4 / GJ, kStages = 3;
   constexpr int kBits = 6;  // log2 of BM
   constexpr int kRow = kB * elem_bytes(XDT), kChunks = kRow / 16, kRowsOfLoad = 64 / kChunks;  // of a row in LDS; rows of a load

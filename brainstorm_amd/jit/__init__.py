@@ -113,7 +113,7 @@ def grouped_linear_int4(x: torch.Tensor, weight: Int4Weight, loads: torch.Tensor
     cell-major and row r is its cell ``(row_entries[r] - 1) // k``: no dispatch is needed.  A row without an entry is a row of zeros.
 
     The result has ``x``'s type (or ``out_dtype``); a given ``out`` is filled in place (contiguous ``[rows, out_features]``, memory of its
-    own: it is written while the operands are read).  Rows behind the last expert's are not written.  A row that holds NaN or an infinity
+    own, without gradients: it is written while the operands are read).  Rows behind the last expert's are not written.  A row that holds NaN or an infinity
     (or fp32 from 3.39e38 on, which bf16 cannot hold) gives NaN.  Results are cut off from autograd, as those of :func:`grouped_linear`."""
     return _lib.native().grouped_linear_int4(x, weight.values, weight.scales, weight.zeros, weight.in_features, weight.out_features,
                                              weight.group, loads, bias, _ACT[activation], out, out_dtype, row_entries, int(entries_per_cell))
