@@ -384,7 +384,6 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void int4_tiles_kernel(Int4Args
   i32x4 rx;
   if (a.entries != nullptr) rx = make_rsrc(a.x, static_cast<size_t>(a.T) * row_bytes);
   else rx = make_rsrc(static_cast<const char*>(a.x) + static_cast<size_t>(row0) * row_bytes, static_cast<size_t>(rows) * row_bytes);
-  asm volatile("s_nop 4" : "+s"(rx));  // (a scalar that a vector unit wrote is read five states later, which no one counts for inline assembly)
   uint32_t from[XL], chunk_at[XL];
 #pragma unroll
   for (int i = 0; i < XL; ++i) {

@@ -13,6 +13,8 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr int kXcds = 8, kCusPerXcd = 32;
 constexpr uint32_t kNowhere = 0x7ffffff0u;  // an offset past every extent: reads as zero, costs no request
 
+// The descriptor of a buffer for the loads below.  A scalar that a vector unit wrote, as these are where the compiler cannot tell that
+// they are the same in all lanes, may be read by a load five wait states later, which no one counts for inline assembly: they pass here.
 __device__ __forceinline__ i32x4 make_rsrc(const void* p, size_t bytes) {
   const uint64_t a = reinterpret_cast<uint64_t>(p);
   i32x4 r;
@@ -20,6 +22,7 @@ __device__ __forceinline__ i32x4 make_rsrc(const void* p, size_t bytes) {
   r[1] = __builtin_amdgcn_readfirstlane(static_cast<int>((a >> 32) & 0xffff));
   r[2] = __builtin_amdgcn_readfirstlane(static_cast<int>(bytes));
   r[3] = 0x00020000;
+  asm volatile("s_nop 4" : "+s"(r));
   return r;
 }
 // 16 bytes per lane from the buffer into LDS at lds_base + 16 * lane (M0; one wait state between its write and the load).  The
