@@ -54,16 +54,16 @@ __device__ __forceinline__ i32x4 make_rsrc(const void* p, size_t bytes) {
   return r;
 }
 
-// 16 / 4 bytes per lane from the buffer straight into LDS at lds_base + 16 (4) * lane; every wait for
-// such a load is written out below
+// 16 / 4 bytes per lane from the buffer straight into LDS at lds_base + 16 (4) * lane (M0; one wait state between its write and
+// the load); every wait for such a load is written out below
 __device__ __forceinline__ void load_to_lds(const i32x4& rsrc, uint32_t voffset, uint32_t soffset, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(__builtin_amdgcn_readfirstlane(lds_base)), "v"(voffset), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(soffset))
                : "memory");
 }
 __device__ __forceinline__ void load_word_to_lds(const i32x4& rsrc, uint32_t voffset, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
                :
                : "s"(lds_base), "v"(voffset), "s"(rsrc)
                : "memory");

@@ -1,8 +1,9 @@
 """What the compiler does not check in the built kernels.
 
 A scalar register that a vector instruction writes (``v_readfirstlane`` and its like) may be read by a memory instruction five wait states
-later at the earliest.  The compiler inserts them for its own instructions, not in front of inline assembly, and loads straight into LDS are
-inline assembly here: a descriptor, an offset or an LDS base that is read too early sends such a load somewhere else, now and then.
+later at the earliest; M0, which holds the LDS address of a load straight into LDS, is read one wait state after a scalar instruction wrote it.
+The compiler sees to both for its own instructions, not in front of inline assembly, and loads straight into LDS are inline assembly here: a
+descriptor, an offset or an LDS address that is read too early sends such a load somewhere else, now and then.
 """
 import os
 import re
@@ -63,6 +64,8 @@ def read_too_early(code):
                 continue
             seen.add((j, states))
             writer, given, _ = code[at[j]]
+            if writer.startswith("s_") and states < 1 and given[:1] == ["m0"]:
+                early.append(f"{address:#x} {opcode} {operands} right after {writer} {given}")
             if writer.startswith("v_") and any(scalars(o) & read for o in given[:2 if "_co_" in writer or "div_scale" in writer else 1]):
                 early.append(f"{address:#x} {opcode} {operands} {states} wait states after {writer} {given}")
             ways += [(p, states + (int(given[0], 0) + 1 if writer == "s_nop" else 1)) for p in before[j]]
@@ -85,6 +88,8 @@ def test_the_check_finds_what_it_looks_for():
     code, name = instructions(text)
     loads, early = read_too_early(code)
     assert (name, loads, [line.split()[0] for line in early]) == ("kernel", 3, ["0x100c", "0x1020"])
+    at_once = text.replace("s_mov_b32 m0, s4 ", "s_nop 4 ").replace("s_nop 2 ", "s_mov_b32 m0, s4 ")
+    assert "0x100c buffer_load_dword ['v1', 's[8:11]', '0', 'offen', 'lds'] right after s_mov_b32 ['m0', 's4']" in read_too_early(instructions(at_once)[0])[1]
     later = text.replace("s_nop 2 ", "s_nop 3 ")
     assert [line.split()[0] for line in read_too_early(instructions(later)[0])[1]] == ["0x1020"]
     back = later.replace("s7, v3", "s9, v3")  # (what the branch back leads to)
