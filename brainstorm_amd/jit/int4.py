@@ -55,8 +55,8 @@ def _empty_values(experts: int, rows: int, columns: int, device) -> torch.Tensor
 
 def pack_int4(values: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *, group: int = 128) -> Int4Weight:
     """Weights that are in 4 bits already: ``values`` uint8 ``[experts, out_features, in_features]`` of 0 .. 15, ``scales``
-    ``[experts, out_features, groups]`` and ``zeros`` (uint8, of the same shape; 8 without them), ``groups = ceil(in_features / group)``.
-    On the host or the device; a step of loading a model, not of running it."""
+    ``[experts, out_features, groups]`` (finite) and ``zeros`` (uint8, of the same shape; 8 without them), ``groups = ceil(in_features /
+    group)``.  On the host or the device; a step of loading a model, not of running it."""
     _check_group(group)
     if values.dim() != 3 or values.dtype != torch.uint8:
         raise RuntimeError("values must be a uint8 tensor [experts, out_features, in_features]")
@@ -69,6 +69,8 @@ def pack_int4(values: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.
         raise RuntimeError("zeros must be a uint8 tensor of the scales' shape")
     if values.numel() and int(values.max()) > 15:
         raise RuntimeError("values must be 0 .. 15")
+    if not bool(torch.isfinite(scales).all()):
+        raise RuntimeError("scales must be finite")
     packed = _empty_values(experts, rows, columns, values.device)
     for e in range(experts):
         _packed_values(values[e], packed[e])
@@ -80,7 +82,8 @@ def quantize_int4(weight: torch.Tensor, group: int = 128, *, zeros: bool = False
     """``weight`` (``[experts, out_features, in_features]``, fp32 / fp16 / bf16) rounded to 4 bits.  Over every ``group`` elements of a row
     ``scale = max(|w|) / 7`` and ``q = round(w / scale) + 8``, or with ``zeros`` ``scale = (max(w, 0) - min(w, 0)) / 15``, ``zero =
     round(-min(w, 0) / scale)`` and ``q = round(w / scale) + zero``, both held to 0 .. 15.  The scale is rounded to ``scale_dtype`` (the
-    weight's type) first; where it is zero, so is the group.  On the host or the device; a step of loading a model, not of running it."""
+    weight's type) first; where it is zero, so is the group.  Weights that are not finite, and groups whose scale ``scale_dtype`` cannot hold,
+    are refused.  On the host or the device; a step of loading a model, not of running it."""
     _check_group(group)
     if weight.dim() != 3 or weight.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise RuntimeError("weight must be an fp32, fp16 or bf16 tensor [experts, out_features, in_features]")
@@ -95,11 +98,15 @@ def quantize_int4(weight: torch.Tensor, group: int = 128, *, zeros: bool = False
     for e in range(experts):
         padded = torch.zeros(rows, groups * group, device=weight.device)
         padded[:, :columns] = weight[e].detach()
+        if not bool(torch.isfinite(padded).all()):
+            raise RuntimeError(f"weight of expert {e} holds values that are not finite")
         parts = padded.view(rows, groups, group)
         low = parts.amin(2).clamp(max=0.0) if columns else parts.new_zeros(rows, groups)
         high = parts.amax(2).clamp(min=0.0) if columns else low
         scales[e] = ((high - low) / 15.0 if zeros else torch.maximum(high, -low) / 7.0).to(scale_dtype)
         scale = scales[e].float()
+        if not bool(torch.isfinite(scale).all()):
+            raise RuntimeError(f"a group of expert {e} needs a scale beyond {scale_dtype}")
         by = torch.where(scale == 0.0, 1.0, scale)
         zero = torch.where(scale == 0.0, 0.0, (-low / by).round().clamp(0, 15)) if zeros else torch.full_like(scale, 8.0)
         if zeros:

@@ -180,6 +180,32 @@ def test_refusals_of_the_layout():
             call()
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_weights_and_scales_that_are_not_finite_are_refused(bad, zeros):
+    """They would come out as scales that are not finite, or as weights of any value in their place."""
+    for dtype in TYPES.values():
+        weight = normal(1, 3, 5, 72, dtype=dtype)
+        weight[2, 4, 71] = bad
+        with pytest.raises(RuntimeError, match="expert 2 holds values that are not finite"):
+            quantize_int4(weight, 32, zeros=zeros)
+        scales = torch.ones(2, 16, 2, dtype=dtype)
+        scales[1, 3, 1] = bad
+        with pytest.raises(RuntimeError, match="scales must be finite"):
+            pack_int4(torch.zeros(2, 16, 64, dtype=torch.uint8), scales, group=32)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_scales_beyond_their_type_are_refused(zeros):
+    weight = torch.zeros(2, 4, 64)
+    weight[1, 2, 5] = 15 * 65504.0
+    assert quantize_int4(weight, 32, zeros=zeros).scales.isfinite().all()
+    at_the_border = weight / 15 * (15 if zeros else 7)
+    assert float(quantize_int4(at_the_border, 32, zeros=zeros, scale_dtype=torch.float16).scales.max()) == 65504.0
+    with pytest.raises(RuntimeError, match="expert 1 needs a scale beyond torch.float16"):
+        quantize_int4(weight * 2, 32, zeros=zeros, scale_dtype=torch.float16)
+
+
 # ---------------------------------------------------------------------------------- the products
 SHAPES = [  # rows, in, out, experts, group
     (1, 8, 1, 1, 32), (1, 128, 16, 1, 128), (1, 2048, 512, 4, 128), (2, 136, 17, 3, 64), (5, 64, 40, 2, 32), (16, 256, 64, 1, 128), (17, 384, 33, 1, 32),
