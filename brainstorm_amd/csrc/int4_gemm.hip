@@ -9,9 +9,12 @@
 // lane is 1 KB in one piece, 16 rows of 128 columns, and word j of a lane its fragment of the j-th v_mfma_f32_16x16x32.  The four bits of a
 // weight as a byte are an e4m3 number, q * 2^-9, all sixteen of them (below 8 they are subnormal, from 8 on normal of the same
 // spacing), so that a word becomes a fragment of bf16 or fp16 in one shift, two masks and four conversions, exactly.  The rows stay in their
-// type; fp32 rows are split into three bf16 parts (8 bits each: all of them) and take three instructions.  A group's products are summed
+// type; fp32 rows are split into three bf16 parts (8 bits each: all of them, down to 2^-133) and take three instructions.  A group's products are summed
 // by the matrix unit on top of -z times its sum of x, which one more instruction with a constant fragment leaves in the
 // result's layout, and the group's sum is scaled in fp32 by one multiply-add.  So nothing but the result is rounded below fp32.
+//   Elements of the range of fp32 are multiplied by q * 2^-15: before the scale a group may add up to 128 * 255 times as much as its
+// largest element, which is then still within the range, and so are the sums of scaled groups whose results are.  The results are multiplied
+// by 2^15 where the bias is added; the matrix unit keeps subnormal numbers, and those products are whole multiples of 2^-148.
 //   The weight fragment is the first operand: a lane holds results of one row and four neighbouring columns.
 #include <algorithm>
 #include <type_traits>
@@ -44,17 +47,22 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-// Eight weights of a word, as the numbers 0 .. 15: the low halves of its bytes are elements 0 .. 3, the high ones 4 .. 7.
+// What weights are multiplied by, and the results of their products with rows of that type divided by.
+template <int XDT>
+constexpr float kWeightUnit = XDT == BRT_F16 ? 1.0f : 0x1p-15f;
+
+// Eight weights of a word, as the numbers 0 .. 15 in such units: the low halves of its bytes are elements 0 .. 3, the high ones 4 .. 7.
 template <int XDT>
 __device__ __forceinline__ auto weights_of(uint32_t word) {
+  constexpr float kUnit = 512.0f * kWeightUnit<XDT>;
   const int lo = static_cast<int>(word & 0x0f0f0f0fu), hi = static_cast<int>((word >> 4) & 0x0f0f0f0fu);
   if constexpr (XDT == BRT_F16) {
-    const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, true);
-    const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, true);
+    const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, kUnit, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, kUnit, true);
+    const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, kUnit, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, kUnit, true);
     return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
   } else {
-    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, true);
-    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, true);
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, kUnit, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, kUnit, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, kUnit, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, kUnit, true);
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
   }
 }
@@ -202,7 +210,7 @@ __global__ __launch_bounds__(W * 64) void int4_few_rows_kernel(Int4Args a) {
   for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   Weights minus_one;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) minus_one[i] = -1.0f;
+  for (int i = 0; i < 8; ++i) minus_one[i] = -kWeightUnit<XDT>;
   for (int kb = wave; kb < a.KB; kb += W) {
     u32x4 raw_w[NT], raw_x[4 * Part::kUnits];
     uint32_t raw_s[NT][kGroups], raw_z[NT][kGroups];
@@ -281,7 +289,7 @@ __global__ __launch_bounds__(W * 64) void int4_few_rows_kernel(Int4Args a) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) v[q] += s_part[w][j][r][c4 + q];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = activated_for(v[q] + bias[f][q], a.act, a.out_dtype);
+    for (int q = 0; q < 4; ++q) v[q] = activated_for(__builtin_fmaf(v[q], 1.0f / kWeightUnit<XDT>, bias[f][q]), a.act, a.out_dtype);
     const size_t to = static_cast<size_t>(at.row0) + r;
     if (a.out_dtype == BRT_F32) store_four<BRT_F32>(a, to, n, v);
     else if (a.out_dtype == BRT_F16) store_four<BRT_F16>(a, to, n, v);
@@ -459,7 +467,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void int4_tiles_kernel(Int4Args
   auto part_of = [&](int stage, int r0, int p) { return Part(reinterpret_cast<const u32x4*>(smem + (part_at[p] + stage) + r0 * kRow)); };
   W one;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) one[i] = 1.0f;
+  for (int i = 0; i < 8; ++i) one[i] = kWeightUnit<XDT>;
   auto sum_up = [&](int kb, int stage) {
     if (wave >= MT) return;
 #pragma unroll
@@ -558,7 +566,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void int4_tiles_kernel(Int4Args
       for (int i = 0; i < MT; ++i) {
         float v[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = activated_for<ACT, OUT>(acc[i][j][q] + bias[q]);
+        for (int q = 0; q < 4; ++q) v[q] = activated_for<ACT, OUT>(__builtin_fmaf(acc[i][j][q], 1.0f / kWeightUnit<XDT>, bias[q]));
         if (i * 16 + c16 < rows && n < a.N) store_four<OUT>(a, static_cast<size_t>(row0) + i * 16 + c16, n, v);
       }
     }

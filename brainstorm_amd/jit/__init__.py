@@ -106,8 +106,10 @@ def grouped_linear_int4(x: torch.Tensor, weight: Int4Weight, loads: torch.Tensor
                         row_entries: Optional[torch.Tensor] = None, entries_per_cell: int = 1) -> torch.Tensor:
     """:func:`grouped_linear` on 4-bit weights: ``out[s_e : s_e + loads[e]] = act(x[s_e : s_e + loads[e]] @ W_e^T + b_e)`` with an
     :class:`Int4Weight` (:func:`quantize_int4`, :func:`pack_int4`).  ``x`` (``[rows, in_features]``, fp32 / fp16 / bf16, in_features a
-    multiple of 8) is not rounded; a group's products are summed with fp32 accumulation, scaled in fp32 and summed in an order that the
-    shape fixes; bias (``[experts, out_features]``), activation and one rounding follow.
+    multiple of 8) is not rounded (but for fp32 elements whose last bits are below 2^-133); a group's products are summed with fp32
+    accumulation, scaled in fp32 and summed in an order that the shape fixes, whatever finite elements they are of: only a result beyond
+    its type is an infinity, and of bf16 and fp32 rows one below 2^-111 is off by up to 2^-135 an addition.  Bias (``[experts, out_features]``),
+    activation and one rounding follow.
 
     With ``row_entries`` (what ``route_by_path`` writes: 1-based entry ``t * k + j + 1`` of every row, ``k = entries_per_cell``) ``x`` is
     cell-major and row r is its cell ``(row_entries[r] - 1) // k``: no dispatch is needed.  A row without an entry is a row of zeros.

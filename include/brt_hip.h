@@ -561,7 +561,8 @@ int brt_hip_grouped_gemm_fp8_blocks(int E, int P, int N, int K, int out_dtype);
  *   w [E, ceil(N/16), ceil(K/128), 1024] bytes: byte 16 * (16 * g + r) + 4 * j + m of a block is row r of the tile, column 32 * j + 8 * g + m in its
  *   low and column + 4 in its high four bits.  scales (of scale_dtype) and zeros (bytes) [E, ceil(N/16), ceil(K/group), 16].  What stands behind
  *   the N-th row or K-th column does not count (scales there are finite).
- * Products are exact, sums fp32 in an order that the shape fixes, the result is rounded once.  K is a multiple of 8, x, w and scales are 16-byte
+ * Products are exact (but for what fp32 elements hold below 2^-133), sums fp32 in an order that the shape fixes and of any finite elements
+ *   within its range where the result is, the result is rounded once.  K is a multiple of 8, x, w and scales are 16-byte
  * aligned, zeros 4-byte; P below 2^24, N, K and E up to 2^28.  Loads below zero count as none, rows of experts behind the P-th do not exist.
  * The first call of a shape on a device has to happen outside graph capture.
  */
