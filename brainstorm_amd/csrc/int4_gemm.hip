@@ -315,23 +315,31 @@ long small_tiles(const Int4Args& a) {
 // rows; NT, W) 1 row 2048 -> 8192: 2, 8 4.7, 1, 16 6.3, 4, 4 6.9; 1 row 8192 -> 1024: 1, 16 6.4, 2, 8 8.9; 64 rows 4096 -> 4096: 4, 8 9.7, 2, 8
 // 12.4; 4 rows of 4 experts 4096 -> 4096: 2, 8 8.9, 4, 8 9.7; 48 rows of 8 1024 -> 4096: 2, 4 7.4, 4, 8 8.1, 2, 8 8.3; 128 rows of 32
 // 1024 -> 4096: 4, 2 16.0, 2, 4 18.7, 4, 8 19.9, 1, 8 27; 128 of 32 4096 -> 1024: 4, 8 16.5, 4, 4 18.2, 4, 2 25.
-template <int XDT, int GJ>
-int launch_few_rows(Int4Args& a, hipStream_t st) {
+struct FewRows {
+  int tiles, waves;  // NT, W
+};
+FewRows few_rows_of(const Int4Args& a) {
   const long tiles = small_tiles(a);
-  if (tiles < 384) {
-    if (a.KB >= 32 && tiles <= 256) return launch_few_rows<XDT, GJ, 1, 16>(a, st);
-    return launch_few_rows<XDT, GJ, 1, 8>(a, st);
-  }
+  if (tiles < 384) return {1, a.KB >= 32 && tiles <= 256 ? 16 : 8};
   // (about one row block to an expert: no other workgroup reads its weights)
   const bool alone = a.P <= 8l * a.E && (tiles <= 1024 || (tiles <= 2048 && a.KB < 32));
-  if (tiles < 640 || a.KB < 4 || alone) {
-    if (a.KB >= 8 && tiles <= 1024) return launch_few_rows<XDT, GJ, 2, 8>(a, st);
-    if (a.KB >= 4) return launch_few_rows<XDT, GJ, 2, 4>(a, st);
-    return launch_few_rows<XDT, GJ, 2, 2>(a, st);
+  if (tiles < 640 || a.KB < 4 || alone) return {2, a.KB >= 8 && tiles <= 1024 ? 8 : a.KB >= 4 ? 4 : 2};
+  if (a.KB >= 8 && tiles <= 2048) return {4, 8};
+  return {4, a.KB >= 16 || a.KB <= 4 || tiles <= 4096 ? 4 : 2};
+}
+template <int XDT, int GJ>
+int launch_few_rows(Int4Args& a, hipStream_t st) {
+  const FewRows by = few_rows_of(a);
+  switch (by.tiles * 100 + by.waves) {
+    case 116: return launch_few_rows<XDT, GJ, 1, 16>(a, st);
+    case 108: return launch_few_rows<XDT, GJ, 1, 8>(a, st);
+    case 208: return launch_few_rows<XDT, GJ, 2, 8>(a, st);
+    case 204: return launch_few_rows<XDT, GJ, 2, 4>(a, st);
+    case 202: return launch_few_rows<XDT, GJ, 2, 2>(a, st);
+    case 408: return launch_few_rows<XDT, GJ, 4, 8>(a, st);
+    case 404: return launch_few_rows<XDT, GJ, 4, 4>(a, st);
+    default: return launch_few_rows<XDT, GJ, 4, 2>(a, st);
   }
-  if (a.KB >= 8 && tiles <= 2048) return launch_few_rows<XDT, GJ, 4, 8>(a, st);
-  if (a.KB >= 16 || a.KB <= 4 || tiles <= 4096) return launch_few_rows<XDT, GJ, 4, 4>(a, st);
-  return launch_few_rows<XDT, GJ, 4, 2>(a, st);
 }
 
 // Row blocks of all experts (blocks of 1 << bits rows; at most `most`, which the host has made the grid for).
@@ -652,6 +660,14 @@ extern "C" int brt_hip_grouped_gemm_int4_kernel(int x_dtype, int T, int group, i
   a.entries = T >= 0 ? &kRoutes : nullptr;  // (whether there are any is all that is asked)
   a.T = T; a.E = E; a.P = P; a.N = N; a.K = K; a.KB = (K + kB - 1) / kB; a.tiles = (N + 15) / 16;
   return rows_kind(a, group, x_dtype);
+}
+
+extern "C" int brt_hip_grouped_gemm_int4_few_rows(int E, int P, int N, int K) {
+  if (E <= 0 || P <= 0 || N <= 0 || K <= 0) return BRT_E_INVALID;
+  Int4Args a{};
+  a.E = E; a.P = P; a.N = N; a.K = K; a.KB = (K + kB - 1) / kB; a.tiles = (N + 15) / 16;
+  const FewRows by = few_rows_of(a);
+  return by.tiles * 100 + by.waves;
 }
 
 extern "C" int brt_hip_grouped_gemm_int4(const void* x, int x_dtype, const int32_t* row_entries, int entries_per_cell, int T,
