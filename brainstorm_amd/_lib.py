@@ -166,7 +166,7 @@ SIGNATURES = {
          _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr],
     ),
     "brt_hip_grouped_gemm_int4_kernel": (_c_int, [_c_int] * 7),
-    "brt_hip_grouped_gemm_int4_few_rows": (_c_int, [_c_int] * 4),
+    "brt_hip_grouped_gemm_int4_few_rows": (_c_int, [_c_int] * 5),
     "brt_hip_grouped_gemm_fp8_blocks": (_c_int, [_c_int] * 5),
     "brt_hip_gate_topk_grad": (
         _c_int,

@@ -575,7 +575,7 @@ int brt_hip_grouped_gemm_int4(const void* x, int x_dtype, const int32_t* row_ent
 int brt_hip_grouped_gemm_int4_kernel(int x_dtype, int T, int group, int E, int P, int N, int K);
 /* ... and which form of the kernel for few rows takes them where that one does: 100 times the 16 columns that a workgroup has, plus its
  * wavefronts. */
-int brt_hip_grouped_gemm_int4_few_rows(int E, int P, int N, int K);
+int brt_hip_grouped_gemm_int4_few_rows(int x_dtype, int E, int P, int N, int K);
 
 /*
  * brt_hip_grouped_gemm / _f32out / _routed / _routed_f32out / _by_rows on fp32 rows of x (16-byte aligned), which the

@@ -91,16 +91,19 @@ def test_subnormal_elements_of_fp16(rows, k, n, experts, group):
 
 # ------------------------------------------------------------------------------- the kernel of few rows
 #: 100 times the 16 columns of a workgroup plus its wavefronts; rows, in, out, experts
-FORMS = [(116, 20, 4104, 100, 2), (108, 70, 1096, 520, 4), (208, 24, 1032, 1001, 8), (204, 40, 600, 1300, 16), (202, 300, 264, 520, 5),
+FORMS = [(116, 20, 4104, 100, 2), (108, 70, 1096, 520, 4), (208, 24, 1032, 1001, 8), (204, 20, 600, 500, 16), (202, 300, 264, 520, 5),
          (408, 130, 1032, 1300, 2), (404, 333, 776, 1001, 12), (402, 60, 904, 2100, 40)]
 
 
 def test_the_forms_below_are_reached():
     form = _lib.lib().brt_hip_grouped_gemm_int4_few_rows
-    assert form(0, 1, 1, 1) == form(1, 0, 1, 1) == form(1, 1, 0, 1) == form(1, 1, 1, 0) == -1
+    assert form(3, 1, 1, 1, 1) == form(2, 0, 1, 1, 1) == form(2, 1, 0, 1, 1) == form(2, 1, 1, 0, 1) == form(2, 1, 1, 1, 0) == -1
     for which, rows, k, n, experts in FORMS:
-        assert form(experts, rows, n, k) == which
+        assert all(form(code, experts, rows, n, k) == which for code in CODES.values())
         assert all(columns_of(dtype, rows, k, n, experts, group) == 16 for dtype in TYPES for group in (32, 64, 128))
+    # one row block to an expert: 32 columns a workgroup for 16-bit rows, 64 for fp32 ones, which every workgroup splits anew
+    for rows, k, n, experts, by16, by32 in ((24, 1792, 8192, 4, 204, 408), (72, 768, 512, 24, 204, 404), (16, 3584, 1000, 16, 208, 408)):
+        assert [form(code, experts, rows, n, k) for code in (2, 1, 0)] == [by16, by16, by32]
 
 
 @pytest.mark.gpu
