@@ -109,7 +109,8 @@ def grouped_linear_int4(x: torch.Tensor, weight: Int4Weight, loads: torch.Tensor
     multiple of 8) is not rounded (but for fp32 elements whose last bits are below 2^-133); a group's products are summed with fp32
     accumulation, scaled in fp32 and summed in an order that the shape fixes, whatever finite elements they are of: only a result beyond
     its type is an infinity, and of bf16 and fp32 rows one below 2^-111 is off by up to 2^-135 an addition.  Bias (``[experts, out_features]``),
-    activation and one rounding follow.
+    activation and one rounding follow.  GELU is a fit that is within 4.3e-6 of the erf form for 16-bit results (as in :func:`grouped_linear`), erf
+    in fp32 for fp32 ones.  Rows are fewer than 2^24, and ``rows * out_features`` stays below about 2^34 for fp32 rows, 2^36 for 16-bit ones.
 
     With ``row_entries`` (what ``route_by_path`` writes: 1-based entry ``t * k + j + 1`` of every row, ``k = entries_per_cell``) ``x`` is
     cell-major and row r is its cell ``(row_entries[r] - 1) // k``: no dispatch is needed.  A row without an entry is a row of zeros.

@@ -563,7 +563,9 @@ int brt_hip_grouped_gemm_fp8_blocks(int E, int P, int N, int K, int out_dtype);
  *   the N-th row or K-th column does not count (scales there are finite).
  * Products are exact (but for what fp32 elements hold below 2^-133), sums fp32 in an order that the shape fixes and of any finite elements
  *   within its range where the result is, the result is rounded once.  K is a multiple of 8, x, w and scales are 16-byte
- * aligned, zeros 4-byte; P below 2^24, N, K and E up to 2^28.  Loads below zero count as none, rows of experts behind the P-th do not exist.
+ * aligned, zeros 4-byte; P below 2^24, N, K and E up to 2^28, and a launch of 2^32 threads is refused (BRT_E_UNSUPPORTED): (P + 16 min(E, P)) * N
+ * from about 2^34 for fp32 rows, (P + 64 min(E, P)) * N from about 2^36 for 16-bit ones.  Loads below zero count as none, rows of experts
+ * behind the P-th do not exist.  GELU is the fit that brt_hip_grouped_gemm uses (4.3e-6 off the erf form at most) for 16-bit results, erf for fp32 ones.
  * The first call of a shape on a device has to happen outside graph capture.
  */
 int brt_hip_grouped_gemm_int4(const void* x, int x_dtype, const int32_t* row_entries, int entries_per_cell, int T,

@@ -329,3 +329,13 @@ def test_cells_up_to_two_gib_in_tiles(columns, n):
     got = grouped_linear_int4(x, w, loads, row_entries=entries)
     want = grouped_linear_int4(x[-rows:].flip(0), w, loads)
     assert torch.equal(got, want) and bool(want.any(1).all())
+
+
+def test_launches_of_too_many_threads_are_refused_without_a_gpu():
+    lib, some = _lib.lib(), 16  # an address that is never read: every call ends before a launch
+
+    def code(x_dtype, experts, rows, n, k):
+        return lib.brt_hip_grouped_gemm_int4(some, x_dtype, None, 1, 0, some, some, 2, None, 128, some, None, 0, some, x_dtype, experts, rows, n, k, 0, None)
+
+    for given in ((0, 8, 1 << 20, 1 << 14, 2048), (0, 1 << 22, 1 << 23, 1 << 8, 512), (2, 8, (1 << 24) - 1, 1 << 14, 2048), (1, 1 << 20, 1 << 22, 1 << 11, 1024)):
+        assert code(*given) == -4 and b"too many tiles" in lib.brt_hip_last_error(), given
