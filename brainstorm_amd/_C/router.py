@@ -690,8 +690,8 @@ def balance_loss(score: torch.Tensor, path_ids: torch.Tensor, counted: Optional[
     that count a loss is zero.
 
     The losses carry the gradient of ``score`` where gradients are recorded (counts have none), made in one launch; cells that do not
-    count have none, whatever they hold, and no gradients of these gradients.  A counted cell that holds NaN, or no score above -inf,
-    makes the losses NaN, as its softmax is.  At most 1024 paths."""
+    count have none, whatever they hold, and no gradients of these gradients.  A counted cell that holds NaN or +inf, or no score above
+    -inf, makes the losses NaN, as its softmax is.  At most 1024 paths."""
     return _lib.native().balance_loss(score, path_ids, counted)
 
 

@@ -45,7 +45,8 @@ struct BalanceArgs {
   int ls;  // log2 of the lanes that share a row
 };
 
-// exp(x) for x <= 0, within 2 + |x| steps of 2^-24: small exponents are exact to the last bits, where the large probabilities are
+// exp(x) for x <= 0, within 2 + 1.23 |x| steps of 2^-24 (the product's rounding is up to |x| of them, the constant's 0.22 |x|): small
+// exponents are exact to the last bits, where the large probabilities are
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2E); }
 
 // Column sums and what belongs to the batch -> the losses, the counts and the gradient's coefficients; by the whole workgroup.
