@@ -96,7 +96,7 @@ def quantize_int4(weight: torch.Tensor, group: int = 128, *, zeros: bool = False
     scales = torch.empty(experts, rows, groups, dtype=scale_dtype, device=weight.device)
     points = torch.empty(experts, rows, groups, dtype=torch.uint8, device=weight.device) if zeros else None
     for e in range(experts):
-        padded = torch.zeros(rows, groups * group, device=weight.device)
+        padded = torch.zeros(rows, groups * group, dtype=torch.float32, device=weight.device)
         padded[:, :columns] = weight[e].detach()
         if not bool(torch.isfinite(padded).all()):
             raise RuntimeError(f"weight of expert {e} holds values that are not finite")

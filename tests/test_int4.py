@@ -195,6 +195,21 @@ def test_weights_and_scales_that_are_not_finite_are_refused(bad, zeros):
             pack_int4(torch.zeros(2, 16, 64, dtype=torch.uint8), scales, group=32)
 
 
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float16, torch.float64])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantized_weights_do_not_depend_on_the_default_type(default, zeros):
+    weight = normal(1, 2, 33, 200) * 3e4
+    want = quantize_int4(weight, 64, zeros=zeros)
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        got = quantize_int4(weight, 64, zeros=zeros)
+        again = pack_int4(torch.zeros(2, 33, 200, dtype=torch.uint8), torch.ones(2, 33, 4, dtype=torch.float32), group=64)
+    finally:
+        torch.set_default_dtype(before)
+    assert all(a is b is None or torch.equal(a, b) for a, b in zip(got[:3], want[:3])) and got.scales.dtype == again.scales.dtype == torch.float32
+
+
 @pytest.mark.parametrize("zeros", [False, True])
 def test_scales_beyond_their_type_are_refused(zeros):
     weight = torch.zeros(2, 4, 64)
