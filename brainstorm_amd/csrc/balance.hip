@@ -10,10 +10,10 @@
 // once per workgroup and to memory as one vector of E per workgroup, which a second launch adds up (one launch, one workgroup, for
 // small batches).  No floating-point atomics: the order of every sum follows from the sizes.  Exponents are taken of s - max, so rows of the
 // type's lowest value have a softmax; a cell that does not count is read as zeros, whatever it holds.
-//   What bounds it (MI355X): 65536 x 128 bf16 10.4 us forward (16.8 MB, 1.6 TB/s), 6.0 to join 256 workgroups' sums and 13.0 backward (33.6
-// MB, 2.6 TB/s), where the bytes alone take 3.3 and 6.5: a launch, a round of loads and the exchanges along a row that follow one another (four
-// rows at a time hide part of them: the gradient takes 20.9 with one), vector instructions 0.32 and 0.23 of the time.  1024 x 16 fp32
-// 7.1 + 3.5, 4099 x 60 fp16 6.3 + 5.2 + 3.5 us: launches and dependent loads.
+//   What bounds it (MI355X, the least of 40 launches; their mean is up to 0.6 us more): 65536 x 128 bf16 10.4-10.8 us forward (16.8 MB, 1.6
+// TB/s), 6.0-6.2 to join 256 workgroups' sums and 13.0-13.4 backward (33.6 MB, 2.5 TB/s), where the bytes alone take 3.3 and 6.5: a launch, a
+// round of loads and the exchanges along a row that follow one another (four rows at a time hide part of them: the gradient takes 20.9 with one), vector instructions 0.32 and 0.23 of the time.  1024 x 16 fp32
+// 7.1 + 3.4, 4099 x 60 fp16 6.4 + 5.2 + 3.6 us: launches and dependent loads, and behind them a reduction whose end one thread adds up.
 #include <algorithm>
 
 #include "gate.hpp"

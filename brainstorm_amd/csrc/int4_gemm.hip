@@ -179,10 +179,10 @@ __device__ __forceinline__ const char* row_of(const Int4Args& a, int row) {
 // Few rows per expert: the weights are streamed once and set the time.  A workgroup takes 16 NT columns and 16 rows; its W
 // wavefronts take blocks of 128 columns in turn, weights and rows straight into the fragments' registers, and add up their sums through
 // LDS.  The rows are the first operand here: a lane holds results of one column, whose scale and zero point are one register each.
-//   256 rows of 64 experts 4096 -> 1024 30.1 us, 139 MB at 4.6 TB/s (a large copy's rate is 5.2): memory.  1 row 2048 -> 8192 4.5 us and 48
-// rows of 8 experts 1024 -> 4096 7.4 us, of which the bytes take 1.7 and 3.6: a launch, the loads and two dependent rounds of requests.
+//   (Back to back.)  256 rows of 64 experts 4096 -> 1024 30 us, 139 MB at 4.6 TB/s (a large copy's rate is 5.2): memory.  1 row 2048 -> 8192
+// 5.0 us and 48 rows of 8 experts 1024 -> 4096 7.4 us, of which the bytes take 1.7 and 3.6: a launch, the loads and two dependent rounds of requests.
 // Two blocks of a wavefront in flight instead of one, or two and four row blocks a workgroup, which share the weights, gained nothing.
-//   fp32 rows: 333 rows of 12 experts 776 -> 1001, groups of 32, 12.1 us: two rounds of requests as well, the rows' splitting
+//   fp32 rows: 333 rows of 12 experts 776 -> 1001, groups of 32, 12.5 us: two rounds of requests as well, the rows' splitting
 // (over again for every 16 NT columns) and three products in place of one between them; vector units 0.22 of the time, matrix units 0.06.
 template <int XDT, int GJ, int NT, int W>
 __global__ __launch_bounds__(W * 64) void int4_few_rows_kernel(Int4Args a) {
@@ -312,8 +312,8 @@ long small_tiles(const Int4Args& a) {
 }
 // Columns of a workgroup (16 NT) and wavefronts that share its K (W), by the tiles that there are to deal out and the blocks of K.  Few
 // tiles: as many wavefronts as possible on each; many: more columns to a wavefront, which fetches the rows once for all of them.  (us, bf16
-// rows; NT, W) 1 row 2048 -> 8192: 2, 8 4.7, 1, 16 6.3, 4, 4 6.9; 1 row 8192 -> 1024: 1, 16 6.4, 2, 8 8.9; 64 rows 4096 -> 4096: 4, 8 9.7, 2, 8
-// 12.4; 4 rows of 4 experts 4096 -> 4096: 2, 8 8.9, 4, 8 9.7; 48 rows of 8 1024 -> 4096: 2, 4 7.4, 4, 8 8.1, 2, 8 8.3; 128 rows of 32
+// rows; NT, W) 1 row 2048 -> 8192: 2, 8 5.0, 1, 16 6.6, 4, 4 8.1; 1 row 8192 -> 1024: 1, 16 6.4, 2, 8 8.9; 64 rows 4096 -> 4096: 4, 8 10.2, 2, 8
+// 13.1; 4 rows of 4 experts 4096 -> 4096: 2, 8 8.9, 4, 8 9.7; 48 rows of 8 1024 -> 4096: 2, 4 7.4, 4, 8 7.8, 2, 8 8.3; 128 rows of 32
 // 1024 -> 4096: 4, 2 16.0, 2, 4 18.7, 4, 8 19.9, 1, 8 27; 128 of 32 4096 -> 1024: 4, 8 16.5, 4, 4 18.2, 4, 2 25.
 struct FewRows {
   int tiles, waves;  // NT, W
@@ -363,7 +363,7 @@ __device__ __forceinline__ int count_blocks(const Int4Args& a, int bits, int mos
 // unpack and scale beside the matrix units, have no part in it.
 //   Two workgroups of 8 wavefronts fit a CU (125 registers, 66 KB), which hides the loads and the barrier: 64 x 256 tiles took four
 // wavefronts of twice the columns 76 us where these take 65 (4096 rows of 32 experts 1024 -> 4096), and as long as them where the matrix
-// units' power sets the time (16384 rows of 8 experts 4096 -> 4096, groups of 128: 575 us, 956 TFLOP/s).  There the products alone take
+// units' power sets the time (16384 rows of 8 experts 4096 -> 4096, groups of 128: 575 us, 956 TFLOP/s; 612 on another card).  There the products alone take
 // 357 us; without the unpacking and scaling the kernel takes as long as with them, without the loads 140 us less, without the sums and
 // their product 46 less (groups of 64, of which there are twice as many: 667 us in all).
 constexpr int kTileWaves = 8;
@@ -608,8 +608,8 @@ int launch_tiles(Int4Args& a, hipStream_t st) {
 // Which kernel takes 16-bit rows, by what each is estimated to take (us): few rows, or 64 x 128 and 64 x 256 tiles.  The first fetches the
 // weights again for every 16 rows, 5300 tiles of 16 x 16 x 128 a microsecond with the chip full; the others take a time per block of 128
 // columns, waiting for loads while there is a workgroup to a CU at most, multiplying beyond (us, groups of 128): 64 rows 4096 -> 4096
-// 9.7 and 33 / 43; 600 rows of 2 experts 4096 -> 4096 50 and 44 / 44; 1024 rows of 16 1024 -> 4096 32 and 24 / 23; 8192 of 64 2048 -> 2048 187
-// and 127 / 100.  (Over 400 shapes, 32 to 20000 rows of 1 to 64 experts, 512 to 8192 -> 256 to 8192, the choice takes 0.4 % longer in the mean than the
+// 10 and 31 / 43; 600 rows of 2 experts 4096 -> 4096 56 and 45 / 45; 1024 rows of 16 1024 -> 4096 33 and 25 / 24; 8192 of 64 2048 -> 2048 211
+// and 127 / 102.  (Over 400 shapes, 32 to 20000 rows of 1 to 64 experts, 512 to 8192 -> 256 to 8192, the choice takes 0.4 % longer in the mean than the
 // best of the three, 1.29 times at worst: 281 rows of 16 1024 -> 5120.)
 enum RowsKind { kFewRows = 16, kTiles128 = 128, kTiles256 = 256 };
 RowsKind rows_kind(const Int4Args& a, int group, int x_dtype) {
